@@ -25,6 +25,8 @@ FGMM_FLAG_ACCUMULATE = 1
 FGMM_FLAG_FORCE_GENERAL = 2
 FGMM_X_F32 = 0
 FGMM_X_BF16 = 1
+FGMM_REDUCE = {"none": 0, "sum": 1, "mean": 2}
+FGMM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 _ERRORS = {1: "invalid argument", 2: "workspace", 3: "unsupported shape",
            4: "CUDA error", 5: "unsupported device", 6: "device-side failure"}
@@ -82,6 +84,25 @@ def load():
         lib.fgmm_generate_iso_rows.argtypes = [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_i32,
                                                _c_ptr, _c_i32, ctypes.c_uint64, _c_ptr]
         lib.fgmm_generate_iso_rows.restype = ctypes.c_int
+        mat = [_c_ptr, _c_i64, _c_i64]
+        rows = mat + mat + [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32]
+        scratch = [_c_ptr, ctypes.c_size_t]
+        lib.fgmm_xent_workspace_bytes.argtypes = [ctypes.c_int, ctypes.c_int, _c_i64, _c_i32,
+                                                  _c_i32]
+        lib.fgmm_xent_workspace_bytes.restype = ctypes.c_size_t
+        lib.fgmm_xent_fwd.argtypes = [ctypes.c_int] + rows + [
+            _c_ptr, _c_ptr, ctypes.c_int, _c_ptr, _c_ptr] + scratch + [_c_ptr]
+        lib.fgmm_xent_bwd.argtypes = [ctypes.c_int] + rows + [
+            _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr] + scratch + [_c_ptr]
+        lib.fgmm_embed_fwd.argtypes = [ctypes.c_int] + mat + [
+            _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32, ctypes.c_float, _c_ptr, _c_ptr]
+        lib.fgmm_embed_workspace_bytes.argtypes = [_c_i64, _c_i32, _c_i32]
+        lib.fgmm_embed_workspace_bytes.restype = ctypes.c_size_t
+        lib.fgmm_embed_bwd.argtypes = [ctypes.c_int] + mat + [
+            _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32, ctypes.c_float, _c_ptr] + scratch + [
+            ctypes.c_uint, _c_ptr]
+        for name in ("fgmm_xent_fwd", "fgmm_xent_bwd", "fgmm_embed_fwd", "fgmm_embed_bwd"):
+            getattr(lib, name).restype = ctypes.c_int
         _lib = lib
         return lib
 
@@ -199,6 +220,97 @@ def generate_iso_rows(X: torch.Tensor, centres: torch.Tensor, seed: int, row0: i
                                           centres.data_ptr(), centres.shape[0],
                                           seed & 0xFFFFFFFFFFFFFFFF, stream))
     return X
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _scratch(device: torch.device, nbytes: int) -> torch.Tensor:
+    """A workspace of one call.  Unlike the E-step's, it is not kept: a call
+    that is captured into a graph gets memory of that graph's own pool, and
+    calls of several host threads on one stream never share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def xent_fwd(X: torch.Tensor, W: torch.Tensor, targets: torch.Tensor, bias, ignore_index: int,
+             reduction: str):
+    """fgmm_xent_fwd on torch's current stream: (loss rows, logZ rows, reduced,
+    count), the last two None for reduction "none".  Arguments as checked by
+    flash_vocab.linear_cross_entropy, X two-dimensional."""
+    lib = load()
+    dev = X.device
+    N, D = X.shape
+    V = W.shape[0]
+    code = FGMM_REDUCE[reduction]
+    kind = FGMM_TYPES[X.dtype]
+    with torch.cuda.device(dev):
+        loss = torch.empty(N, device=dev, dtype=torch.float32)
+        logZ = torch.empty(N, device=dev, dtype=torch.float32)
+        reduced = count = None
+        if code:
+            reduced = torch.empty((), device=dev, dtype=torch.float32)
+            count = torch.empty((), device=dev, dtype=torch.float32)
+        ws = _scratch(dev, lib.fgmm_xent_workspace_bytes(0, kind, N, V, D))
+        _check(lib.fgmm_xent_fwd(
+            kind, X.data_ptr(), X.stride(0), X.stride(1), W.data_ptr(), W.stride(0), W.stride(1),
+            _ptr(bias), targets.data_ptr(), ignore_index, N, V, D, loss.data_ptr(),
+            logZ.data_ptr(), code, _ptr(reduced), _ptr(count), ws.data_ptr(), ws.numel(),
+            torch.cuda.current_stream(dev).cuda_stream))
+    return loss, logZ, reduced, count
+
+
+def xent_bwd(X, W, targets, bias, ignore_index: int, logZ, dloss, count, dlogZ, want):
+    """fgmm_xent_bwd on torch's current stream: (dX, dW, dbias), None where
+    ``want`` is false.  dloss has one value per row, or one in all."""
+    lib = load()
+    dev = X.device
+    N, D = X.shape
+    V = W.shape[0]
+    kind = FGMM_TYPES[X.dtype]
+    with torch.cuda.device(dev):
+        dX = torch.empty(N, D, device=dev, dtype=X.dtype) if want[0] else None
+        dW = torch.empty(V, D, device=dev, dtype=X.dtype) if want[1] else None
+        dbias = torch.empty(V, device=dev, dtype=torch.float32) if want[2] else None
+        ws = _scratch(dev, lib.fgmm_xent_workspace_bytes(1, kind, N, V, D))
+        _check(lib.fgmm_xent_bwd(
+            kind, X.data_ptr(), X.stride(0), X.stride(1), W.data_ptr(), W.stride(0), W.stride(1),
+            _ptr(bias), targets.data_ptr(), ignore_index, N, V, D, logZ.data_ptr(), _ptr(dloss),
+            1 if dloss is not None and dloss.dim() else 0, _ptr(count), _ptr(dlogZ), _ptr(dX),
+            _ptr(dW), _ptr(dbias), ws.data_ptr(), ws.numel(),
+            torch.cuda.current_stream(dev).cuda_stream))
+    return dX, dW, dbias
+
+
+def embed_fwd(table, ids, scale: float, ignore_index: int) -> torch.Tensor:
+    """fgmm_embed_fwd on torch's current stream; ids is one-dimensional."""
+    lib = load()
+    dev = table.device
+    V, D = table.shape
+    N = ids.numel()
+    with torch.cuda.device(dev):
+        out = torch.empty(N, D, device=dev, dtype=table.dtype)
+        _check(lib.fgmm_embed_fwd(
+            FGMM_TYPES[table.dtype], table.data_ptr(), table.stride(0), table.stride(1),
+            ids.data_ptr(), ignore_index, N, V, D, scale, out.data_ptr(),
+            torch.cuda.current_stream(dev).cuda_stream))
+    return out
+
+
+def embed_bwd(dout, ids, scale: float, ignore_index: int, out, accumulate: bool) -> torch.Tensor:
+    """fgmm_embed_bwd on torch's current stream into ``out`` (V, D)."""
+    lib = load()
+    dev = dout.device
+    V, D = out.shape
+    N = ids.numel()
+    with torch.cuda.device(dev):
+        ws = _scratch(dev, lib.fgmm_embed_workspace_bytes(N, V, D))
+        _check(lib.fgmm_embed_bwd(
+            FGMM_TYPES[dout.dtype], dout.data_ptr(), dout.stride(0), dout.stride(1),
+            ids.data_ptr(), ignore_index, N, V, D, scale, out.data_ptr(), ws.data_ptr(),
+            ws.numel(), FGMM_FLAG_ACCUMULATE if accumulate else 0,
+            torch.cuda.current_stream(dev).cuda_stream))
+    return out
 
 
 def launch_count() -> int:

@@ -1,0 +1,103 @@
+// Shared by the vocabulary operators (fgmm_xent.cu, fgmm_embed.cu): element
+// types and their conversions, and the argument checks of the entry points.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include <exception>
+#include <string>
+
+#include "../../include/flashgmm.h"
+#include "fgmm_internal.cuh"
+
+namespace fgmm {
+
+constexpr int64_t kVocabMaxN = int64_t(1) << 30;
+constexpr int32_t kVocabMaxV = 1 << 30;
+constexpr int32_t kVocabMaxD = 1 << 16;
+
+inline int type_size(int type) { return type == FGMM_T_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// Calls f with a null pointer of the element type (a type tag).
+template <class F>
+decltype(auto) with_type(int type, F&& f) {
+  if (type == FGMM_T_BF16) return f(static_cast<__nv_bfloat16*>(nullptr));
+  if (type == FGMM_T_F16) return f(static_cast<__half*>(nullptr));
+  return f(static_cast<float*>(nullptr));
+}
+
+// FGMM_OK, or the status of a refused type or shape with its message recorded.
+inline int vocab_check_shape(const char* name, int type, int64_t N, int32_t V, int32_t D) {
+  char buf[200];
+  if (type != FGMM_T_F32 && type != FGMM_T_BF16 && type != FGMM_T_F16) {
+    snprintf(buf, sizeof buf, "%s: unknown type %d", name, type);
+    return entry_fail(FGMM_ERR_ARG, buf);
+  }
+  if (N < 0 || V < 1 || D < 1) {
+    snprintf(buf, sizeof buf, "%s: invalid shape N=%lld V=%d D=%d", name, (long long)N, V, D);
+    return entry_fail(FGMM_ERR_ARG, buf);
+  }
+  if (N >= kVocabMaxN || V >= kVocabMaxV || D > kVocabMaxD) {
+    snprintf(buf, sizeof buf, "%s: N=%lld V=%d D=%d exceeds the supported N < 2^30, V < 2^30, "
+             "D <= 65536", name, (long long)N, V, D);
+    return entry_fail(FGMM_ERR_UNSUPPORTED, buf);
+  }
+  return FGMM_OK;
+}
+
+// Negative strides and pointers that are not aligned to their elements.
+inline int vocab_check_array(const char* name, const char* what, const void* p, int size,
+                             int64_t s0, int64_t s1) {
+  if (s0 < 0 || s1 < 0)
+    return entry_fail(FGMM_ERR_ARG, std::string(name) + ": negative stride of " + what);
+  if (reinterpret_cast<uintptr_t>(p) % (unsigned)size)
+    return entry_fail(FGMM_ERR_ARG, std::string(name) + ": " + what +
+                                        " is not aligned to its elements");
+  return FGMM_OK;
+}
+
+inline int vocab_check_workspace(const char* name, const void* ws, size_t got, size_t need) {
+  if (need > 0 && (ws == nullptr || got < need || (reinterpret_cast<uintptr_t>(ws) & 255))) {
+    char buf[200];
+    snprintf(buf, sizeof buf, "%s: workspace of %zu bytes (256-byte aligned) required, got %zu at %p",
+             name, need, got, ws);
+    return entry_fail(FGMM_ERR_WORKSPACE, buf);
+  }
+  return FGMM_OK;
+}
+
+// Runs an entry point's body; no C++ exception crosses the C ABI.
+template <class F>
+int vocab_entry(const char* name, F&& body) noexcept {
+  try {
+    entry_fail(FGMM_OK, "");
+    return body();
+  } catch (const std::exception& e) {
+    try {
+      return entry_fail(FGMM_ERR_CUDA, std::string(name) + ": " + e.what());
+    } catch (...) {
+      return FGMM_ERR_CUDA;
+    }
+  } catch (...) {
+    return FGMM_ERR_CUDA;
+  }
+}
+
+}  // namespace fgmm

@@ -32,6 +32,7 @@ from typing import Callable, Iterable, Optional
 import torch
 
 import _fgmm_lib as L
+import flash_vocab as FV
 import gmm_stream as GS
 
 _VARIANT = {"iso": L.FGMM_VARIANT_ISO, "diag": L.FGMM_VARIANT_DIAG, "full": L.FGMM_VARIANT_FULL}
@@ -44,7 +45,10 @@ def init_params(X: torch.Tensor, K: int, covariance_type: str = "iso", seed: int
     g = torch.Generator(device="cpu")
     g.manual_seed(seed)
     idx = torch.randperm(N, generator=g)[:K].to(X.device)
-    mu = X[idx].float().clone()
+    if X.is_cuda and X.dtype in L.FGMM_TYPES and N < 2 ** 30:
+        mu = FV.embedding_lookup(X.detach(), idx).float()
+    else:
+        mu = X[idx].float().clone()
     dev = X.device
     if covariance_type == "iso":
         cov = torch.zeros(K, device=dev)

@@ -195,6 +195,86 @@ FGMM_API int fgmm_generate_iso_rows(float* X, const int64_t* row_ids, int64_t ro
                            int64_t nrows, int32_t D, const float* centres,
                            int32_t K, uint64_t seed, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators over a vocabulary: rows X (N, D) with one label each, against the
+ * V rows of a table W (V, D).  The labelled counterpart of the isotropic
+ * E-step: the same log-sum-exp of X W^T over the table without the N x V
+ * matrix, with a one-hot label where the E-step has responsibilities.  No
+ * counterpart in the reference.
+ *
+ *  - type is the element type of X and W and of their gradients (FGMM_T_*).
+ *    Sums, exponentials and normalisers are fp32; each stored gradient is
+ *    rounded once.
+ *  - X and W take element strides (>= 0; overlapping rows are fine, they are
+ *    read only).  Labels are int64; bias, loss, logZ, dloss, dlogZ and dbias
+ *    are float32; these, dX, dW, out and dtable are contiguous.
+ *  - A label equal to ignore_index leaves its row out: loss 0, logZ 0, no
+ *    gradient, and nothing of the row is used (its X may hold NaN).  Any
+ *    other label outside [0, V) makes that row's loss and every gradient it
+ *    would contribute to NaN.
+ *  - Workspaces are 256-byte aligned, as for the E-step; nothing in them has
+ *    to be initialised and nothing is kept in them between calls.  Results
+ *    are bitwise reproducible run to run.
+ *  - Limits: N < 2^30, V < 2^30, D <= 2^16.
+ * ------------------------------------------------------------------------- */
+#define FGMM_T_F32 0
+#define FGMM_T_BF16 1
+#define FGMM_T_F16 2
+
+#define FGMM_REDUCE_NONE 0
+#define FGMM_REDUCE_SUM 1
+#define FGMM_REDUCE_MEAN 2
+
+/* Bytes of workspace fgmm_xent_fwd (backward = 0) or fgmm_xent_bwd
+ * (backward = 1) needs for this shape, whatever the strides. */
+FGMM_API size_t fgmm_xent_workspace_bytes(int backward, int type, int64_t N, int32_t V,
+                                          int32_t D);
+
+/* S = X W^T + bias (bias may be NULL; -inf removes an entry),
+ *   logZ_n = log sum_v exp S_nv,   loss_n = logZ_n - S_{n, target_n}.
+ * loss and logZ (N) are always written.  With FGMM_REDUCE_SUM or _MEAN also
+ * *reduced = the sum of the losses, or their mean over the rows not ignored
+ * (NaN when there is none), and *count = the number of those rows. */
+FGMM_API int fgmm_xent_fwd(int type, const void* X, int64_t x_stride_n, int64_t x_stride_d,
+                  const void* W, int64_t w_stride_v, int64_t w_stride_d, const float* bias,
+                  const int64_t* targets, int64_t ignore_index,
+                  int64_t N, int32_t V, int32_t D,
+                  float* loss, float* logZ, int reduction, float* reduced, float* count,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradient of fgmm_xent_fwd.  With p_nv = exp(S_nv - logZ_n), recomputed in
+ * pieces of the vocabulary, and w_n = dloss_n (loss's gradient: N values, or
+ * one when dloss_stride is 0; divided by *count when count is not NULL):
+ *   g_nv = (w_n + dlogZ_n) p_nv - w_n [v = target_n]
+ *   dX = g W,   dW = g^T X,   dbias_v = sum_n g_nv
+ * dloss or dlogZ may be NULL (zero), and each of dX, dW, dbias that is NULL
+ * is not computed.  logZ is the forward call's. */
+FGMM_API int fgmm_xent_bwd(int type, const void* X, int64_t x_stride_n, int64_t x_stride_d,
+                  const void* W, int64_t w_stride_v, int64_t w_stride_d, const float* bias,
+                  const int64_t* targets, int64_t ignore_index,
+                  int64_t N, int32_t V, int32_t D, const float* logZ,
+                  const float* dloss, int64_t dloss_stride, const float* count,
+                  const float* dlogZ, void* dX, void* dW, float* dbias,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* out_i = scale * table[ids_i] (N, D); ids equal to ignore_index give a row
+ * of zeros, other ids outside [0, V) a row of NaN. */
+FGMM_API int fgmm_embed_fwd(int type, const void* table, int64_t t_stride_v, int64_t t_stride_d,
+                   const int64_t* ids, int64_t ignore_index, int64_t N, int32_t V, int32_t D,
+                   float scale, void* out, void* stream);
+
+FGMM_API size_t fgmm_embed_workspace_bytes(int64_t N, int32_t V, int32_t D);
+
+/* dtable_v = scale * sum over {i : ids_i = v} of dout_i, summed in fp32 over
+ * the sorted ids in an order that is the same on every run.  With
+ * FGMM_FLAG_ACCUMULATE the sum is added to dtable (rows that no id names are
+ * not touched); without it every row of dtable is written.  Ids equal to
+ * ignore_index or outside [0, V) contribute nothing. */
+FGMM_API int fgmm_embed_bwd(int type, const void* dout, int64_t d_stride_n, int64_t d_stride_d,
+                   const int64_t* ids, int64_t ignore_index, int64_t N, int32_t V, int32_t D,
+                   float scale, void* dtable, void* workspace, size_t workspace_bytes,
+                   unsigned flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,495 @@
+"""The vocabulary operators (flash_vocab) on the GPU against plain 64-bit forms,
+within bounds derived from the arithmetic (vocab_ref)."""
+
+import math
+
+import pytest
+import torch
+
+import _fgmm_lib as L
+import flash_gmm
+import flash_vocab as F
+import vocab_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, FH, FS = torch.bfloat16, torch.float16, torch.float32
+
+
+def check_xent(X, W, t, bias=None, *, reduction="none", wantgrad=True, seed=1, **kw):
+    """Forward and all gradients of a weighted sum of loss and logZ."""
+    N = t.numel()
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    w = (torch.rand(N, generator=g) + 0.5).to(DEV)
+    z = (0.25 * torch.rand(N, generator=g)).to(DEV)
+    leaves = [x.detach().clone(memory_format=torch.preserve_format).requires_grad_()
+              for x in (X, W)]
+    c = None if bias is None else bias.detach().clone().requires_grad_()
+    loss, logZ = F.linear_cross_entropy(leaves[0], leaves[1], t, c, reduction="none",
+                                        return_logZ=True, **kw)
+    ref = R.xent(X.reshape(-1, X.shape[-1]), W, t.reshape(-1), bias, w=w, dlogZ=z, **{
+        k.replace("ignore_index", "ignore"): v for k, v in kw.items()})
+    R.assert_within(loss.detach().reshape(-1), ref["loss"], ref["e_loss"], "loss")
+    R.assert_within(logZ.detach().reshape(-1), ref["logZ"], ref["e_logZ"], "logZ")
+    if wantgrad:
+        ((loss.reshape(-1) * w).sum() + (logZ.reshape(-1) * z).sum()).backward()
+        assert leaves[0].grad.dtype == X.dtype and leaves[1].grad.dtype == W.dtype
+        R.assert_within(leaves[0].grad.reshape(-1, X.shape[-1]), ref["dX"], ref["e_dX"], "dX")
+        R.assert_within(leaves[1].grad, ref["dW"], ref["e_dW"], "dW")
+        if c is not None:
+            R.assert_within(c.grad, ref["dbias"], ref["e_dbias"], "dbias")
+    return loss.detach(), logZ.detach(), leaves[0].grad, leaves[1].grad
+
+
+# N, V, D: one row, odd sizes, edges of the 64/128/256 tiles and one past them
+SHAPES = [(1, 1, 1), (1, 1000, 64), (3, 7, 5), (37, 501, 103), (128, 256, 64), (129, 257, 65),
+          (255, 300, 128), (257, 1024, 72), (300, 4099, 200), (513, 130, 1000), (700, 2049, 256)]
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,V,D", SHAPES)
+def test_xent_matches_64_bits(N, V, D, dtype):
+    X, W, t, c = R.problem(N, V, D, dtype, seed=N + V + D, ignored=0.2 if N > 30 else 0,
+                           bias=(N + D) % 2 == 1)
+    check_xent(X, W, t, c)
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,V,D", [(5, 70001, 96), (2500, 9001, 320), (9000, 600, 64)])
+def test_xent_larger(N, V, D, dtype):
+    X, W, t, c = R.problem(N, V, D, dtype, seed=7, ignored=0.3, bias=True)
+    check_xent(X, W, t, c)
+
+
+@pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+def test_xent_reductions(reduction, dtype):
+    X, W, t, c = R.problem(333, 555, 88, dtype, ignored=0.25, bias=True)
+    X.requires_grad_(), W.requires_grad_(), c.requires_grad_()
+    loss = F.linear_cross_entropy(X, W, t, c, reduction=reduction)
+    assert loss.shape == () and loss.dtype == torch.float32
+    (3.0 * loss).backward()
+    count = int((t != R.IGNORE).sum())
+    w = torch.full((333,), 3.0 / (count if reduction == "mean" else 1.0), device=DEV)
+    ref = R.xent(X, W, t, c, w=w)
+    scale = count if reduction == "mean" else 1.0
+    R.assert_within(loss.detach(), ref["loss"].sum() / scale,
+                    ref["e_loss"].sum() / scale + 2 ** -23 * ref["loss"].sum() / scale, "loss")
+    for got, name in ((X.grad, "dX"), (W.grad, "dW"), (c.grad, "dbias")):
+        R.assert_within(got, ref[name], ref["e_" + name] * (1 + 2 ** -20)
+                        + 2 ** -22 * ref[name].abs(), name)
+
+
+def test_xent_leading_dimensions_and_int32_targets():
+    X, W, t, _ = R.problem(60, 200, 40, BF)
+    a = F.linear_cross_entropy(X.view(3, 20, 40), W, t.view(3, 20).int(), reduction="none")
+    b = F.linear_cross_entropy(X, W, t, reduction="none")
+    assert a.shape == (3, 20) and torch.equal(a.reshape(-1), b)
+    one = F.linear_cross_entropy(X[0], W, t[0], reduction="none")
+    assert one.shape == () and abs((one - b[0]).item()) <= 1e-5 * max(1.0, float(b[0]))
+
+
+@pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("layout", ["transposed W", "transposed X", "odd row stride",
+                                    "column step", "offset base", "expanded X"])
+def test_xent_strides(layout, dtype):
+    X, W, t, c = R.problem(150, 333, 48, dtype, bias=True, seed=3)
+    if layout == "transposed W":
+        W = W.t().contiguous().t()
+    elif layout == "transposed X":
+        X = X.t().contiguous().t()
+    elif layout == "odd row stride":
+        X = torch.cat([X, X[:, :3]], 1)[:, :48]
+        W = torch.cat([W, W[:, :5]], 1)[:, :48]
+    elif layout == "column step":
+        X = torch.stack([X, X * 0 + 9], 2).reshape(150, 96)[:, ::2]
+        W = torch.stack([W, W * 0 + 9], 2).reshape(333, 96)[:, ::2]
+    elif layout == "offset base":
+        X = torch.cat([X.new_zeros(1), X.reshape(-1)])[1:].view(150, 48)
+        W = torch.cat([W.new_zeros(1), W.reshape(-1)])[1:].view(333, 48)
+    else:
+        X = X[:1].expand(150, 48)
+    Xl, Wl, cl = X.detach().requires_grad_(), W.detach().requires_grad_(), c.requires_grad_()
+    assert Xl.stride() == X.stride() and Wl.stride() == W.stride()
+    w = torch.rand(150, device=DEV) + 0.5
+    loss = F.linear_cross_entropy(Xl, Wl, t, cl, reduction="none")
+    got = torch.autograd.grad((loss * w).sum(), (Xl, Wl, cl))
+    ref = R.xent(X, W, t, c, w=w)
+    R.assert_within(loss.detach(), ref["loss"], ref["e_loss"], "loss")
+    for x, name in zip(got, ("dX", "dW", "dbias")):
+        R.assert_within(x, ref[name], ref["e_" + name], name)
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N", [100, 300])
+def test_xent_ignored_rows_may_hold_anything(N, dtype):
+    X, W, t, c = R.problem(N, 400, 72, dtype, ignored=0.4, bias=True)
+    dead = t == R.IGNORE
+    assert 0 < int(dead.sum()) < N
+    X[dead] = float("nan")
+    X[dead.nonzero()[0]] = float("inf")
+    X.requires_grad_(), W.requires_grad_(), c.requires_grad_()
+    loss, logZ = F.linear_cross_entropy(X, W, t, c, reduction="none", return_logZ=True)
+    assert not loss[dead].any() and not logZ[dead].any()
+    loss.sum().backward()
+    ref = R.xent(X, W, t, c, w=torch.ones(N, device=DEV))
+    R.assert_within(loss.detach(), ref["loss"], ref["e_loss"], "loss")
+    assert not X.grad[dead].any()
+    for got, name in ((X.grad, "dX"), (W.grad, "dW"), (c.grad, "dbias")):
+        R.assert_within(got, ref[name], ref["e_" + name], name)
+
+
+@pytest.mark.parametrize("N", [0, 5, 300])
+def test_xent_no_live_rows(N):
+    X = torch.full((N, 24), float("nan"), device=DEV, dtype=BF, requires_grad=True)
+    W = torch.randn(50, 24, device=DEV).to(BF).requires_grad_()
+    c = torch.zeros(50, device=DEV, requires_grad=True)
+    t = torch.full((N,), R.IGNORE, device=DEV)
+    assert math.isnan(F.linear_cross_entropy(X, W, t, c).item())
+    loss = F.linear_cross_entropy(X, W, t, c, reduction="sum")
+    assert loss.item() == 0.0
+    loss.backward()
+    for g in (X.grad, W.grad, c.grad):
+        assert not g.any()
+    mean = F.linear_cross_entropy(X, W, t, c)
+    for g in torch.autograd.grad(mean, (X, W, c)):
+        assert not g.any()
+
+
+@pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("N", [70, 400])
+def test_xent_label_outside_the_table_is_nan(N, dtype):
+    X, W, t, _ = R.problem(N, 300, 32, dtype)
+    t[3], t[N - 1] = 300, -7
+    X.requires_grad_(), W.requires_grad_()
+    loss = F.linear_cross_entropy(X, W, t, reduction="none")
+    bad = torch.zeros(N, dtype=torch.bool, device=DEV)
+    bad[3] = bad[N - 1] = True
+    assert torch.equal(torch.isnan(loss), bad)
+    loss.sum().backward()
+    assert torch.equal(torch.isnan(X.grad).any(1), bad) and bool(torch.isnan(W.grad).all())
+
+
+def test_xent_ignore_index_inside_the_table():
+    X, W, t, c = R.problem(90, 40, 16, FH, bias=True)
+    check_xent(X, W, t % 4, c, ignore_index=2)
+
+
+@pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
+def test_xent_removed_entries(dtype):
+    X, W, t, c = R.problem(140, 700, 64, dtype, bias=True)
+    gone = torch.zeros(700, dtype=torch.bool, device=DEV)
+    gone[200:650] = True                 # whole tiles of the vocabulary among it
+    gone[t] = False
+    c[gone] = float("-inf")
+    _, _, _, dW = check_xent(X, W, t, c)
+    assert not dW[gone].any()
+    # the type's lowest value instead of -inf: the same removal, without a NaN
+    lowest = torch.where(gone, torch.full_like(c, torch.finfo(torch.float32).min), c)
+    a = F.linear_cross_entropy(X, W, t, lowest, reduction="none")
+    b = F.linear_cross_entropy(X, W, t, c, reduction="none")
+    assert torch.equal(a, b)
+
+
+def test_xent_every_entry_removed():
+    X, W, t, c = R.problem(9, 300, 16, BF, bias=True)
+    c[:] = float("-inf")
+    loss, logZ = F.linear_cross_entropy(X, W, t, c, reduction="none", return_logZ=True)
+    assert bool((logZ == -math.inf).all()) and bool(torch.isnan(loss).all())
+    c[:] = torch.finfo(torch.float32).min    # all equal: a uniform distribution, up to fp32 steps
+    loss, logZ = F.linear_cross_entropy(X, W, t, c, reduction="none", return_logZ=True)
+    assert bool((logZ == torch.finfo(torch.float32).min).all()) and not loss.any()
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+def test_xent_large_logits(dtype):
+    """Logits of several hundred: exp alone would overflow; peaked rows."""
+    X, W, t, _ = R.problem(64, 500, 64, dtype, spread=60.0)
+    check_xent(X, W, t)
+
+
+def test_xent_small_and_uneven_weights():
+    """fp16 gradients of weights that span 2^-20 .. 1 within one call."""
+    X, W, t, _ = R.problem(200, 300, 32, FH)
+    X.requires_grad_(), W.requires_grad_()
+    w = torch.exp2(-20 * torch.rand(200, device=DEV))
+    (F.linear_cross_entropy(X, W, t, reduction="none") * w).sum().backward()
+    ref = R.xent(X, W, t, None, w=w)
+    R.assert_within(X.grad, ref["dX"], ref["e_dX"], "dX")
+    R.assert_within(W.grad, ref["dW"], ref["e_dW"], "dW")
+
+
+def test_xent_gradient_by_differences():
+    X, W, t, c = R.problem(20, 60, 24, FS, bias=True, seed=5)
+    X.requires_grad_(), W.requires_grad_(), c.requires_grad_()
+    F.linear_cross_entropy(X, W, t, c, reduction="sum").backward()
+    h = 2.0 ** -6
+    for leaf in (X, W, c):
+        U = torch.randn_like(leaf)
+        U /= U.norm()
+        old = leaf.data.clone()
+        leaf.data = old + h * U
+        up = F.linear_cross_entropy(X, W, t, c, reduction="sum").item()
+        leaf.data = old - h * U
+        down = F.linear_cross_entropy(X, W, t, c, reduction="sum").item()
+        leaf.data = old
+        # sums of 20 losses below 2^8 are off by at most 2^-17 each way; the difference
+        # quotient by h^2 times a third derivative, which a step of norm 1 in logits of
+        # rows |x|, |w| < 16 keeps below 16^3 / 6 on its few rows
+        assert abs((up - down) / (2 * h) - float((leaf.grad * U).sum())) \
+            <= 2.0 ** -17 / h + h * h * 16 ** 3 / 6
+
+
+def test_xent_only_what_is_asked():
+    X, W, t, c = R.problem(50, 80, 16, BF, bias=True)
+    for k in range(3):
+        leaves = [x.detach().clone().requires_grad_(i == k) for i, x in enumerate((X, W, c))]
+        F.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2]).backward()
+        assert [x.grad is not None for x in leaves] == [i == k for i in range(3)]
+    with torch.no_grad():
+        assert not F.linear_cross_entropy(X, W, t, c).requires_grad
+
+
+def test_xent_same_bits_every_run():
+    X, W, t, c = R.problem(3000, 5000, 136, BF, ignored=0.1, bias=True)
+    X.requires_grad_(), W.requires_grad_(), c.requires_grad_()
+    runs = []
+    for _ in range(3):
+        loss = F.linear_cross_entropy(X, W, t, c)
+        runs.append((loss.detach(), *torch.autograd.grad(loss, (X, W, c))))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+def test_xent_other_stream_and_two_at_once():
+    X, W, t, _ = R.problem(500, 3000, 128, BF)
+    X2, W2, t2, _ = R.problem(400, 2500, 96, BF, seed=9)
+    want, want2 = (F.linear_cross_entropy(*p, reduction="none") for p in ((X, W, t), (X2, W2, t2)))
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            a = F.linear_cross_entropy(X, W, t, reduction="none")
+        with torch.cuda.stream(s2):
+            b = F.linear_cross_entropy(X2, W2, t2, reduction="none")
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want2)
+
+
+def test_training_step_captured_into_graphs():
+    """Lookup, loss and both gradients, captured twice and replayed on new data."""
+    X, W, t, _ = R.problem(300, 700, 64, BF, ignored=0.1)
+    ids = torch.randint(0, 700, (300,), device=DEV)
+
+    def step(X, W, t, ids):
+        rows = F.embedding_lookup(W, ids, scale=8.0)
+        loss = F.linear_cross_entropy(X + rows, W, t)
+        return loss.detach(), *torch.autograd.grad(loss, (X, W))
+
+    graphs = []
+    side = torch.cuda.Stream()
+    for _ in range(2):
+        a = [X.detach().clone().requires_grad_(), W.detach().clone().requires_grad_(), t.clone(),
+             ids.clone()]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*a)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(*a)
+        graphs.append((g, a, out))
+    for k, (g, a, out) in enumerate(graphs):
+        with torch.no_grad():
+            a[0].copy_(X.flip(0) if k else X * 0.5)
+            a[2].copy_(t.flip(0) if k else t)
+    for g, _, _ in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for _, a, out in graphs:
+        want = step(*[x.detach().clone().requires_grad_(x.is_floating_point()) for x in a])
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+def test_tied_table_step():
+    """Lookup, loss, and both ends' gradients of one table added in place."""
+    V, D, N = 900, 80, 350
+    X, W, t, _ = R.problem(N, V, D, FS, ignored=0.1)
+    ids = torch.randint(0, V, (N,), device=DEV)
+    W.requires_grad_()
+    rows = F.embedding_lookup(W, ids, scale=0.5)
+    h = (rows + X).detach().requires_grad_()
+    loss = F.linear_cross_entropy(h, W, t)
+    dh, dW = torch.autograd.grad(loss, (h, W))
+    total = F.embedding_grad(dh, ids, V, scale=0.5, out=dW.clone(), accumulate=True)
+    # the same through autograd, both ends at once
+    loss2 = F.linear_cross_entropy(F.embedding_lookup(W, ids, scale=0.5) + X, W, t)
+    auto, = torch.autograd.grad(loss2, W)
+    extra, bound = R.embed_grad(dh, ids, V, 0.5)
+    assert torch.equal(loss, loss2)
+    want = dW.double() + extra
+    R.assert_within(total, want, bound + 2 ** -23 * (want.abs() + dW.double().abs()), "tied")
+    R.assert_within(auto, want, bound + 2 ** -22 * (want.abs() + dW.double().abs()), "autograd")
+
+
+def test_xent_logz_is_the_estep():
+    """W = mu, bias = log pi - |mu|^2/2: logZ and the gradients of its sum are the
+    isotropic E-step's logZ, mu_acc and Nk at unit variance."""
+    g = torch.Generator().manual_seed(2)
+    N, K, D = 3000, 200, 48
+    mu = torch.randn(K, D, generator=g).to(DEV)
+    X = (mu[torch.randint(0, K, (N,), generator=g).to(DEV)]
+         + torch.randn(N, D, generator=g).to(DEV))
+    lpi = torch.log_softmax(torch.randn(K, generator=g), 0).to(DEV)
+    logZ, Nk, mu_acc, _ = flash_gmm.flash_gmm_estep(X, mu, torch.zeros(K, device=DEV), lpi)
+    W = mu.clone().requires_grad_()
+    c = (lpi - 0.5 * mu.double().square().sum(1)).float().requires_grad_()
+    t = torch.zeros(N, dtype=torch.int64, device=DEV)
+    _, z = F.linear_cross_entropy(X, W, t, c, reduction="none", return_logZ=True)
+    shift = 0.5 * X.double().square().sum(1) + 0.5 * D * math.log(2 * math.pi)
+    off = ((z.detach().double() - shift) - logZ.double()).abs().max()
+    # each side is held to 1e-5 of max(1, |logZ|); z is |x|^2/2 larger at most
+    assert off.item() <= 1e-5 * (logZ.abs().max().item() + shift.max().item())
+    z.sum().backward()
+    for got, want in ((W.grad, mu_acc), (c.grad, Nk)):
+        assert float((got - want).abs().max()) <= 2e-4 * float(want.abs().max())
+
+
+# ---------------------------------------------------------------- embedding
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 1000, 64), (7, 3, 5), (300, 50, 129),
+                                   (2048, 256, 72), (2049, 70000, 33), (5000, 4097, 264),
+                                   (40000, 300, 16), (1500, 65536, 1000)])
+def test_embedding_matches_64_bits(N, V, D, dtype):
+    g = torch.Generator().manual_seed(N + V)
+    table = torch.randn(V, D, generator=g).to(dtype).to(DEV).requires_grad_()
+    # half of the ids from a few rows: long runs beside single ids and empty rows
+    ids = torch.where(torch.rand(N, generator=g) < 0.5, torch.randint(0, min(V, 3), (N,), generator=g),
+                      torch.randint(0, V, (N,), generator=g)).to(DEV)
+    if N > 100:
+        ids[::17] = R.IGNORE
+    dout = torch.randn(N, D, generator=g).to(dtype).to(DEV)
+    out = F.embedding_lookup(table, ids, scale=0.7)
+    keep = (ids != R.IGNORE)[:, None]
+    want = torch.where(keep, table.detach().double()[ids.clamp_min(0)] * 0.7, 0.0)
+    u = R.U[dtype]
+    R.assert_within(out.detach(), want, (u + 2 ** -22) * want.abs() + R.TINY[dtype], "lookup")
+    out.backward(dout)
+    ref, bound = R.embed_grad(dout, ids, V, 0.7)
+    R.assert_within(table.grad, ref, bound, "dtable")
+    again = F.embedding_grad(dout, ids, V, scale=0.7)
+    assert torch.equal(again, table.grad)
+
+
+@pytest.mark.parametrize("layout", ["transposed", "odd row stride", "offset base"])
+def test_embedding_strides(layout):
+    table, dout = torch.randn(90, 40, device=DEV), torch.randn(200, 40, device=DEV).to(BF)
+    ids = torch.randint(0, 90, (200,), device=DEV)
+    if layout == "transposed":
+        a, d = table.t().contiguous().t(), dout.t().contiguous().t()
+    elif layout == "odd row stride":
+        a, d = torch.cat([table, table[:, :1]], 1)[:, :40], torch.cat([dout, dout[:, :1]], 1)[:, :40]
+    else:
+        a = torch.cat([table.new_zeros(1), table.reshape(-1)])[1:].view(90, 40)
+        d = torch.cat([dout.new_zeros(1), dout.reshape(-1)])[1:].view(200, 40)
+    assert torch.equal(F.embedding_lookup(a, ids.view(10, 20)), table[ids].view(10, 20, 40))
+    assert torch.equal(F.embedding_grad(d, ids, 90), F.embedding_grad(dout, ids, 90))
+
+
+def test_embedding_bad_ids():
+    table = torch.randn(20, 8, device=DEV, requires_grad=True)
+    ids = torch.tensor([3, 20, -1, -100, 19], device=DEV)
+    out = F.embedding_lookup(table, ids)
+    assert torch.isnan(out[1:3]).all() and not out[3].any()
+    assert torch.equal(out[[0, 4]], table[[3, 19]])
+    dtable = F.embedding_grad(torch.ones(5, 8, device=DEV), ids, 20)
+    want = torch.zeros(20, 8, device=DEV)
+    want[3] = want[19] = 1
+    assert torch.equal(dtable, want)
+
+
+def test_embedding_ignore_index_inside_the_table():
+    table = torch.randn(20, 8, device=DEV, requires_grad=True)
+    ids = torch.tensor([0, 5, 0, 6], device=DEV)
+    out = F.embedding_lookup(table, ids, ignore_index=0)
+    assert not out[[0, 2]].any()
+    out.sum().backward()
+    assert not table.grad[0].any() and bool((table.grad[5] == 1).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
+def test_embedding_accumulate_leaves_other_rows(dtype):
+    V, D, N = 500, 72, 90
+    ids = torch.randint(0, 40, (N,), device=DEV)
+    dout = torch.randn(N, D, device=DEV).to(dtype)
+    old = torch.randn(V, D, device=DEV).to(dtype)
+    old[100] = float("nan")
+    got = F.embedding_grad(dout, ids, V, out=old.clone(), accumulate=True)
+    assert torch.equal(got[101:], old[101:]) and bool(torch.isnan(got[100]).all())
+    ref, bound = R.embed_grad(dout, ids, V, 1.0)
+    want = old[:100].double() + ref[:100]
+    touched = torch.bincount(ids, minlength=V)[:100, None] > 0
+    R.assert_within(got[:100], want, torch.where(
+        touched, bound[:100] + (R.U[dtype] + 2 ** -23) * (want.abs() + old[:100].double().abs()),
+        torch.zeros_like(want)), "accumulated")
+
+
+def test_embedding_empty_calls():
+    table = torch.randn(20, 8, device=DEV, requires_grad=True)
+    out = F.embedding_lookup(table, torch.zeros(0, 3, dtype=torch.int64, device=DEV))
+    assert out.shape == (0, 3, 8)
+    out.sum().backward()
+    assert not table.grad.any()
+    keep = torch.ones(20, 8, device=DEV)
+    F.embedding_grad(torch.zeros(0, 8, device=DEV), torch.zeros(0, dtype=torch.int64, device=DEV),
+                     20, out=keep, accumulate=True)
+    assert bool((keep == 1).all())
+
+
+def test_embedding_one_id_many_times():
+    """One id 30,000 times beside a few others: the longest run and its neighbours."""
+    N, D = 30011, 40
+    ids = torch.full((N,), 11, device=DEV)
+    ids[::1000] = torch.arange(len(ids[::1000]), device=DEV)
+    dout = torch.randn(N, D, device=DEV)
+    ref, bound = R.embed_grad(dout, ids, 64, 1.0)
+    R.assert_within(F.embedding_grad(dout, ids, 64), ref, bound, "dtable")
+
+
+def test_tables_longer_than_32_bit_offsets():
+    """V * D > 2^31 elements: rows and columns at the far end."""
+    V, D = 1_200_000, 2048
+    table = torch.empty(V, D, device=DEV, dtype=BF)
+    for i in range(0, V, 100_000):
+        table[i:i + 100_000] = torch.randn(1, D, device=DEV) * 0.02
+    table[V - 3:] = torch.randn(3, D, device=DEV) * 0.05
+    ids = torch.tensor([V - 1, 0, V - 2, 600_000, V - 1], device=DEV)
+    assert torch.equal(F.embedding_lookup(table, ids), table[ids])
+    X = table[ids[:3]].float().mul(4).to(BF)
+    loss, logZ = F.linear_cross_entropy(X, table, ids[:3], reduction="none", return_logZ=True)
+    S = torch.cat([X.double() @ table[i:i + 100_000].double().t() for i in range(0, V, 100_000)], 1)
+    want = torch.logsumexp(S, 1)
+    assert float((logZ.double() - want).abs().max()) < 1e-3
+    assert float((loss.double() - (want - S[[0, 1, 2], ids[:3]])).abs().max()) < 1e-3
+    g = torch.randn(5, D, device=DEV).to(BF)
+    d = F.embedding_grad(g, ids, V)
+    assert torch.equal(d[V - 1], (g[0].float() + g[4].float()).to(BF))
+    assert torch.equal(d[600_000], g[3]) and not d[V - 3].any()
+
+
+def test_launches_are_the_librarys():
+    before = L.launch_count()
+    X, W, t, _ = R.problem(20, 30, 8, BF)
+    F.linear_cross_entropy(X, W, t)
+    F.embedding_lookup(W, t)
+    assert L.launch_count() >= before + 3
+
+
+@pytest.mark.parametrize("dtype", [FS, BF, torch.float64], ids=["fp32", "bf16", "fp64"])
+def test_init_params_rows_are_unchanged(dtype):
+    import gmm_em
+    X = torch.randn(5000, 24, device=DEV).to(dtype)
+    for Y in (X, X.t().contiguous().t()):
+        mu, _, _ = gmm_em.init_params(Y, 64, seed=3)
+        idx = torch.randperm(5000, generator=torch.Generator().manual_seed(3))[:64].to(DEV)
+        assert mu.dtype == torch.float32 and torch.equal(mu, X[idx].float())

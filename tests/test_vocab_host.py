@@ -1,0 +1,128 @@
+"""The vocabulary operators' refusals, without a GPU: argument checks of
+flash_vocab and of the C entries (validated before any device call)."""
+
+import ctypes
+
+import pytest
+import torch
+
+import _fgmm_lib as L
+import flash_vocab as F
+import vocab_ref as R
+
+X, W, T = torch.zeros(4, 8), torch.zeros(5, 8), torch.zeros(4, dtype=torch.int64)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import os
+    if not os.path.exists(L.LIB_PATH):
+        import build_lib
+        build_lib.build()
+    return L.load()
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda: F.linear_cross_entropy(X, W, T), "must be on GPU"),
+    (lambda: F.linear_cross_entropy(X, W, T, reduction="avg"), "reduction"),
+    (lambda: F.linear_cross_entropy(X, torch.zeros(5, 7), T), r"X must be \(\.\.\., D\)"),
+    (lambda: F.linear_cross_entropy(X, torch.zeros(8), T), r"W \(V, D\)"),
+    (lambda: F.linear_cross_entropy(torch.tensor(1.0), W, T), r"X must be"),
+    (lambda: F.linear_cross_entropy(X, torch.zeros(0, 8), T), "must not be empty"),
+    (lambda: F.linear_cross_entropy(torch.zeros(4, 0), torch.zeros(5, 0), T), "must not be empty"),
+    (lambda: F.linear_cross_entropy(X, W, T[:3]), r"targets must be \(4,\)"),
+    (lambda: F.linear_cross_entropy(X, W, T.float()), "int64 or int32"),
+    (lambda: F.linear_cross_entropy(X.double(), W.double(), T), "float32, bfloat16 or float16"),
+    (lambda: F.linear_cross_entropy(X.bfloat16(), W, T), "one type"),
+    (lambda: F.linear_cross_entropy(X, W, T, torch.zeros(4)), r"bias must be \(5,\)"),
+    (lambda: F.linear_cross_entropy(X, W, T, torch.zeros(5, dtype=torch.int64)), "floating point"),
+    (lambda: F.embedding_lookup(W, T), "must be on GPU"),
+    (lambda: F.embedding_lookup(W[0], T), r"table must be \(V, D\)"),
+    (lambda: F.embedding_lookup(W[:0], T), "not empty"),
+    (lambda: F.embedding_lookup(W.double(), T), "float32, bfloat16 or float16"),
+    (lambda: F.embedding_lookup(W, T.float()), "int64 or int32"),
+    (lambda: F.embedding_grad(X, T, 5), "must be on GPU"),
+    (lambda: F.embedding_grad(X, T[:2], 5), r"ids must be \(4,\)"),
+    (lambda: F.embedding_grad(X, T, 0), "must be positive"),
+    (lambda: F.embedding_grad(X, T, 5, accumulate=True), "needs the out= buffer"),
+])
+def test_refusals(call, match):
+    with pytest.raises(ValueError, match=match):
+        call()
+
+
+class C:
+    """One entry's arguments by name, valid ones for pointers that are never read."""
+    XENT = dict(type=1, X=256, sxn=8, sxd=1, W=256, swv=8, swd=1, bias=None, targets=256,
+                ignore=-100, N=4, V=5, D=8)
+    FWD = dict(XENT, loss=256, logZ=256, reduction=0, reduced=None, count=None, ws=256, nws=1 << 40,
+               stream=None)
+    BWD = dict(XENT, logZ=256, dloss=256, ds=1, count=None, dlogZ=None, dX=256, dW=256, dbias=None,
+               ws=256, nws=1 << 40, stream=None)
+    EFWD = dict(type=1, table=256, tsv=8, tsd=1, ids=256, ignore=-100, N=4, V=5, D=8, scale=1.0,
+                out=256, stream=None)
+    EBWD = dict(type=1, dout=256, dsn=8, dsd=1, ids=256, ignore=-100, N=4, V=5, D=8, scale=1.0,
+                dtable=256, ws=256, nws=1 << 40, flags=0, stream=None)
+
+
+@pytest.mark.parametrize("entry,args,change,code,match", [
+    (e, a, ch, code, m)
+    for e, a in (("fgmm_xent_fwd", C.FWD), ("fgmm_xent_bwd", C.BWD),
+                 ("fgmm_embed_fwd", C.EFWD), ("fgmm_embed_bwd", C.EBWD))
+    for ch, code, m in (
+        (dict(type=3), 1, "unknown type"), (dict(N=-1), 1, "invalid shape"),
+        (dict(V=0), 1, "invalid shape"), (dict(D=0), 1, "invalid shape"),
+        (dict(N=1 << 30), 3, "exceeds"), (dict(V=1 << 30), 3, "exceeds"),
+        (dict(D=65537), 3, "exceeds"))
+] + [
+    ("fgmm_xent_fwd", C.FWD, dict(X=None), 1, "null pointer"),
+    ("fgmm_xent_fwd", C.FWD, dict(W=None), 1, "null pointer"),
+    ("fgmm_xent_fwd", C.FWD, dict(targets=None), 1, "null pointer"),
+    ("fgmm_xent_fwd", C.FWD, dict(loss=None), 1, "null pointer"),
+    ("fgmm_xent_fwd", C.FWD, dict(reduction=2), 1, "null pointer"),
+    ("fgmm_xent_fwd", C.FWD, dict(reduction=3), 1, "unknown reduction"),
+    ("fgmm_xent_fwd", C.FWD, dict(sxn=-8), 1, "negative stride"),
+    ("fgmm_xent_fwd", C.FWD, dict(W=257), 1, "not aligned"),
+    ("fgmm_xent_fwd", C.FWD, dict(bias=258), 1, "not aligned"),
+    ("fgmm_xent_bwd", C.BWD, dict(ds=2), 1, "dloss_stride"),
+    ("fgmm_xent_bwd", C.BWD, dict(logZ=None), 1, "null pointer"),
+    ("fgmm_xent_bwd", C.BWD, dict(dX=257), 1, "not aligned"),
+    ("fgmm_embed_fwd", C.EFWD, dict(out=None), 1, "null pointer"),
+    ("fgmm_embed_fwd", C.EFWD, dict(tsd=-1), 1, "negative stride"),
+    ("fgmm_embed_bwd", C.EBWD, dict(dtable=None), 1, "null pointer"),
+    ("fgmm_embed_bwd", C.EBWD, dict(flags=2), 1, "unknown flags"),
+    ("fgmm_embed_bwd", C.EBWD, dict(dout=257), 1, "not aligned"),
+])
+def test_c_entries_refuse_before_any_device_call(lib, entry, args, change, code, match):
+    got = getattr(lib, entry)(*dict(args, **change).values())
+    assert got == code, lib.fgmm_last_error()
+    message = lib.fgmm_last_error().decode()
+    assert match in message and entry in message
+
+
+def test_workspace_sizes(lib):
+    for back in (0, 1):
+        for kind in (0, 1, 2):
+            sizes = [lib.fgmm_xent_workspace_bytes(back, kind, n, 5000, 256) for n in (0, 1, 1000)]
+            assert sizes == sorted(sizes) and sizes[1] > 0
+    assert lib.fgmm_xent_workspace_bytes(0, 9, 10, 10, 10) == 0
+    assert lib.fgmm_embed_workspace_bytes(1000, 50, 8) > 0
+    assert lib.fgmm_embed_workspace_bytes(-1, 50, 8) == 0
+
+
+def test_oracle_against_autograd():
+    """The plain form the GPU tests compare with, against torch's own gradients in 64 bits."""
+    X, W, t, c = R.problem(40, 30, 12, torch.float32, ignored=0.3, bias=True, device="cpu")
+    w, z = torch.rand(40), torch.rand(40)
+    ref = R.xent(X, W, t, c, w=w, dlogZ=z)
+    X, W, c = (x.double().requires_grad_() for x in (X, W, c))
+    S = X @ W.t() + c
+    loss = torch.nn.functional.cross_entropy(S, t, reduction="none", ignore_index=R.IGNORE)
+    keep = (t != R.IGNORE).double()
+    ((loss * w).sum() + (torch.logsumexp(S, 1) * z * keep).sum()).backward()
+    for got, name in ((loss.detach(), "loss"), (X.grad, "dX"), (W.grad, "dW"), (c.grad, "dbias")):
+        assert float((got - ref[name]).abs().max()) < 1e-12
+    g, ids = torch.randn(40, 6), torch.randint(0, 9, (40,))
+    e = torch.zeros(9, 6, dtype=torch.float64, requires_grad=True)
+    (e[ids] * 0.3 * g.double()).sum().backward()
+    assert float((R.embed_grad(g, ids, 9, 0.3)[0] - e.grad).abs().max()) < 1e-12
