@@ -87,8 +87,8 @@ def load():
         mat = [_c_ptr, _c_i64, _c_i64]
         rows = mat + mat + [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32]
         scratch = [_c_ptr, ctypes.c_size_t]
-        lib.fgmm_xent_workspace_bytes.argtypes = [ctypes.c_int, ctypes.c_int, _c_i64, _c_i32,
-                                                  _c_i32]
+        lib.fgmm_xent_workspace_bytes.argtypes = [
+            ctypes.c_int, ctypes.c_int, _c_i64, _c_i32, _c_i32] + mat + [ctypes.c_int]
         lib.fgmm_xent_workspace_bytes.restype = ctypes.c_size_t
         lib.fgmm_xent_fwd.argtypes = [ctypes.c_int] + rows + [
             _c_ptr, _c_ptr, ctypes.c_int, _c_ptr, _c_ptr] + scratch + [_c_ptr]
@@ -251,7 +251,8 @@ def xent_fwd(X: torch.Tensor, W: torch.Tensor, targets: torch.Tensor, bias, igno
         if code:
             reduced = torch.empty((), device=dev, dtype=torch.float32)
             count = torch.empty((), device=dev, dtype=torch.float32)
-        ws = _scratch(dev, lib.fgmm_xent_workspace_bytes(0, kind, N, V, D))
+        ws = _scratch(dev, lib.fgmm_xent_workspace_bytes(
+            0, kind, N, V, D, W.data_ptr(), W.stride(0), W.stride(1), bias is not None))
         _check(lib.fgmm_xent_fwd(
             kind, X.data_ptr(), X.stride(0), X.stride(1), W.data_ptr(), W.stride(0), W.stride(1),
             _ptr(bias), targets.data_ptr(), ignore_index, N, V, D, loss.data_ptr(),
@@ -272,7 +273,8 @@ def xent_bwd(X, W, targets, bias, ignore_index: int, logZ, dloss, count, dlogZ, 
         dX = torch.empty(N, D, device=dev, dtype=X.dtype) if want[0] else None
         dW = torch.empty(V, D, device=dev, dtype=X.dtype) if want[1] else None
         dbias = torch.empty(V, device=dev, dtype=torch.float32) if want[2] else None
-        ws = _scratch(dev, lib.fgmm_xent_workspace_bytes(1, kind, N, V, D))
+        ws = _scratch(dev, lib.fgmm_xent_workspace_bytes(
+            1, kind, N, V, D, W.data_ptr(), W.stride(0), W.stride(1), bias is not None))
         _check(lib.fgmm_xent_bwd(
             kind, X.data_ptr(), X.stride(0), X.stride(1), W.data_ptr(), W.stride(0), W.stride(1),
             _ptr(bias), targets.data_ptr(), ignore_index, N, V, D, logZ.data_ptr(), _ptr(dloss),

@@ -226,9 +226,11 @@ FGMM_API int fgmm_generate_iso_rows(float* X, const int64_t* row_ids, int64_t ro
 #define FGMM_REDUCE_MEAN 2
 
 /* Bytes of workspace fgmm_xent_fwd (backward = 0) or fgmm_xent_bwd
- * (backward = 1) needs for this shape, whatever the strides. */
+ * (backward = 1) needs for this shape and this W (which is not read: a W whose
+ * address and strides TMA can take is used in place, another one is copied). */
 FGMM_API size_t fgmm_xent_workspace_bytes(int backward, int type, int64_t N, int32_t V,
-                                          int32_t D);
+                                          int32_t D, const void* W, int64_t w_stride_v,
+                                          int64_t w_stride_d, int has_bias);
 
 /* S = X W^T + bias (bias may be NULL; -inf removes an entry),
  *   logZ_n = log sum_v exp S_nv,   loss_n = logZ_n - S_{n, target_n}.
