@@ -387,7 +387,7 @@ store_slots_kernel(const float* __restrict__ slots, int ks, int64_t slot_rows, i
                    int64_t n, const int* __restrict__ inv, const Header* __restrict__ hdr,
                    int is_dw, int split, T* __restrict__ out) {
   const int per_row = (D + 3) / 4;
-  const Scales sc = std::is_same<T, __nv_bfloat16>::value ? Scales() : Scales(hdr->amax, split);
+  const Scales sc(hdr->amax, !std::is_same<T, __nv_bfloat16>::value, split);
   const float scale = is_dw ? sc.dw : sc.dx;
   const bool vec = D % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0;
   const bool bad = hdr->err != 0;
@@ -420,11 +420,12 @@ store_slots_kernel(const float* __restrict__ slots, int ks, int64_t slot_rows, i
 
 // dbias from the 128-row partial sums, in row order (NaN if a wait gave up).
 __global__ void __launch_bounds__(256) store_dbias_kernel(const XentArgs a, const XentWs w) {
+  const float back = 1.f / Scales(w.hdr->amax, a.type != FGMM_T_BF16, a.type == FGMM_T_F32).g;
   const int nparts = (int)(((int64_t)w.hdr->live + kPairRows - 1) / kPairRows) * 2;
   for (int64_t v = blockIdx.x * 256ll + threadIdx.x; v < a.V; v += gridDim.x * 256ll) {
     float s = 0.f;
     for (int k = 0; k < nparts; ++k) s += w.dbias_part[(int64_t)k * w.Vp + v];
-    a.dbias[v] = w.hdr->err ? __int_as_float(0x7fffffff) : s;
+    a.dbias[v] = w.hdr->err ? __int_as_float(0x7fffffff) : s * back;
   }
 }
 

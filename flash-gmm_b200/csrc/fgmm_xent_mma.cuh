@@ -17,9 +17,13 @@
 // work on one tile while the next is multiplied.
 //
 // SPLIT (fp32 inputs): operands are pairs of fp16 words hi + lo of the values scaled
-// by one power of two per matrix, and a K-block runs lo hi, hi lo and hi hi.  The
-// tensor core cuts its running sum at each step, so the accumulator is emptied into
-// fp32 registers every kSplitBlocks blocks, where sums round to nearest.
+// by one power of two per matrix, and a K-block runs lo hi, hi lo and hi hi.
+//
+// The tensor core cuts its running sum toward zero at each step of 16, about 2^-24 of
+// it on average: logits of 63 steps measured 2.3e-6 low.  Logits (and all of SPLIT) are
+// therefore emptied into fp32 registers every few K-blocks (group_blocks), where sums
+// round to nearest.  Products with G stored in 16 bits are not: their words' rounding
+// of 2^-9 or 2^-12 outweighs a chain's 2^-14.
 //
 // Warps: 0 TMA loads, 1 MMA (the pair's first SM), 2 TMEM, 4-11 epilogue (TMEM lane
 // quadrant = warp & 3, column half = (warp - 4) >> 2).  Every wait is bounded; a
@@ -29,7 +33,8 @@ constexpr int kPairRows = 256;
 constexpr int kBoxBytes = 64 * 128;
 constexpr int kEpiWarps = 8;
 constexpr int kMmaThreads = (4 + kEpiWarps) * 32;
-constexpr int kSplitBlocks = 2;
+constexpr int kSplitBlocks = 2;   // K-blocks per group: 24 steps
+constexpr int kLogitBlocks = 4;   // 16 steps
 
 enum TileKind { kLse = 0, kGrad = 1, kDx = 2, kDw = 3 };
 
@@ -76,23 +81,29 @@ struct MmaMaps {
   CUtensorMap X, W, G, X2, W2, G2;
 };
 
-// Powers of two that keep fp16 words in range.  fp16 inputs: G's words are g / 2^eg
-// with the largest weight in [2^12, 2^13).  SPLIT: X and W too, each with its largest
-// finite magnitude in [2^13, 2^14), so values down to 2^-16 of the largest keep 22 bits
-// and smaller ones an error of 2^-39 of the largest.
+// Scales of the stored words.  G is stored over the largest row weight: with equal
+// weights (a sum or a mean) the -1 at the label is then exact, where a weight like
+// 1/7372 rounded to bf16 would scale the whole gradient by up to 2^-9.  fp16 words are
+// 2^12 times that (at most 2^13, down to p = 2^-27 without losing bits).  SPLIT: X and
+// W too, by a power of two each with the largest finite magnitude in [2^13, 2^14), so
+// values down to 2^-16 of the largest keep 22 bits and smaller ones an error of 2^-39
+// of the largest.
 struct Scales {
-  float s = 1.f, g = 1.f, dx = 1.f, dw = 1.f;   // S, stored G, and the products with G
+  float s, g, dx, dw;   // S, stored G, and the products with G
   __device__ static int exponent(int bits, int target) {
     return max(-100, min(100, scale_exp_to(__int_as_float(bits), target)));
   }
-  __device__ Scales() {}
-  __device__ Scales(const int* amax, bool split) {
-    const int eg = exponent(amax[0], 13);
+  __device__ Scales(const int* amax, bool f16, bool split) {
+    const float top = __int_as_float(amax[0]);
+    const float unit = f16 ? 4096.f : 1.f;
+    // weights outside 2^-100 .. 2^100: their reciprocal would leave fp32
+    const bool sane = top > 7.9e-31f && top < 1.2e30f;
+    g = sane ? unit / top : unit;
+    const float back = sane ? top / unit : 1.f / unit;
     const int ex = split ? exponent(amax[1], 14) : 0, ew = split ? exponent(amax[2], 14) : 0;
     s = ldexpf(1.f, ex + ew);
-    g = ldexpf(1.f, -eg);
-    dx = ldexpf(1.f, eg + ew);
-    dw = ldexpf(1.f, eg + ex);
+    dx = ldexpf(back, ew);
+    dw = ldexpf(back, ex);
   }
 };
 
@@ -136,6 +147,25 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
                : "memory");
+}
+
+// K-blocks that the accumulator takes before it is emptied into registers.
+template <bool SPLIT, bool F16>
+__device__ __forceinline__ int group_blocks(const MmaParams& p, const Tile& t) {
+  if (SPLIT) return kSplitBlocks;
+  // bf16's g does not see the cut of its logits; fp16's and a fp32 dbias do
+  if (t.kind == kLse || (t.kind == kGrad && (F16 || p.dbias_part))) return kLogitBlocks;
+  return t.nkb;
+}
+
+// Moves registers between the warpgroups: 4 warps x 72 + 8 x 216 = 12 x 168.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 __device__ __forceinline__ void idle_cycles(long long n) {
@@ -254,6 +284,13 @@ __device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
   return v[0];
 }
 
+__device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&v)[32]) {
+  uint32_t u[32];
+  tmem_ld32(taddr, u);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
+}
+
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
@@ -310,8 +347,9 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     return mbar_wait_flag<true>(bar, parity, &ctl->abort_flag, p.err, code);
   };
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    regs_down<72>();
+    if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ loads
       TileWalk<FWD, SPLIT> walk(p, pair, npairs);
       Tile t;
@@ -348,9 +386,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       for (uint32_t k = it > NS ? it - NS : 0; ok && k < it; ++k)
         ok = wait(&ctl->empty[k % NS], (k / NS) & 1, 2);
       if (!ok) idle_cycles(4000000);
-    }
-  } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
+    } else if (warp == 1 && rank == 0 && lane == 0) {
       // ------------------------------------------------------------ MMA
       TileWalk<FWD, SPLIT> walk(p, pair, npairs);
       Tile t;
@@ -362,7 +398,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         const uint32_t idesc = (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) |
                                (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
                                ((uint32_t)(t.bn >> 3) << 17) | (16u << 24);
-        const int group = SPLIT ? kSplitBlocks : t.nkb;
+        const int group = group_blocks<SPLIT, f16>(p, t);
         for (int k0 = 0; ok && k0 < t.nkb; k0 += group, ++ac) {
           const uint32_t d = tmem + 256u * (ac & 1);
           if (ac >= 2 && !wait(&ctl->acc_empty[ac & 1], ((ac >> 1) - 1) & 1, 4)) { ok = false; break; }
@@ -401,7 +437,8 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         while (!mbar_try(smem_u32(&ctl->drain), 0) && clock64() - t0 < 100000000LL) {}
       }
     }
-  } else if (warp >= 4) {
+  } else {
+    regs_up<216>();
     // -------------------------------------------------------------- epilogue
     TileWalk<FWD, SPLIT> walk(p, pair, npairs);
     Tile t;
@@ -413,7 +450,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     const uint32_t empty_at[2] = {map_to_cta(smem_u32(&ctl->acc_empty[0]), 0),
                                   map_to_cta(smem_u32(&ctl->acc_empty[1]), 0)};
     constexpr bool f16 = std::is_same<T, __half>::value;
-    const Scales scales = f16 ? Scales(p.amax, SPLIT) : Scales();
+    const Scales scales(p.amax, f16, SPLIT);
     const float sc_s = scales.s;
     float m_run = -3.402823466e38f, s_run = 0.f;            // kLse, over the unit's tiles
     int target = -1;
@@ -428,97 +465,111 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     while (ok && walk.next(t)) {
       const int cols = t.bn / 2, col0 = half * cols;        // this warp's columns of the tile
       const int chunks = cols / 32;
-      float acc[SPLIT ? kChunks : 1][32];
-      uint32_t a_now = ac;
-      if (SPLIT) {
+      // The tile's products of this thread's row, in registers; the accumulator is given
+      // back before they are worked on.
+      float acc[kChunks][32];
+      const int group = group_blocks<SPLIT, f16>(p, t);
+      for (int k0 = 0; ok && k0 < t.nkb; k0 += group, ++ac) {
+        if (!__all_sync(0xffffffffu, wait(&ctl->acc_full[ac & 1], (ac >> 1) & 1, 32))) ok = false;
+        tc_fence_after();
+        const uint32_t at = lanes + 256u * (ac & 1) + col0;
+        if (k0 == 0) {
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) acc[SPLIT ? c : 0][i] = 0.f;
-        for (int k0 = 0; k0 < t.nkb; k0 += kSplitBlocks, ++ac) {
-          if (!__all_sync(0xffffffffu, wait(&ctl->acc_full[ac & 1], (ac >> 1) & 1, 32))) { ok = false; break; }
-          tc_fence_after();
+          for (int c = 0; c < kChunks; ++c)
+            if (c < chunks) tmem_ld32f(at + 32 * c, acc[c]);
+          tmem_wait_ld();
+        } else {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             if (c >= chunks) break;
-            uint32_t v[32];
-            tmem_ld32(lanes + 256u * (ac & 1) + col0 + 32 * c, v);
+            float v[32];
+            tmem_ld32f(at + 32 * c, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[SPLIT ? c : 0][i] += __uint_as_float(v[i]);
+            for (int i = 0; i < 32; ++i) acc[c][i] += v[i];
           }
-          release(ac);
         }
-      } else if (t.nkb > 0) {
-        if (!__all_sync(0xffffffffu, wait(&ctl->acc_full[ac & 1], (ac >> 1) & 1, 32))) ok = false;
-        tc_fence_after();
-        ++ac;
+        release(ac);
       }
       if (!ok) break;
-      // the chunk's 32 columns of this thread's row, products in natural units of the MMA
-      auto chunk = [&](int c, float (&v)[32]) {
+      if (t.nkb == 0) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
+      }
+
+      if (t.kind <= kGrad) {   // products -> logits
+        const int v0 = (int)t.brow + col0;
         if (SPLIT) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = acc[SPLIT ? c : 0][i];
-        } else if (t.nkb > 0) {
-          uint32_t u[32];
-          tmem_ld32(lanes + 256u * (a_now & 1) + col0 + 32 * c, u);
-          tmem_wait_ld();
+          for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+            for (int i = 0; i < 32; ++i) acc[c][i] *= sc_s;
         }
-        if (!SPLIT && t.nkb > 0 && c + 1 == chunks) release(a_now);
-      };
+        if (p.bias) {
+          const float4* b = reinterpret_cast<const float4*>(p.bias + v0);
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 x = __ldg(b + 8 * c + i);
+              acc[c][4 * i] += x.x; acc[c][4 * i + 1] += x.y;
+              acc[c][4 * i + 2] += x.z; acc[c][4 * i + 3] += x.w;
+            }
+        }
+      }
 
       if (FWD) {
         const int64_t row = t.arow + row_in;
+        const int v0 = (int)t.brow + col0;
         if (t.n == t.ks * p.per_split) {   // first tile of the unit
           m_run = -3.402823466e38f;
           s_run = 0.f;
           target = p.target[row];
         }
+        if (v0 + BN / 2 > p.V) {
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          float v[32];
-          chunk(c, v);
-          const int v0 = (int)t.brow + col0 + 32 * c;
-          if (SPLIT) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= sc_s;
-          }
-          if (p.bias) {
-            const float4* b = reinterpret_cast<const float4*>(p.bias + v0);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 x = __ldg(b + i);
-              v[4 * i] += x.x; v[4 * i + 1] += x.y; v[4 * i + 2] += x.z; v[4 * i + 3] += x.w;
-            }
-          } else if (v0 + 32 > p.V) {
+          for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (v0 + i >= p.V) v[i] = __int_as_float(0xff800000);
-          }
-          const bool mine = target >= v0 && target < v0 + 32;
-          if (__any_sync(0xffffffffu, mine)) {
-            float x = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x = target == v0 + i ? v[i] : x;
-            if (mine) p.tlogit[row] = x;
-          }
-          float mx = v[0];
-#pragma unroll
-          for (int i = 1; i < 32; ++i) mx = fmaxf(mx, v[i]);
-          const float mn = fmaxf(m_run, mx);
-          s_run *= ex2((m_run - mn) * kLog2Ef);
-          m_run = mn;
-          float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s4[i & 3] += ex2((v[i] - mn) * kLog2Ef);
-          s_run += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+              if (v0 + 32 * c + i >= p.V) acc[c][i] = __int_as_float(0xff800000);
         }
+        const int tc = target - v0;
+        const bool mine = tc >= 0 && tc < BN / 2;
+        if (__any_sync(0xffffffffu, mine)) {
+          float x = 0.f;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x = tc == 32 * c + i ? acc[c][i] : x;
+          if (mine) p.tlogit[row] = x;
+        }
+        float m8[8], s8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { m8[k] = acc[0][k]; s8[k] = 0.f; }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) m8[i & 7] = fmaxf(m8[i & 7], acc[c][i]);
+        const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                               fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+        const float mn = fmaxf(m_run, mx);
+        s_run *= ex2((m_run - mn) * kLog2Ef);
+        m_run = mn;
+        if (p.bias) {   // differences first: a bias may be the lowest float
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s8[i & 7] += ex2((acc[c][i] - mn) * kLog2Ef);
+        } else {
+          const float nm = fminf(-mn, 2e38f) * kLog2Ef;   // finite where every entry is masked
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s8[i & 7] += ex2(fmaf(acc[c][i], kLog2Ef, nm));
+        }
+        s_run += ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
         if (t.last) p.part[(int64_t)(2 * t.ks + half) * p.Np + row] = make_float2(m_run, s_run);
         continue;
       }
@@ -526,49 +577,49 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       if (t.kind == kGrad) {
         const int64_t row = t.arow + row_in;
         const RowGrad rg = p.rg[row];
-        const float gs = scales.g;
-        const int64_t grow = row - p.cur.r0;                // row of the G buffer
-        float csum[kChunks];
+        const int v0 = (int)t.brow + col0;
+        const int vend = p.cur.v0 + p.cur.nv;
+        const float ga = rg.a * scales.g, gb = rg.b * scales.g;
+        if (SPLIT || p.bias) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[c][i] = ga * ex2((acc[c][i] - rg.lse) * kLog2Ef);
+        } else {
+          const float nl = -rg.lse * kLog2Ef;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[c][i] = ga * ex2(fmaf(acc[c][i], kLog2Ef, nl));
+        }
+        const int tc = rg.target - v0;
+        if (__any_sync(0xffffffffu, tc >= 0 && tc < BN / 2)) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (tc == 32 * c + i) acc[c][i] -= gb;
+        }
+        // rows without a weight (padding) and entries behind the last: exactly zero
+        const bool empty = rg.a == 0.f && rg.b == 0.f;
+        if (v0 + BN / 2 > vend || __any_sync(0xffffffffu, empty)) {
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (empty || v0 + 32 * c + i >= vend) acc[c][i] = 0.f;
+        }
+        // 128-byte staged rows: 64 columns of 16-bit words, or 32 of hi and lo words
+        const int64_t grow0 = row - lane - p.cur.r0;        // rows of the G buffer
+        const int64_t gcol0 = t.brow - p.cur.v0 + col0;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          float v[32];
-          chunk(c, v);
-          const int v0 = (int)t.brow + col0 + 32 * c;
-          const int vend = p.cur.v0 + p.cur.nv;
-          float b[32];
-          if (p.bias) {
-            const float4* bp = reinterpret_cast<const float4*>(p.bias + v0);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 x = __ldg(bp + i);
-              b[4 * i] = x.x; b[4 * i + 1] = x.y; b[4 * i + 2] = x.z; b[4 * i + 3] = x.w;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) b[i] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float s = SPLIT ? fmaf(v[i], sc_s, b[i]) : v[i] + b[i];
-            float g = rg.a * ex2((s - rg.lse) * kLog2Ef);
-            if (v0 + i == rg.target) g -= rg.b;
-            if (v0 + 32 > vend && v0 + i >= vend) g = 0.f;
-            // rows without a weight (padding): exactly zero whatever S is
-            v[i] = rg.a == 0.f && rg.b == 0.f ? 0.f : g;
-          }
-          if (p.dbias_part) {
-            float w[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = v[i];
-            csum[c] = column_sums(w, lane);
-          }
-          // 32 columns = 64 bytes of a row; two chunks fill a 128-byte staged row
 #pragma unroll
           for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float a = v[2 * i] * gs, bb = v[2 * i + 1] * gs;
+              const float a = acc[c][2 * i], bb = acc[c][2 * i + 1];
               uint32_t hi = pack2<T>(a, bb);
               if (SPLIT && h) hi = pack_f16(a - f16lo_f(hi), bb - f16hi_f(hi));
               w[i] = hi;
@@ -581,8 +632,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           }
           if (SPLIT || (c & 1)) {
             __syncwarp();
-            const int64_t gcol = t.brow - p.cur.v0 + col0 + 32 * (SPLIT ? c : c - 1);
-            const int64_t grow0 = grow - lane;
+            const int64_t gcol = gcol0 + 32 * (SPLIT ? c : c - 1);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = 4 * i + (lane >> 3), g = lane & 7;
@@ -598,9 +648,11 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           }
         }
         if (p.dbias_part) {
-          // the four quadrants' sums meet in the (now free) stages: [half][quadrant][BN / 2]
+          // column sums of the unrounded g; the four quadrants' meet in the (now free)
+          // stages: [half][quadrant][BN / 2]
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) reinterpret_cast<float*>(stage)[32 * c + lane] = csum[c];
+          for (int c = 0; c < kChunks; ++c)
+            reinterpret_cast<float*>(stage)[32 * c + lane] = column_sums(acc[c], lane);
           asm volatile("bar.sync 1, 256;" ::: "memory");
           const int e = (int)threadIdx.x - 128;
           if (e < BN) {
@@ -624,8 +676,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         if (c >= chunks) break;
-        float v[32];
-        chunk(c, v);
+        const float (&v)[32] = acc[c];
         const int64_t col = t.brow + col0 + 32 * c;
         // 32 fp32 columns = a 128-byte staged row
 #pragma unroll
