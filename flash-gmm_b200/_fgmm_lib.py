@@ -233,6 +233,23 @@ def _scratch(device: torch.device, nbytes: int) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+def _launch(fn, dev: torch.device, *args):
+    """fn(*args, stream) on ``dev`` and torch's current stream there."""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if torch.cuda.current_device() == dev.index:
+        code = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, stream)
+    if code != 0:
+        _check(code)
+
+
+@functools.lru_cache(maxsize=1024)
+def _xent_bytes(backward, kind, N, V, D, align, s0, s1, has_bias) -> int:
+    return load().fgmm_xent_workspace_bytes(backward, kind, N, V, D, align, s0, s1, has_bias)
+
+
 def xent_fwd(X: torch.Tensor, W: torch.Tensor, targets: torch.Tensor, bias, ignore_index: int,
              reduction: str):
     """fgmm_xent_fwd on torch's current stream: (loss rows, logZ rows, reduced,
@@ -242,22 +259,20 @@ def xent_fwd(X: torch.Tensor, W: torch.Tensor, targets: torch.Tensor, bias, igno
     dev = X.device
     N, D = X.shape
     V = W.shape[0]
+    xs, ws_, wp = X.stride(), W.stride(), W.data_ptr()
     code = FGMM_REDUCE[reduction]
     kind = FGMM_TYPES[X.dtype]
-    with torch.cuda.device(dev):
-        loss = torch.empty(N, device=dev, dtype=torch.float32)
-        logZ = torch.empty(N, device=dev, dtype=torch.float32)
-        reduced = count = None
-        if code:
-            reduced = torch.empty((), device=dev, dtype=torch.float32)
-            count = torch.empty((), device=dev, dtype=torch.float32)
-        ws = _scratch(dev, lib.fgmm_xent_workspace_bytes(
-            0, kind, N, V, D, W.data_ptr(), W.stride(0), W.stride(1), bias is not None))
-        _check(lib.fgmm_xent_fwd(
-            kind, X.data_ptr(), X.stride(0), X.stride(1), W.data_ptr(), W.stride(0), W.stride(1),
+    loss = torch.empty(N, device=dev, dtype=torch.float32)
+    logZ = torch.empty_like(loss)
+    reduced = count = None
+    if code:
+        reduced = torch.empty((), device=dev, dtype=torch.float32)
+        count = torch.empty_like(reduced)
+    nbytes = _xent_bytes(0, kind, N, V, D, wp & 15, ws_[0], ws_[1], bias is not None)
+    ws = _scratch(dev, nbytes)
+    _launch(lib.fgmm_xent_fwd, dev, kind, X.data_ptr(), xs[0], xs[1], wp, ws_[0], ws_[1],
             _ptr(bias), targets.data_ptr(), ignore_index, N, V, D, loss.data_ptr(),
-            logZ.data_ptr(), code, _ptr(reduced), _ptr(count), ws.data_ptr(), ws.numel(),
-            torch.cuda.current_stream(dev).cuda_stream))
+            logZ.data_ptr(), code, _ptr(reduced), _ptr(count), ws.data_ptr(), nbytes)
     return loss, logZ, reduced, count
 
 
@@ -268,19 +283,17 @@ def xent_bwd(X, W, targets, bias, ignore_index: int, logZ, dloss, count, dlogZ, 
     dev = X.device
     N, D = X.shape
     V = W.shape[0]
+    xs, ws_, wp = X.stride(), W.stride(), W.data_ptr()
     kind = FGMM_TYPES[X.dtype]
-    with torch.cuda.device(dev):
-        dX = torch.empty(N, D, device=dev, dtype=X.dtype) if want[0] else None
-        dW = torch.empty(V, D, device=dev, dtype=X.dtype) if want[1] else None
-        dbias = torch.empty(V, device=dev, dtype=torch.float32) if want[2] else None
-        ws = _scratch(dev, lib.fgmm_xent_workspace_bytes(
-            1, kind, N, V, D, W.data_ptr(), W.stride(0), W.stride(1), bias is not None))
-        _check(lib.fgmm_xent_bwd(
-            kind, X.data_ptr(), X.stride(0), X.stride(1), W.data_ptr(), W.stride(0), W.stride(1),
+    dX = torch.empty(N, D, device=dev, dtype=X.dtype) if want[0] else None
+    dW = torch.empty(V, D, device=dev, dtype=X.dtype) if want[1] else None
+    dbias = torch.empty(V, device=dev, dtype=torch.float32) if want[2] else None
+    nbytes = _xent_bytes(1, kind, N, V, D, wp & 15, ws_[0], ws_[1], bias is not None)
+    ws = _scratch(dev, nbytes)
+    _launch(lib.fgmm_xent_bwd, dev, kind, X.data_ptr(), xs[0], xs[1], wp, ws_[0], ws_[1],
             _ptr(bias), targets.data_ptr(), ignore_index, N, V, D, logZ.data_ptr(), _ptr(dloss),
             1 if dloss is not None and dloss.dim() else 0, _ptr(count), _ptr(dlogZ), _ptr(dX),
-            _ptr(dW), _ptr(dbias), ws.data_ptr(), ws.numel(),
-            torch.cuda.current_stream(dev).cuda_stream))
+            _ptr(dW), _ptr(dbias), ws.data_ptr(), nbytes)
     return dX, dW, dbias
 
 
@@ -289,13 +302,11 @@ def embed_fwd(table, ids, scale: float, ignore_index: int) -> torch.Tensor:
     lib = load()
     dev = table.device
     V, D = table.shape
-    N = ids.numel()
-    with torch.cuda.device(dev):
-        out = torch.empty(N, D, device=dev, dtype=table.dtype)
-        _check(lib.fgmm_embed_fwd(
-            FGMM_TYPES[table.dtype], table.data_ptr(), table.stride(0), table.stride(1),
-            ids.data_ptr(), ignore_index, N, V, D, scale, out.data_ptr(),
-            torch.cuda.current_stream(dev).cuda_stream))
+    N = ids.shape[0]
+    s = table.stride()
+    out = torch.empty(N, D, device=dev, dtype=table.dtype)
+    _launch(lib.fgmm_embed_fwd, dev, FGMM_TYPES[table.dtype], table.data_ptr(), s[0], s[1],
+            ids.data_ptr(), ignore_index, N, V, D, scale, out.data_ptr())
     return out
 
 
@@ -304,14 +315,13 @@ def embed_bwd(dout, ids, scale: float, ignore_index: int, out, accumulate: bool)
     lib = load()
     dev = dout.device
     V, D = out.shape
-    N = ids.numel()
-    with torch.cuda.device(dev):
-        ws = _scratch(dev, lib.fgmm_embed_workspace_bytes(N, V, D))
-        _check(lib.fgmm_embed_bwd(
-            FGMM_TYPES[dout.dtype], dout.data_ptr(), dout.stride(0), dout.stride(1),
-            ids.data_ptr(), ignore_index, N, V, D, scale, out.data_ptr(), ws.data_ptr(),
-            ws.numel(), FGMM_FLAG_ACCUMULATE if accumulate else 0,
-            torch.cuda.current_stream(dev).cuda_stream))
+    N = ids.shape[0]
+    s = dout.stride()
+    nbytes = lib.fgmm_embed_workspace_bytes(N, V, D)
+    ws = _scratch(dev, nbytes)
+    _launch(lib.fgmm_embed_bwd, dev, FGMM_TYPES[dout.dtype], dout.data_ptr(), s[0], s[1],
+            ids.data_ptr(), ignore_index, N, V, D, scale, out.data_ptr(), ws.data_ptr(), nbytes,
+            FGMM_FLAG_ACCUMULATE if accumulate else 0)
     return out
 
 

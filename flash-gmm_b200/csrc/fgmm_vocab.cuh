@@ -35,6 +35,14 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// VEC consecutive elements, moved as one access (VEC * sizeof(T) = 16, or one element).
+template <class T, int VEC>
+struct __align__(VEC * sizeof(T)) Pack {
+  T v[VEC];
+  __device__ __forceinline__ void load(const T* p) { *this = *reinterpret_cast<const Pack*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Pack*>(p) = *this; }
+};
+
 // Calls f with a null pointer of the element type (a type tag).
 template <class F>
 decltype(auto) with_type(int type, F&& f) {

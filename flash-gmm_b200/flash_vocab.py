@@ -41,6 +41,11 @@ def _need_gpu(**tensors):
             raise ValueError(f"{name} is on {t.device}, the other arguments on {dev}")
 
 
+def _tracked(*tensors) -> bool:
+    """Whether autograd has to see the call."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _need_type(name: str, t: torch.Tensor):
     if t.dtype not in L.FGMM_TYPES:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
@@ -49,7 +54,11 @@ def _need_type(name: str, t: torch.Tensor):
 def _labels(name: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{name} must be int64 or int32, got {t.dtype}")
-    return t.reshape(-1).to(torch.int64).contiguous()
+    if t.dim() != 1:
+        t = t.reshape(-1)
+    if t.dtype != torch.int64:
+        t = t.long()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -114,11 +123,18 @@ def linear_cross_entropy(X: torch.Tensor, W: torch.Tensor, targets: torch.Tensor
     if bias is not None:
         bias = bias.float().contiguous()
     shape = targets.shape
-    loss, logZ = _LinearCrossEntropy.apply(X.reshape(-1, X.shape[-1]), W, bias, labels,
-                                           int(ignore_index), reduction)
-    if reduction == "none":
-        loss = loss.reshape(shape)
-    return (loss, logZ.reshape(shape)) if return_logZ else loss
+    if X.dim() != 2:
+        X = X.reshape(-1, X.shape[-1])
+    if _tracked(X, W, bias):
+        loss, logZ = _LinearCrossEntropy.apply(X, W, bias, labels, int(ignore_index), reduction)
+    else:
+        loss, logZ, reduced, _ = L.xent_fwd(X, W, labels, bias, int(ignore_index), reduction)
+        loss = loss if reduced is None else reduced
+    if len(shape) != 1:
+        logZ = logZ.reshape(shape)
+        if reduction == "none":
+            loss = loss.reshape(shape)
+    return (loss, logZ) if return_logZ else loss
 
 
 class _EmbeddingLookup(torch.autograd.Function):
@@ -151,8 +167,9 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
     _need_type("table", table)
     flat = _labels("ids", ids)
     _need_gpu(table=table, ids=ids)
-    out = _EmbeddingLookup.apply(table, flat, float(scale), int(ignore_index))
-    return out.reshape(*ids.shape, table.shape[1])
+    fn = _EmbeddingLookup.apply if _tracked(table) else L.embed_fwd
+    out = fn(table, flat, float(scale), int(ignore_index))
+    return out if ids.dim() == 1 else out.reshape(*ids.shape, table.shape[1])
 
 
 def embedding_grad(dout: torch.Tensor, ids: torch.Tensor, V: int, *, scale: float = 1.0,
