@@ -250,6 +250,11 @@ def _xent_bytes(backward, kind, N, V, D, align, s0, s1, has_bias) -> int:
     return load().fgmm_xent_workspace_bytes(backward, kind, N, V, D, align, s0, s1, has_bias)
 
 
+@functools.lru_cache(maxsize=1024)
+def _embed_bytes(N, V, D) -> int:
+    return load().fgmm_embed_workspace_bytes(N, V, D)
+
+
 def xent_fwd(X: torch.Tensor, W: torch.Tensor, targets: torch.Tensor, bias, ignore_index: int,
              reduction: str):
     """fgmm_xent_fwd on torch's current stream: (loss rows, logZ rows, reduced,
@@ -317,7 +322,7 @@ def embed_bwd(dout, ids, scale: float, ignore_index: int, out, accumulate: bool)
     V, D = out.shape
     N = ids.shape[0]
     s = dout.stride()
-    nbytes = lib.fgmm_embed_workspace_bytes(N, V, D)
+    nbytes = _embed_bytes(N, V, D)
     ws = _scratch(dev, nbytes)
     _launch(lib.fgmm_embed_bwd, dev, FGMM_TYPES[dout.dtype], dout.data_ptr(), s[0], s[1],
             ids.data_ptr(), ignore_index, N, V, D, scale, out.data_ptr(), ws.data_ptr(), nbytes,

@@ -12,6 +12,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "fgmm_ptx.cuh"
 #include "fgmm_vocab.cuh"
 
 namespace fgmm {
@@ -23,50 +24,48 @@ constexpr int kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = 256;
 constexpr int kSortItems = 8;
 constexpr int kSortTile = kSortThreads * kSortItems;
-// Short sorts (up to 16,384 ids): one block, all passes in shared memory.
-constexpr int kBlockSortThreads = 1024;
-constexpr int64_t kBlockSortMax = 16384;
+// Up to 131,072 ids: one cluster of up to 8 blocks, all passes in shared memory.
+constexpr int kClusterSortThreads = 1024;
+constexpr int kClusterSortBlocks = 8;
+constexpr int64_t kClusterSortMax = (int64_t)kClusterSortThreads * 16 * kClusterSortBlocks;
 // Sorted positions per block of the gradient.
 constexpr int kRun = 32;
 
 // ---------------------------------------------------------------- lookup
-// out = scale * table[id], 16 bytes (VEC elements) a thread; four independent
-// rows' pieces in flight each.  Bound by DRAM: N D read (distinct rows) and
-// N D written.
+// out = scale * table[id].  Each row is read by `lanes` threads (a power of two),
+// 16 bytes (VEC elements) each, and a thread has four rows' pieces in flight.
+// Bound by DRAM: N D read (distinct rows) and N D written.
 template <class T, int VEC>
 __global__ void __launch_bounds__(256)
 lookup_kernel(const T* __restrict__ table, int64_t tsv, int64_t tsd,
               const int64_t* __restrict__ ids, int64_t ignore, int64_t N, int V, int D, float scale,
-              T* __restrict__ out) {
+              int lanes, T* __restrict__ out) {
+  const int rows = 256 / lanes, mine = threadIdx.x / lanes, piece0 = threadIdx.x % lanes;
   const int per_row = D / VEC;
-  const int64_t total = N * per_row, step = gridDim.x * 256ll;
-  for (int64_t e0 = blockIdx.x * 256ll + threadIdx.x; e0 < total; e0 += 4 * step) {
-    Pack<T, VEC> x[4];
-    int how[4];   // 0 outside, 1 a row, 2 ignored, 3 bad id
+  for (int64_t i0 = blockIdx.x * (4ll * rows) + mine; i0 < N; i0 += gridDim.x * (4ll * rows)) {
+    const T* src[4];
+    float fill[4];   // of a row that is not read
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t e = e0 + u * step;
-      how[u] = 0;
-      if (e < total) {
-        const int64_t i = e / per_row;
-        const int64_t id = __ldg(ids + i);
-        how[u] = id == ignore ? 2 : id < 0 || id >= V ? 3 : 1;
-        if (how[u] == 1) {
-          const T* src = table + id * tsv + (e - i * per_row) * VEC * tsd;
-          x[u].load(src);
-        }
-      }
+      const int64_t i = i0 + u * rows, id = i < N ? __ldg(ids + i) : ignore;
+      const bool skip = id == ignore, bad = !skip && (id < 0 || id >= V);
+      src[u] = skip || bad ? nullptr : table + id * tsv;
+      fill[u] = bad ? __int_as_float(0x7fffffff) : 0.f;
     }
+    for (int c = piece0; c < per_row; c += lanes) {
+      Pack<T, VEC> x[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (how[u] == 0) continue;
+      for (int u = 0; u < 4; ++u)
+        if (src[u]) x[u].load(src[u] + (int64_t)c * VEC * tsd);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        float v = how[u] == 1 ? to_f32(x[u].v[k]) * scale : 0.f;
-        if (how[u] == 3) v = __int_as_float(0x7fffffff);
-        x[u].v[k] = from_f32<T>(v);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t i = i0 + u * rows;
+        if (i >= N) break;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          x[u].v[k] = from_f32<T>(src[u] ? to_f32(x[u].v[k]) * scale : fill[u]);
+        x[u].store(out + i * D + (int64_t)c * VEC);
       }
-      x[u].store(out + (e0 + u * step) * VEC);
     }
   }
 }
@@ -77,37 +76,25 @@ __device__ __forceinline__ uint32_t sort_key(int64_t id, int64_t ignore, int V) 
   return id == ignore || id < 0 || id >= V ? (uint32_t)V : (uint32_t)id;
 }
 
-// Part of the gradient table that a sorting launch clears: the sort is bound by
-// latency and uses few SMs, so the blocks behind its own write the zeros of the
-// rows that no id names (and of the others, which the sums overwrite).
-struct Fill {
-  uint4* ptr;
-  int64_t n;   // 16-byte units
-  int first;   // first block that fills
-  __device__ __forceinline__ bool run() const {
-    if ((int)blockIdx.x < first) return false;
-    const int64_t step = (int64_t)(gridDim.x - first) * blockDim.x;
-    for (int64_t i = (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x; i < n; i += step)
-      ptr[i] = make_uint4(0u, 0u, 0u, 0u);
-    return true;
+// The lanes of the warp that hold the same digit (one ballot per bit: cheaper here
+// than a match instruction, whose time grows with the distinct values).
+__device__ __forceinline__ uint32_t same_digit(uint32_t d, int bits) {
+  uint32_t same = 0xffffffffu;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (d >> b) & 1u;
+    const uint32_t m = __ballot_sync(0xffffffffu, one);
+    same &= one ? m : ~m;
   }
-};
+  return same;
+}
 
-// Rank of each of a warp's ITEMS x 32 consecutive keys among the warp's equal
-// digits, in order; cnt (the warp's digit counts, zero before) ends as totals.
-template <int ITEMS>
-__device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ITEMS], uint32_t* cnt,
-                                           uint32_t (&rank)[ITEMS], int lane) {
-#pragma unroll
-  for (int r = 0; r < ITEMS; ++r) {
-    const uint32_t d = digit[r];   // kDigits: none
-    const uint32_t same = __match_any_sync(0xffffffffu, d);
-    const uint32_t before = d < kDigits ? cnt[d] : 0u;
-    __syncwarp();
-    rank[r] = before + __popc(same & ((1u << lane) - 1u));
-    if (d < kDigits && lane == 31 - __clz(same)) cnt[d] = rank[r] + 1;
-    __syncwarp();
-  }
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_cluster2(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
 }
 
 // Exclusive prefix sum of one value per thread over 1024 threads; *all: the sum.
@@ -136,41 +123,44 @@ __device__ __forceinline__ uint32_t block_prefix1024(uint32_t v, uint32_t* warp_
   return (warp ? warp_sum[warp - 1] : 0u) + s - v;
 }
 
-// Stable sort of up to 1024 ITEMS ids by block 0; the other blocks clear the table.
-// A warp owns 32 ITEMS consecutive places; digits are ranked within the warp, the
-// warps' counts are summed per digit in warp order, and keys and positions change
-// places through shared memory.
+// Stable sort of up to 1024 ITEMS x (blocks of the cluster) ids, all passes in
+// shared memory.  A warp owns 32 ITEMS consecutive places; digits are ranked within
+// the warp, the warps' counts summed per digit in warp order, the blocks' counts in
+// block order (read from each other's shared memory), and each key goes to its place
+// in the block that owns it.  Bound by latency: two cluster barriers a pass.
 template <int ITEMS>
-__global__ void __launch_bounds__(kBlockSortThreads)
-block_sort_kernel(const int64_t* __restrict__ ids, int64_t ignore, int V, int N, int bits,
-                  int digit_bits, uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
-                  const Fill fill) {
-  if (fill.run()) return;
+__global__ void __launch_bounds__(kClusterSortThreads)
+cluster_sort_kernel(const int64_t* __restrict__ ids, int64_t ignore, int V, int N, int bits,
+                    int digit_bits, uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
+                    uint32_t* __restrict__ joins) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) joins[0] = 0;
   extern __shared__ uint32_t sm[];
-  constexpr int kAll = kBlockSortThreads * ITEMS;
-  uint32_t* skey = sm;
-  uint32_t* spos = sm + kAll;
-  uint16_t* cnt16 = reinterpret_cast<uint16_t*>(sm + 2 * kAll);   // [32][256]
+  constexpr int kMine = kClusterSortThreads * ITEMS;               // places of a block
+  uint2* place = reinterpret_cast<uint2*>(sm);                     // [kMine] (key, pos)
+  uint16_t* cnt16 = reinterpret_cast<uint16_t*>(sm + 2 * kMine);   // [32][256]
+  __shared__ uint32_t total[kDigits];    // this block's count of each digit
+  __shared__ uint32_t offset[kDigits];   // first place of this block's keys of the digit
   __shared__ uint32_t warp_sum[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank_c = (int)cluster_rank(), blocks = gridDim.x;      // one cluster
   const int base = warp * 32 * ITEMS;
   uint32_t key[ITEMS], pos[ITEMS], rank[ITEMS];
 #pragma unroll
   for (int r = 0; r < ITEMS; ++r) {
-    const int i = base + 32 * r + lane;
-    key[r] = i < N ? sort_key(ids[i], ignore, V) : 0xffffffffu;   // behind the last: stays last
+    const int i = rank_c * kMine + base + 32 * r + lane;
+    key[r] = i < N ? sort_key(ids[i], ignore, V) : 0xffffffffu;    // behind the last: stays last
     pos[r] = (uint32_t)i;
   }
   const uint32_t mask = (1u << digit_bits) - 1u;
+  uint16_t* cnt = cnt16 + warp * kDigits;
   for (int shift = 0; shift < bits; shift += digit_bits) {
-    for (int i = threadIdx.x; i < 32 * kDigits / 2; i += kBlockSortThreads)
+    for (int i = threadIdx.x; i < 32 * kDigits / 2; i += kClusterSortThreads)
       reinterpret_cast<uint32_t*>(cnt16)[i] = 0u;
     __syncthreads();
-    uint16_t* cnt = cnt16 + warp * kDigits;
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
       const uint32_t d = (key[r] >> shift) & mask;
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      const uint32_t same = same_digit(d, digit_bits);
       const uint32_t before = cnt[d];
       __syncwarp();
       rank[r] = before + __popc(same & ((1u << lane) - 1u));
@@ -178,38 +168,55 @@ block_sort_kernel(const int64_t* __restrict__ ids, int64_t ignore, int V, int N,
       __syncwarp();
     }
     __syncthreads();
-    // digit d = thread / 4 of four threads, each for 8 warps: counts -> offsets
-    const int d = threadIdx.x >> 2, part = threadIdx.x & 3;
-    uint32_t mine = 0;
+    // four threads per digit, each for 8 warps: the warps' counts become offsets
+    {
+      const int d = threadIdx.x >> 2, part = threadIdx.x & 3;
+      uint32_t c[8], mine = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) mine += cnt16[(part * 8 + w) * kDigits + d];
-    uint32_t all;
-    uint32_t run = block_prefix1024(mine, warp_sum, &all);
+      for (int w = 0; w < 8; ++w) { c[w] = cnt16[(part * 8 + w) * kDigits + d]; mine += c[w]; }
+      uint32_t run = mine;
+      uint32_t t = __shfl_up_sync(0xffffffffu, run, 1, 4);
+      if (part >= 1) run += t;
+      t = __shfl_up_sync(0xffffffffu, run, 2, 4);
+      if (part >= 2) run += t;
+      if (part == 3) total[d] = run;
+      run -= mine;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      uint16_t* c = cnt16 + (part * 8 + w) * kDigits + d;
-      const uint32_t v = *c;
-      *c = (uint16_t)run;
-      run += v;
+      for (int w = 0; w < 8; ++w) {
+        cnt16[(part * 8 + w) * kDigits + d] = (uint16_t)run;
+        run += c[w];
+      }
     }
+    cluster_sync_all();            // every block's totals are there
+    uint32_t all_d = 0, below = 0;
+    if (threadIdx.x < kDigits) {
+      for (int b = 0; b < blocks; ++b) {
+        const uint32_t v = ld_cluster(map_to_cta(smem_u32(&total[threadIdx.x]), b));
+        all_d += v;
+        if (b < rank_c) below += v;
+      }
+    }
+    uint32_t sum;
+    const uint32_t first = block_prefix1024(all_d, warp_sum, &sum);
+    if (threadIdx.x < kDigits) offset[threadIdx.x] = first + below;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
-      const uint32_t at = cnt[(key[r] >> shift) & mask] + rank[r];
-      skey[at] = key[r];
-      spos[at] = pos[r];
+      const uint32_t d = (key[r] >> shift) & mask;
+      const uint32_t at = offset[d] + cnt[d] + rank[r];
+      st_cluster2(map_to_cta(smem_u32(&place[at % kMine]), at / kMine), key[r], pos[r]);
     }
-    __syncthreads();
+    cluster_sync_all();            // every key is in its place, every total has been read
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
-      key[r] = skey[base + 32 * r + lane];
-      pos[r] = spos[base + 32 * r + lane];
+      const uint2 x = place[base + 32 * r + lane];
+      key[r] = x.x;
+      pos[r] = x.y;
     }
-    __syncthreads();
   }
 #pragma unroll
   for (int r = 0; r < ITEMS; ++r) {
-    const int i = base + 32 * r + lane;
+    const int i = rank_c * kMine + base + 32 * r + lane;
     if (i < N) {
       key_out[i] = key[r];
       pos_out[i] = pos[r];
@@ -235,8 +242,7 @@ struct SortIn {
 
 __global__ void __launch_bounds__(kSortThreads)
 sort_count_kernel(SortIn in, int64_t N, int shift, uint32_t mask, uint32_t* __restrict__ hist,
-                  int nblocks, const Fill fill) {
-  if (fill.run()) return;
+                  int nblocks) {
   __shared__ uint32_t h[kDigits];
   h[threadIdx.x] = 0;
   __syncthreads();
@@ -251,8 +257,8 @@ sort_count_kernel(SortIn in, int64_t N, int shift, uint32_t mask, uint32_t* __re
 
 // Exclusive prefix sum of hist[0, n) by one block.
 __global__ void __launch_bounds__(1024)
-sort_scan_kernel(uint32_t* __restrict__ hist, int64_t n, const Fill fill) {
-  if (fill.run()) return;
+sort_scan_kernel(uint32_t* __restrict__ hist, int64_t n, uint32_t* __restrict__ joins) {
+  if (threadIdx.x == 0) joins[0] = 0;
   __shared__ uint32_t warp_sum[32];
   uint32_t carry = 0;
   for (int64_t base = 0; base < n; base += 8192) {   // 8 consecutive values a thread
@@ -276,10 +282,10 @@ sort_scan_kernel(uint32_t* __restrict__ hist, int64_t n, const Fill fill) {
 
 // Stable scatter: a warp owns 256 consecutive items and ranks 32 at a time.
 __global__ void __launch_bounds__(kSortThreads)
-sort_scatter_kernel(SortIn in, int64_t N, int shift, uint32_t mask,
+sort_scatter_kernel(SortIn in, int64_t N, int shift, int digit_bits,
                     const uint32_t* __restrict__ offs, int nblocks, uint32_t* __restrict__ key_out,
-                    uint32_t* __restrict__ pos_out, const Fill fill) {
-  if (fill.run()) return;
+                    uint32_t* __restrict__ pos_out) {
+  const uint32_t mask = (1u << digit_bits) - 1u;
   constexpr int kWarps = kSortThreads / 32;
   __shared__ uint32_t cnt[kWarps][kDigits];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -290,10 +296,18 @@ sort_scatter_kernel(SortIn in, int64_t N, int shift, uint32_t mask,
 #pragma unroll
   for (int r = 0; r < kSortItems; ++r) {
     const int64_t i = base + r * 32 + lane;
-    key[r] = i < N ? in.get_key(i) : 0u;
-    digit[r] = i < N ? (key[r] >> shift) & mask : (uint32_t)kDigits;
+    key[r] = i < N ? in.get_key(i) : 0xffffffffu;   // behind the last: ranked last, not stored
+    digit[r] = (key[r] >> shift) & mask;
   }
-  warp_ranks<kSortItems>(digit, cnt[warp], rank, lane);
+#pragma unroll
+  for (int r = 0; r < kSortItems; ++r) {
+    const uint32_t same = same_digit(digit[r], digit_bits);
+    const uint32_t before = cnt[warp][digit[r]];
+    __syncwarp();
+    rank[r] = before + __popc(same & ((1u << lane) - 1u));
+    if (lane == 31 - __clz(same)) cnt[warp][digit[r]] = rank[r] + 1;
+    __syncwarp();
+  }
   __syncthreads();
   uint32_t run = offs[(size_t)threadIdx.x * nblocks + blockIdx.x];
   for (int w = 0; w < kWarps; ++w) {
@@ -314,11 +328,46 @@ sort_scatter_kernel(SortIn in, int64_t N, int shift, uint32_t mask,
 }
 
 // ---------------------------------------------------------------- gradient
-// A block sums kRun sorted positions (blockIdx.x) of 256 VEC columns (blockIdx.y).
+// A block sums kRun sorted positions of 256 VEC columns.
 // Ids whose run of positions lies inside write their row of the table; a run cut by
 // the block's ends leaves an fp32 part: parts[2 b] of the one that began before,
 // parts[2 b + 1] of the one that began here and goes on.  So a frequent id's rows
 // are read by as many blocks as they fill, and every order of sums is fixed.
+// The blocks behind the sums (clear_rows) write the rows that no id names: a table
+// row is written once, and the two kinds of blocks share the DRAM's time.
+constexpr int kClearRows = 32;
+
+// Rows [v0, v0 + 32) of the table: lane = row finds whether an id names it.
+template <class T>
+__device__ __forceinline__ void clear_rows(const uint32_t* __restrict__ key, int64_t N, int64_t v0,
+                                           int V, int D, int vec, T* __restrict__ dtable) {
+  __shared__ uint32_t s_empty;
+  if (threadIdx.x < 32) {
+    const uint32_t v = (uint32_t)v0 + threadIdx.x;
+    bool empty = false;
+    if (v < (uint32_t)V) {
+      int64_t lo = 0, hi = N;
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (key[mid] < v) lo = mid + 1; else hi = mid;
+      }
+      empty = lo == N || key[lo] != v;
+    }
+    const uint32_t m = __ballot_sync(0xffffffffu, empty);
+    if (threadIdx.x == 0) s_empty = m;
+  }
+  __syncthreads();
+  for (uint32_t m = s_empty; m; m &= m - 1) {
+    T* row = dtable + (v0 + (__ffs(m) - 1)) * D;
+    if (vec) {
+      const int n = (int)(D * sizeof(T) / 16);
+      for (int i = threadIdx.x; i < n; i += 256) reinterpret_cast<uint4*>(row)[i] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int i = threadIdx.x; i < D; i += 256) row[i] = from_f32<T>(0.f);
+    }
+  }
+}
+
 template <class T, int VEC>
 __device__ __forceinline__ void write_row(T* dst, const float (&s)[VEC], float scale,
                                           int accumulate) {
@@ -331,12 +380,18 @@ __device__ __forceinline__ void write_row(T* dst, const float (&s)[VEC], float s
 }
 
 template <class T, int VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 5)
 run_sum_kernel(const T* __restrict__ g, int64_t dsn, int64_t dsd, const uint32_t* __restrict__ key,
                const uint32_t* __restrict__ pos, int64_t N, int V, int D, float scale,
-               int accumulate, T* __restrict__ dtable, float* __restrict__ parts) {
+               int accumulate, int col_blocks, int64_t sums, T* __restrict__ dtable,
+               float* __restrict__ parts, uint32_t* __restrict__ joins) {
+  if (blockIdx.x >= sums) {
+    clear_rows<T>(key, N, (blockIdx.x - sums) * (int64_t)kClearRows, V, D, VEC > 1, dtable);
+    return;
+  }
   __shared__ uint32_t skey[kRun + 2], spos[kRun];
-  const int64_t base = (int64_t)blockIdx.x * kRun;
+  const int64_t run = blockIdx.x / col_blocks;
+  const int64_t base = run * kRun;
   const int n = (int)min((int64_t)kRun, N - base);
   if (threadIdx.x < kRun + 2) {   // the key before the block's, its keys, and the one behind
     const int64_t i = base + (int)threadIdx.x - 1;
@@ -344,19 +399,24 @@ run_sum_kernel(const T* __restrict__ g, int64_t dsn, int64_t dsd, const uint32_t
   }
   if (threadIdx.x < n) spos[threadIdx.x] = pos[base + threadIdx.x];
   __syncthreads();
-  const int64_t d0 = (blockIdx.y * 256ll + threadIdx.x) * VEC;
+  const int64_t d0 = ((blockIdx.x - run * col_blocks) * 256ll + threadIdx.x) * VEC;
+  // the block's last run began here and goes on: a join for the closing kernel (joins[0]
+  // counts them; their order does not matter, each writes its own row)
+  if (d0 == 0 && n == kRun && skey[kRun] != (uint32_t)V && skey[kRun + 1] == skey[kRun] &&
+      !(skey[1] == skey[kRun] && skey[0] == skey[1]))
+    joins[1 + atomicAdd(&joins[0], 1u)] = (uint32_t)run;
   if (d0 >= D) return;
   float s[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) s[k] = 0.f;
   bool from_before = skey[0] == skey[1];
-  for (int j0 = 0; j0 < n; j0 += 8) {
-    Pack<T, VEC> x[8];
+  for (int j0 = 0; j0 < n; j0 += 4) {
+    Pack<T, VEC> x[4];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < 4; ++u)
       if (j0 + u < n && skey[j0 + u + 1] != (uint32_t)V) x[u].load(g + (int64_t)spos[j0 + u] * dsn + d0 * dsd);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < 4; ++u) {
       const int j = j0 + u;
       if (j >= n || skey[j + 1] == (uint32_t)V) break;
 #pragma unroll
@@ -366,7 +426,7 @@ run_sum_kernel(const T* __restrict__ g, int64_t dsn, int64_t dsd, const uint32_t
       if (ends && !from_before) {
         write_row<T, VEC>(dtable + (int64_t)skey[j + 1] * D + d0, s, scale, accumulate);
       } else {
-        float* dst = parts + (2 * (int64_t)blockIdx.x + (from_before ? 0 : 1)) * D + d0;
+        float* dst = parts + (2 * run + (from_before ? 0 : 1)) * D + d0;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) dst[k] = s[k];
       }
@@ -377,135 +437,141 @@ run_sum_kernel(const T* __restrict__ g, int64_t dsn, int64_t dsd, const uint32_t
   }
 }
 
-// Joins the parts of a run that began in block b and goes on: the part it began
-// with, then one per block up to its end.  32 lanes x 4 columns x 8 part groups.
+// Joins the parts of the runs that blocks cut: the part a run began with, then one
+// per block up to its end.  Blocks take (run, 256 columns) in turn; 512 threads = 8
+// groups of parts x 64 threads of 4 columns.
 template <class T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 join_runs_kernel(const uint32_t* __restrict__ key, int64_t N, int V, int D, float scale,
-                 int accumulate, T* __restrict__ dtable, const float* __restrict__ parts) {
-  const int64_t b = blockIdx.x, end = (b + 1) * kRun;   // first position behind the block
-  if (end >= N) return;
-  const uint32_t v = key[end - 1];
-  if (v == (uint32_t)V || key[end] != v) return;                // nothing goes on
-  const bool whole = key[b * kRun] == v;                        // the block holds nothing else
-  if (whole && b > 0 && key[b * kRun - 1] == v) return;         // it began earlier
+                 int accumulate, T* __restrict__ dtable, const float* __restrict__ parts,
+                 const uint32_t* __restrict__ joins) {
   __shared__ int64_t s_last;
-  if (threadIdx.x == 0) {
-    int64_t lo = end, hi = N;                                   // first position with another id
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (key[mid] == v) lo = mid + 1; else hi = mid;
+  __shared__ float red[8][64][4];
+  const int tiles = (D + 255) / 256;
+  const int64_t units = (int64_t)joins[0] * tiles;
+  const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
+  const bool vec = D % 4 == 0;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t j = u / tiles, b = joins[1 + j], end = (b + 1) * kRun;
+    const uint32_t v = key[end];
+    if (threadIdx.x < 32) {   // first position with another id, 32 probes a round
+      int64_t lo = end, hi = N;
+      while (lo < hi) {
+        const int64_t step = (hi - lo + 31) / 32, at = lo + threadIdx.x * step;
+        const uint32_t same = __ballot_sync(0xffffffffu, at < hi && key[at] == v);
+        const int n = __popc(same);                     // probes of the id: a prefix of the lanes
+        if (n == 0) break;
+        hi = min(hi, lo + n * step);
+        lo += (n - 1) * step + 1;
+      }
+      if (threadIdx.x == 0) s_last = (lo - 1) / kRun;
     }
-    s_last = (lo - 1) / kRun;
-  }
-  __shared__ float red[8][32][4];
-  __syncthreads();
-  const int64_t last = s_last;
-  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
-  const int d0 = (blockIdx.y * 32 + lane) * 4;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  // part i of the run: i = 0 the beginning, i >= 1 block b + i's first
-  for (int64_t i = grp; i <= last - b; i += 8) {
-    const float* src = parts + (i == 0 ? 2 * b + 1 : 2 * (b + i)) * D;
+    __syncthreads();
+    const int64_t count = s_last - b + 1;
+    const int d0 = (int)(u - j * tiles) * 256 + lane * 4;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (d0 < D) {
+#pragma unroll 4
+      for (int64_t i = grp; i < count; i += 8) {
+        // part i of the run: i = 0 the beginning, i >= 1 block b + i's first
+        const float* src = parts + (i == 0 ? 2 * b + 1 : 2 * (b + i)) * D + d0;
+        if (vec) {
+          const float4 x = *reinterpret_cast<const float4*>(src);
+          s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+        } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (d0 + k < D) s[k] += src[d0 + k];
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) red[grp][lane][k] = s[k];
-  __syncthreads();
-  if (grp == 0) {
-    for (int k = 0; k < 4; ++k) {
-      if (d0 + k >= D) break;
-      float t = red[0][lane][k];
-      for (int q = 1; q < 8; ++q) t += red[q][lane][k];
-      T* dst = dtable + (int64_t)v * D + d0 + k;
-      *dst = from_f32<T>(fmaf(t, scale, accumulate ? to_f32(*dst) : 0.f));
+          for (int k = 0; k < 4; ++k)
+            if (d0 + k < D) s[k] += src[k];
+        }
+      }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) red[grp][lane][k] = s[k];
+    __syncthreads();
+    if (grp == 0) {
+      for (int k = 0; k < 4 && d0 + k < D; ++k) {
+        float t = red[0][lane][k];
+        for (int q = 1; q < 8; ++q) t += red[q][lane][k];
+        T* dst = dtable + (int64_t)v * D + d0 + k;
+        *dst = from_f32<T>(fmaf(t, scale, accumulate ? to_f32(*dst) : 0.f));
+      }
+    }
+    __syncthreads();
   }
 }
 
 struct EmbedWs {
-  uint32_t *key[2], *pos[2], *hist;
+  uint32_t *key[2], *pos[2], *hist, *joins;
   float* parts;
   size_t bytes;
   EmbedWs(void* p, int64_t N, int D) {
     WsCarve c(p);
-    const bool long_sort = N > kBlockSortMax;
+    const bool long_sort = N > kClusterSortMax;
     const int64_t nblocks = (N + kSortTile - 1) / kSortTile;
     for (int k = 0; k < 2; ++k) {
       key[k] = c.take<uint32_t>(k == 0 || long_sort ? N : 0);
       pos[k] = c.take<uint32_t>(k == 0 || long_sort ? N : 0);
     }
     hist = c.take<uint32_t>(long_sort ? (size_t)kDigits * nblocks : 0);
+    joins = c.take<uint32_t>(1 + (N + kRun - 1) / kRun);
     parts = c.take<float>((size_t)((N + kRun - 1) / kRun) * 2 * D);
     bytes = c.used;
   }
 };
 
-// Sorts the ids into ws.key[*at], ws.pos[*at], clearing `bytes` of the table on the way.
+template <int ITEMS>
+cudaError_t cluster_sort(const int64_t* ids, int64_t ignore, int64_t N, int V, int bits,
+                         int digit_bits, const EmbedWs& ws, cudaStream_t stream) {
+  const size_t smem = (size_t)kClusterSortThreads * ITEMS * 8 + 32 * kDigits * 2;
+  auto* kernel = cluster_sort_kernel<ITEMS>;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  int blocks = 1;
+  while ((int64_t)blocks * kClusterSortThreads * ITEMS < N) blocks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kClusterSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, kernel, ids, ignore, V, (int)N, bits, digit_bits, ws.key[0],
+                            ws.pos[0], ws.joins);
+}
+
+// Sorts the ids into ws.key[*at], ws.pos[*at].
 cudaError_t sort_ids(const int64_t* ids, int64_t ignore, int64_t N, int V, const EmbedWs& ws,
-                     void* table, size_t bytes, cudaStream_t stream, int* at) {
+                     cudaStream_t stream, int* at) {
   int bits = 1;
   while ((int64_t(1) << bits) <= V) ++bits;    // keys 0 .. V
   const int passes = (bits + kDigitBits - 1) / kDigitBits;
   const int digit_bits = (bits + passes - 1) / passes;
-  const uint32_t mask = (1u << digit_bits) - 1u;
-  // 16-byte units of the table between its first and last aligned address, in as many
-  // shares as there are launches; the ragged ends (under 16 bytes each) by memset
-  char* p0 = static_cast<char*>(table);
-  const int launches = N <= kBlockSortMax ? 1 : 3 * passes;
-  size_t head = 0, units = 0;
-  if (bytes > 0) {
-    head = std::min<size_t>(bytes, (16 - (reinterpret_cast<uintptr_t>(p0) & 15)) & 15);
-    units = (bytes - head) / 16;
-    const size_t tail = bytes - head - 16 * units;
-    cudaError_t e = cudaSuccess;
-    if (head) e = cudaMemsetAsync(p0, 0, head, stream);
-    if (tail && e == cudaSuccess) e = cudaMemsetAsync(p0 + head + 16 * units, 0, tail, stream);
-    if (e != cudaSuccess) return e;
-  }
-  const int64_t share = ((int64_t)units + launches - 1) / launches;
-  int64_t filled = 0;
-  auto next_fill = [&](int first, int threads) {
-    Fill f;
-    f.ptr = reinterpret_cast<uint4*>(p0 + head) + filled;
-    f.n = std::min<int64_t>(share, (int64_t)units - filled);
-    f.first = first;
-    filled += f.n;
-    const int64_t blocks = std::min<int64_t>((f.n + 4 * threads - 1) / (4 * threads),
-                                             (int64_t)num_sms() * (2048 / threads));
-    return std::make_pair(f, (unsigned)(first + blocks));
-  };
   *at = 0;
-  if (N <= kBlockSortMax) {
+  if (N <= kClusterSortMax) {
+    // few ids a thread: the ranking's rounds are the time of a pass
     auto run = [&](auto items) {
-      constexpr int ITEMS = decltype(items)::value;
-      const size_t smem = (size_t)kBlockSortThreads * ITEMS * 8 + 32 * kDigits * 2;
-      cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(block_sort_kernel<ITEMS>), smem);
-      if (e != cudaSuccess) return e;
-      const auto f = next_fill(1, kBlockSortThreads);
-      block_sort_kernel<ITEMS><<<f.second, kBlockSortThreads, smem, stream>>>(
-          ids, ignore, V, (int)N, bits, digit_bits, ws.key[0], ws.pos[0], f.first);
-      count_launches(1);
-      return cudaSuccess;
+      return cluster_sort<decltype(items)::value>(ids, ignore, N, V, bits, digit_bits, ws, stream);
     };
-    if (N <= 1024) return run(std::integral_constant<int, 1>{});
-    if (N <= 4096) return run(std::integral_constant<int, 4>{});
+    constexpr int64_t full = (int64_t)kClusterSortThreads * kClusterSortBlocks;
+    if (N <= 2 * full) return run(std::integral_constant<int, 2>{});
+    if (N <= 8 * full) return run(std::integral_constant<int, 8>{});
     return run(std::integral_constant<int, 16>{});
   }
+  const uint32_t mask = (1u << digit_bits) - 1u;
   const int nblocks = (int)((N + kSortTile - 1) / kSortTile);
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
     const SortIn in{pass == 0 ? ids : nullptr, ignore, V, ws.key[*at], ws.pos[*at]};
     const int to = pass == 0 ? 0 : *at ^ 1;
-    auto f = next_fill(nblocks, kSortThreads);
-    sort_count_kernel<<<f.second, kSortThreads, 0, stream>>>(in, N, shift, mask, ws.hist, nblocks, f.first);
-    f = next_fill(1, 1024);
-    sort_scan_kernel<<<f.second, 1024, 0, stream>>>(ws.hist, (int64_t)kDigits * nblocks, f.first);
-    f = next_fill(nblocks, kSortThreads);
-    sort_scatter_kernel<<<f.second, kSortThreads, 0, stream>>>(in, N, shift, mask, ws.hist, nblocks,
-                                                              ws.key[to], ws.pos[to], f.first);
+    sort_count_kernel<<<nblocks, kSortThreads, 0, stream>>>(in, N, shift, mask, ws.hist, nblocks);
+    sort_scan_kernel<<<1, 1024, 0, stream>>>(ws.hist, (int64_t)kDigits * nblocks, ws.joins);
+    sort_scatter_kernel<<<nblocks, kSortThreads, 0, stream>>>(in, N, shift, digit_bits, ws.hist,
+                                                             nblocks, ws.key[to], ws.pos[to]);
     count_launches(3);
     *at = to;
   }
@@ -549,17 +615,16 @@ int fgmm_embed_fwd(int type, const void* table, int64_t t_stride_v, int64_t t_st
       cudaStream_t st = (cudaStream_t)stream;
       const bool vec = rows_vec(table, t_stride_v, t_stride_d, D, sizeof(T)) &&
                        rows_vec(out, D, 1, D, sizeof(T));
-      // a block per 256 pieces while they all fit on the SMs at once, then four each
-      const int64_t pieces = N * (vec ? D / VEC : D);
-      const int blocks = (int)std::max<int64_t>(
-          std::min<int64_t>((pieces + 255) / 256, 8 * num_sms()),
-          std::min<int64_t>((pieces + 1023) / 1024, 1 << 20));
+      int lanes = 1;
+      while (lanes < 256 && lanes < (vec ? D / VEC : D)) lanes *= 2;
+      const int64_t per_block = 4 * (256 / lanes);
+      const int blocks = (int)std::min<int64_t>((N + per_block - 1) / per_block, 1 << 20);
       if (vec)
         lookup_kernel<T, VEC><<<blocks, 256, 0, st>>>(t, t_stride_v, t_stride_d, ids, ignore_index,
-                                                      N, V, D, scale, o);
+                                                      N, V, D, scale, lanes, o);
       else
         lookup_kernel<T, 1><<<blocks, 256, 0, st>>>(t, t_stride_v, t_stride_d, ids, ignore_index, N,
-                                                    V, D, scale, o);
+                                                    V, D, scale, lanes, o);
       count_launches(1);
     });
     cudaError_t e = cudaGetLastError();
@@ -600,13 +665,12 @@ int fgmm_embed_bwd(int type, const void* dout, int64_t d_stride_n, int64_t d_str
     if (rc != FGMM_OK) return rc;
     const int accumulate = (flags & FGMM_FLAG_ACCUMULATE) ? 1 : 0;
     cudaStream_t st = (cudaStream_t)stream;
-    const size_t bytes = accumulate ? 0 : (size_t)V * D * type_size(type);
     cudaError_t e = cudaSuccess;
     if (N == 0) {
-      if (bytes) e = cudaMemsetAsync(dtable, 0, bytes, st);
+      if (!accumulate) e = cudaMemsetAsync(dtable, 0, (size_t)V * D * type_size(type), st);
     } else {
       int at = 0;
-      e = sort_ids(ids, ignore_index, N, V, ws, dtable, bytes, st, &at);
+      e = sort_ids(ids, ignore_index, N, V, ws, st, &at);
       if (e == cudaSuccess) with_type(type, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         constexpr int VEC = 16 / sizeof(T);
@@ -615,18 +679,17 @@ int fgmm_embed_bwd(int type, const void* dout, int64_t d_stride_n, int64_t d_str
         const unsigned runs = (unsigned)((N + kRun - 1) / kRun);
         const bool vec = rows_vec(dout, d_stride_n, d_stride_d, D, sizeof(T)) &&
                          rows_vec(dtable, D, 1, D, sizeof(T));
-        const unsigned cols = 256 * (vec ? VEC : 1);
-        const dim3 grid(runs, (D + cols - 1) / cols);
-        if (vec)
-          run_sum_kernel<T, VEC><<<grid, 256, 0, st>>>(g, d_stride_n, d_stride_d, ws.key[at], ws.pos[at],
-                                                       N, V, D, scale, accumulate, out, ws.parts);
-        else
-          run_sum_kernel<T, 1><<<grid, 256, 0, st>>>(g, d_stride_n, d_stride_d, ws.key[at], ws.pos[at], N,
-                                                     V, D, scale, accumulate, out, ws.parts);
+        const int cols = 256 * (vec ? VEC : 1), col_blocks = (D + cols - 1) / cols;
+        const int64_t sums = (int64_t)runs * col_blocks;
+        const unsigned grid = (unsigned)(sums + (accumulate ? 0 : ((int64_t)V + kClearRows - 1) / kClearRows));
+        auto* kernel = vec ? run_sum_kernel<T, VEC> : run_sum_kernel<T, 1>;
+        kernel<<<grid, 256, 0, st>>>(g, d_stride_n, d_stride_d, ws.key[at], ws.pos[at], N, V, D,
+                                     scale, accumulate, col_blocks, sums, out, ws.parts, ws.joins);
         count_launches(1);
         if (runs > 1) {
-          join_runs_kernel<T><<<dim3(runs - 1, (D + 127) / 128), 256, 0, st>>>(
-              ws.key[at], N, V, D, scale, accumulate, out, ws.parts);
+          const int64_t most = (int64_t)(runs - 1) * ((D + 255) / 256);
+          join_runs_kernel<T><<<(unsigned)std::min<int64_t>(most, 4 * num_sms()), 512, 0, st>>>(
+              ws.key[at], N, V, D, scale, accumulate, out, ws.parts, ws.joins);
           count_launches(1);
         }
       });

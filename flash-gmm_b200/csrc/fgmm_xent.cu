@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const XentArgs a, const Xent
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t base = (int64_t)blockIdx.x * kRowsPerBlock;
   int before = 0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < base; i += 1024) before += a.targets[i] != a.ignore;
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) wsum[warp] = before;
@@ -223,39 +224,63 @@ __global__ void __launch_bounds__(1024) rows_kernel(const XentArgs a, const Xent
   }
 }
 
-// Largest finite magnitude of the listed rows (of every row without a list).
+// Largest finite magnitude of the listed rows (of every row without a list); a
+// warp takes four rows at a time, 16 bytes a lane where the layout allows (vec).
 __global__ void __launch_bounds__(256)
 amax_kernel(const float* __restrict__ A, int64_t s0, int64_t s1, int D, int64_t n,
-            const int* __restrict__ rows, const int* __restrict__ live, int* __restrict__ amax) {
+            const int* __restrict__ rows, const int* __restrict__ live, int vec,
+            int* __restrict__ amax) {
   if (live) n = *live;
+  const int lane = threadIdx.x & 31;
   float m = 0.f;
-  const int64_t total = n * D;
-  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
-    const int64_t i = e / D;
-    const float x = fabsf(A[(rows ? rows[i] : i) * s0 + (e - i * D) * s1]);
+  auto see = [&](float x) {
+    x = fabsf(x);
     if (x < INFINITY) m = fmaxf(m, x);
+  };
+  for (int64_t i0 = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * 4; i0 < n; i0 += gridDim.x * 32ll) {
+    const float* row[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = min(i0 + u, n - 1);
+      row[u] = A + (rows ? rows[i] : i) * s0;
+    }
+    if (vec) {
+      for (int d = lane * 4; d < D; d += 128) {
+        float4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const float4*>(row[u] + d);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) { see(x[u].x); see(x[u].y); see(x[u].z); see(x[u].w); }
+      }
+    } else {
+      for (int d = lane; d < D; d += 32) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) see(row[u][d * s1]);
+      }
+    }
   }
   m = redux_max(m);
-  if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(amax, __float_as_int(m));
+  if (lane == 0 && m > 0.f) atomicMax(amax, __float_as_int(m));
 }
 
 // Dense copies of X's live rows (rows != null; zero rows up to a multiple of
 // kPairRows) or of W, D padded with zeros to Dp; fp32 becomes two fp16 words of
-// the value / 2^e.  One thread per 8 elements.
+// the value / 2^e.  8 elements a thread, `lanes` threads (a power of two) a row.
 template <class T>
 __global__ void __launch_bounds__(256)
 pack_kernel(const T* __restrict__ A, int64_t s0, int64_t s1, int D, int Dp, int64_t n,
-            const int* __restrict__ rows, const int* __restrict__ live, int vec,
+            const int* __restrict__ rows, const int* __restrict__ live, int vec, int lanes,
             const int* __restrict__ amax, uint16_t* __restrict__ out, uint16_t* __restrict__ out2) {
   constexpr bool kSplit = sizeof(T) == 4;
   if (live) n = ((int64_t)*live + kPairRows - 1) / kPairRows * kPairRows;
-  const int per_row = Dp / 8;
-  const int64_t total = n * per_row;
+  const int per_row = Dp / 8, per_block = 256 / lanes;
   const float scale = kSplit ? ldexpf(1.f, -Scales::exponent(*amax, 14)) : 1.f;
-  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
-    const int64_t i = e / per_row;
-    const int d0 = (int)(e - i * per_row) * 8;
+  for (int64_t i = blockIdx.x * (int64_t)per_block + threadIdx.x / lanes; i < n;
+       i += gridDim.x * (int64_t)per_block) {
     const int64_t r = rows ? rows[i] : i;
+    for (int c = threadIdx.x % lanes; c < per_row; c += lanes) {
+    const int64_t e = i * per_row + c;
+    const int d0 = c * 8;
     uint4 w = make_uint4(0u, 0u, 0u, 0u), w2 = w;
     if (r >= 0) {
       const T* src = A + r * s0 + (int64_t)d0 * s1;
@@ -282,6 +307,7 @@ pack_kernel(const T* __restrict__ A, int64_t s0, int64_t s1, int D, int Dp, int6
     }
     reinterpret_cast<uint4*>(out)[e] = w;
     if (kSplit) reinterpret_cast<uint4*>(out2)[e] = w2;
+    }
   }
 }
 
@@ -328,8 +354,9 @@ __global__ void __launch_bounds__(256) finish_forward_kernel(const XentArgs a, c
   const bool on = i < live;
   float m = -3.402823466e38f, s = 0.f;
   if (on)
+#pragma unroll 8
     for (int k = warp; k < 2 * w.splits; k += 8) {
-      const float2 p = w.part[(int64_t)k * w.Np + i];
+      const float2 p = __ldg(&w.part[(int64_t)k * w.Np + i]);
       const float mn = fmaxf(m, p.x);
       s = s * ex2((m - mn) * kLog2Ef) + p.y * ex2((p.x - mn) * kLog2Ef);
       m = mn;
@@ -418,13 +445,22 @@ store_slots_kernel(const float* __restrict__ slots, int ks, int64_t slot_rows, i
   }
 }
 
-// dbias from the 128-row partial sums, in row order (NaN if a wait gave up).
-__global__ void __launch_bounds__(256) store_dbias_kernel(const XentArgs a, const XentWs w) {
-  const float back = 1.f / Scales(w.hdr->amax, a.type != FGMM_T_BF16, a.type == FGMM_T_F32).g;
+// dbias from the 128-row partial sums (NaN if a wait gave up): 32 entries a block,
+// 32 warps that take the parts in turn, joined in warp order.
+__global__ void __launch_bounds__(1024) store_dbias_kernel(const XentArgs a, const XentWs w) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nparts = (int)(((int64_t)w.hdr->live + kPairRows - 1) / kPairRows) * 2;
-  for (int64_t v = blockIdx.x * 256ll + threadIdx.x; v < a.V; v += gridDim.x * 256ll) {
-    float s = 0.f;
-    for (int k = 0; k < nparts; ++k) s += w.dbias_part[(int64_t)k * w.Vp + v];
+  const int64_t v = blockIdx.x * 32ll + lane;      // < Vp
+  float s = 0.f;
+#pragma unroll 4
+  for (int k = warp; k < nparts; k += 32) s += w.dbias_part[(int64_t)k * w.Vp + v];
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && v < a.V) {
+    s = red[0][lane];
+    for (int k = 1; k < 32; ++k) s += red[k][lane];
+    const float back = 1.f / Scales(w.hdr->amax, a.type != FGMM_T_BF16, a.type == FGMM_T_F32).g;
     a.dbias[v] = w.hdr->err ? __int_as_float(0x7fffffff) : s * back;
   }
 }
@@ -493,24 +529,30 @@ cudaError_t prepare_operands(const XentArgs& a, const XentWs& w, MmaMaps* maps) 
   const T* X = static_cast<const T*>(a.X);
   const T* W = static_cast<const T*>(a.W);
   const int* live = &w.hdr->live;
+  auto vec = [&](const void* p, int64_t s0, int64_t s1, int whole) {
+    return s1 == 1 && s0 * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 &&
+           a.D % whole == 0;
+  };
   if (kSplit) {
-    amax_kernel<<<grid_for(a.N * a.D / 4), 256, 0, a.stream>>>(
-        reinterpret_cast<const float*>(X), a.sxn, a.sxd, a.D, a.N, w.rows, live, &w.hdr->amax[1]);
-    amax_kernel<<<grid_for((int64_t)a.V * a.D / 4), 256, 0, a.stream>>>(
-        reinterpret_cast<const float*>(W), a.swv, a.swd, a.D, a.V, nullptr, nullptr, &w.hdr->amax[2]);
+    auto blocks = [&](int64_t n) { return (int)std::min<int64_t>((n + 31) / 32, 8 * num_sms()); };
+    amax_kernel<<<blocks(a.N), 256, 0, a.stream>>>(
+        reinterpret_cast<const float*>(X), a.sxn, a.sxd, a.D, a.N, w.rows, live,
+        vec(X, a.sxn, a.sxd, 4), &w.hdr->amax[1]);
+    amax_kernel<<<blocks(a.V), 256, 0, a.stream>>>(
+        reinterpret_cast<const float*>(W), a.swv, a.swd, a.D, a.V, nullptr, nullptr,
+        vec(W, a.swv, a.swd, 4), &w.hdr->amax[2]);
     count_launches(2);
   }
-  auto vec = [&](const void* p, int64_t s0, int64_t s1) {
-    return s1 == 1 && s0 * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
-  };
-  pack_kernel<T><<<grid_for(w.Np * (w.Dp / 8)), 256, 0, a.stream>>>(
-      X, a.sxn, a.sxd, a.D, w.Dp, 0, w.rows, live, vec(X, a.sxn, a.sxd), &w.hdr->amax[1],
+  int lanes = 1;
+  while (lanes < 256 && lanes < w.Dp / 8) lanes *= 2;
+  pack_kernel<T><<<grid_for(w.Np * lanes), 256, 0, a.stream>>>(
+      X, a.sxn, a.sxd, a.D, w.Dp, 0, w.rows, live, vec(X, a.sxn, a.sxd, 1), lanes, &w.hdr->amax[1],
       static_cast<uint16_t*>(w.Xp), static_cast<uint16_t*>(w.Xp2));
   count_launches(2);
   if (w.pack_w) {
-    pack_kernel<T><<<grid_for((int64_t)a.V * (w.Dp / 8)), 256, 0, a.stream>>>(
-        W, a.swv, a.swd, a.D, w.Dp, a.V, nullptr, nullptr, vec(W, a.swv, a.swd), &w.hdr->amax[2],
-        static_cast<uint16_t*>(w.Wp), static_cast<uint16_t*>(w.Wp2));
+    pack_kernel<T><<<grid_for((int64_t)a.V * lanes), 256, 0, a.stream>>>(
+        W, a.swv, a.swd, a.D, w.Dp, a.V, nullptr, nullptr, vec(W, a.swv, a.swd, 1), lanes,
+        &w.hdr->amax[2], static_cast<uint16_t*>(w.Wp), static_cast<uint16_t*>(w.Wp2));
     count_launches(1);
   }
   if (a.bias) {
@@ -644,7 +686,7 @@ cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
     count_launches(1);
   }
   if (a.dbias) {
-    store_dbias_kernel<<<grid_for(a.V), 256, 0, a.stream>>>(a, w);
+    store_dbias_kernel<<<(unsigned)((a.V + 31) / 32), 1024, 0, a.stream>>>(a, w);
     count_launches(1);
   }
   if (a.dW) {
