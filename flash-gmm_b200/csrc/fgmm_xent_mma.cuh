@@ -144,9 +144,11 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
       "h"((uint16_t)3)
       : "memory");
 }
+// What an epilogue warp hands back is TMEM it has read (tcgen05.wait::ld and the
+// tcgen05 fence order that): nothing of its memory writes, so no cluster-wide release,
+// which cost about 900 cycles a tile.
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
-               : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 
 // K-blocks that the accumulator takes before it is emptied into registers.
@@ -284,6 +286,38 @@ __device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
   return v[0];
 }
 
+// Two fp32 values in one register pair: Blackwell's packed add, multiply and FMA take
+// one issue slot for both.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack(F2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 exp2_pair(F2 x) {
+  float a, b;
+  unpack(x, a, b);
+  return f2(ex2(a), ex2(b));
+}
+
 __device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&v)[32]) {
   uint32_t u[32];
   tmem_ld32(taddr, u);
@@ -344,7 +378,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-    return mbar_wait_flag<true>(bar, parity, &ctl->abort_flag, p.err, code);
+    return mbar_wait_flag(bar, parity, &ctl->abort_flag, p.err, code);
   };
 
   if (warp < 4) {
@@ -545,9 +579,9 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
             for (int i = 0; i < 32; ++i) x = tc == 32 * c + i ? acc[c][i] : x;
           if (mine) p.tlogit[row] = x;
         }
-        float m8[8], s8[8];
+        float m8[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) { m8[k] = acc[0][k]; s8[k] = 0.f; }
+        for (int k = 0; k < 8; ++k) m8[k] = acc[0][k];
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -557,19 +591,26 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         const float mn = fmaxf(m_run, mx);
         s_run *= ex2((m_run - mn) * kLog2Ef);
         m_run = mn;
-        if (p.bias) {   // differences first: a bias may be the lowest float
+        if (p.bias) {   // differences first, and exact zeros: a bias may be the lowest float
+          float s8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i) s8[i & 7] += ex2((acc[c][i] - mn) * kLog2Ef);
+          s_run += ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
         } else {
           const float nm = fminf(-mn, 2e38f) * kLog2Ef;   // finite where every entry is masked
+          const F2 l2 = f2(kLog2Ef, kLog2Ef), nm2 = f2(nm, nm);
+          F2 s4[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s8[i & 7] += ex2(fmaf(acc[c][i], kLog2Ef, nm));
+            for (int j = 0; j < 16; ++j)
+              s4[j & 3] = add2(s4[j & 3], exp2_pair(fma2(f2(acc[c][2 * j], acc[c][2 * j + 1]), l2, nm2)));
+          float sa, sb;
+          unpack(add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])), sa, sb);
+          s_run += sa + sb;
         }
-        s_run += ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
         if (t.last) p.part[(int64_t)(2 * t.ks + half) * p.Np + row] = make_float2(m_run, s_run);
         continue;
       }
@@ -580,17 +621,23 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         const int v0 = (int)t.brow + col0;
         const int vend = p.cur.v0 + p.cur.nv;
         const float ga = rg.a * scales.g, gb = rg.b * scales.g;
-        if (SPLIT || p.bias) {
+        if (p.bias) {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i) acc[c][i] = ga * ex2((acc[c][i] - rg.lse) * kLog2Ef);
         } else {
-          const float nl = -rg.lse * kLog2Ef;
+          // bf16 and fp16 words hide the rounding of lse log2(e) in the product's FMA
+          const F2 l2 = f2(kLog2Ef, kLog2Ef), ga2 = f2(ga, ga);
+          const F2 off = SPLIT ? f2(-rg.lse, -rg.lse) : f2(-rg.lse * kLog2Ef, -rg.lse * kLog2Ef);
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c][i] = ga * ex2(fmaf(acc[c][i], kLog2Ef, nl));
+            for (int j = 0; j < 16; ++j) {
+              const F2 v = f2(acc[c][2 * j], acc[c][2 * j + 1]);
+              const F2 x = SPLIT ? mul2(add2(v, off), l2) : fma2(v, l2, off);
+              unpack(mul2(exp2_pair(x), ga2), acc[c][2 * j], acc[c][2 * j + 1]);
+            }
         }
         const int tc = rg.target - v0;
         if (__any_sync(0xffffffffu, tc >= 0 && tc < BN / 2)) {
