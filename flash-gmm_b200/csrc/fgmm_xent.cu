@@ -89,7 +89,7 @@ struct XentWs {
   int64_t Np, Vp;
   int Dp;                          // row length of the packed operands
   bool split, pack_w;
-  int bn, vtiles, per_split, splits;
+  int vtiles, per_split, splits;
   int bn_d, tiles_d;
   int64_t ldS;
   int row_chunk, piece, n_chunks, n_pieces, ks_x, ks_w;
@@ -107,7 +107,6 @@ struct XentWs {
     Np = std::max<int64_t>((N + kPairRows - 1) / kPairRows * kPairRows, kPairRows);
     Vp = ((int64_t)V + 255) / 256 * 256;
     Dp = (D + 7) / 8 * 8;
-    bn = split ? MmaCfg<true>::kBN : MmaCfg<false>::kBN;
     // W is read in place when TMA can: unit feature stride, rows of whole 16-byte units
     pack_w = split || swd != 1 || swv < D || swv % 8 != 0 || swv >= (int64_t(1) << 38) ||
              (reinterpret_cast<uintptr_t>(W) & 15) != 0;
@@ -124,7 +123,7 @@ struct XentWs {
     if (!backward) {
       // Vocabulary tiles per unit: the fewest rounds of the pairs, counting a quarter
       // of a tile per unit for what starting and ending one costs.
-      vtiles = (int)(((int64_t)V + bn - 1) / bn);
+      vtiles = (int)(((int64_t)V + kBN - 1) / kBN);
       double best = 1e300;
       for (int splits_ = 1; splits_ <= std::min(vtiles, 4 * kPairs); ++splits_) {
         const int per = (vtiles + splits_ - 1) / splits_, got = (vtiles + per - 1) / per;
@@ -138,7 +137,7 @@ struct XentWs {
     } else {
       const int word = split ? 4 : 2;
       // column tiles of dX and dW: 128 wide where that pads D less
-      bn_d = split || (D + 127) / 128 * 128 < (D + 255) / 256 * 256 ? 128 : 256;
+      bn_d = (D + 127) / 128 * 128 < (D + 255) / 256 * 256 ? 128 : 256;
       tiles_d = (D + bn_d - 1) / bn_d;
       ldS = (int64_t)tiles_d * bn_d;
       // G in pieces of at most kPieceBytes: all rows x at least 2048 entries if possible
@@ -587,10 +586,11 @@ template <bool FWD, class T>
 cudaError_t launch_mma(const XentArgs& a, const MmaParams& p, const MmaMaps& maps, int64_t units) {
   constexpr bool kSplit = sizeof(T) == 4;
   auto* kernel = xent_mma_kernel<FWD, kSplit, typename Word<T>::type, T>;
-  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), MmaCfg<kSplit>::kSmem);
+  constexpr size_t smem = MmaCfg<kSplit>::kSmem;
+  cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   const int pairs = (int)std::min<int64_t>(units, num_sms() / 2);
-  kernel<<<2 * pairs, kMmaThreads, MmaCfg<kSplit>::kSmem, a.stream>>>(p, maps);
+  kernel<<<2 * pairs, kMmaThreads, smem, a.stream>>>(p, maps);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -668,7 +668,7 @@ cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
     maps.G = gmap[(j & 1) ^ 1];
     maps.G2 = gmap2[(j & 1) ^ 1];
     const int64_t units =
-        (p.has_grad ? (int64_t)(p.cur.rows / 256) * ((p.cur.nv + w.bn - 1) / w.bn) : 0) +
+        (p.has_grad ? (int64_t)(p.cur.rows / 256) * ((p.cur.nv + kBN - 1) / kBN) : 0) +
         (p.has_dx ? (int64_t)(p.prev.rows / 256) * w.tiles_d * w.ks_x : 0) +
         (p.has_dw ? (int64_t)((p.prev.nv + 255) / 256) * w.tiles_d * w.ks_w : 0);
     e = launch_mma<false, T>(a, p, maps, units);

@@ -25,9 +25,16 @@
 // round to nearest.  Products with G stored in 16 bits are not: their words' rounding
 // of 2^-9 or 2^-12 outweighs a chain's 2^-14.
 //
-// Warps: 0 TMA loads, 1 MMA (the pair's first SM), 2 TMEM, 4-11 epilogue (TMEM lane
-// quadrant = warp & 3, column half = (warp - 4) >> 2).  Every wait is bounded; a
-// timeout sets the error word, all roles leave, and the closing kernels write NaN.
+// Warps: 0 TMA loads, 1 MMA (the pair's first SM), 2 TMEM, 4-11 epilogue in two
+// warpgroups (TMEM lane quadrant = warp & 3) that take a tile's halves, 128 columns of
+// a row per thread.  Every wait is bounded; a timeout sets the error word, all roles
+// leave, and the closing kernels write NaN.
+//
+// Measured and not kept: 128-wide tiles that the warpgroups take in turn (so that one's
+// exponentials overlap the other's waits): an M = 256, N = 128 step reads shared memory
+// at its full rate, 65536 x 8192 x 256 bf16 logits 285 -> 444 us.  Three of eight
+// exponentials as a polynomial on the FMA pipe: 303 -> 317 us at D = 64; the epilogue is
+// bound by its dependent latencies, not by the special-function unit (50% busy).
 
 constexpr int kPairRows = 256;
 constexpr int kBoxBytes = 64 * 128;
@@ -175,10 +182,11 @@ __device__ __forceinline__ void idle_cycles(long long n) {
   while (clock64() - t0 < n) {}
 }
 
+constexpr int kBN = 256;          // widest tile: the width of logits
+
 template <bool SPLIT>
 struct MmaCfg {
-  static constexpr int kBN = SPLIT ? 128 : 256;              // widest tile
-  static constexpr int kStages = SPLIT ? 4 : 6;
+  static constexpr int kStages = SPLIT ? 3 : 6;
   static constexpr int kA = 2 * kBoxBytes;                   // 128 rows x 64
   static constexpr int kB = (kBN / 2 / 64) * kBoxBytes;      // this SM's half of B
   static constexpr int kStage = (SPLIT ? 2 : 1) * (kA + kB);
@@ -200,7 +208,7 @@ template <bool FWD, bool SPLIT>
 struct TileWalk {
   const MmaParams& p;
   int64_t live;
-  int unit, step, sub = 0;
+  int unit, step, sub = 0, um = 0, us = 0;
   int mt, mtx, n_dw, n_dx, n_grad, units;
   __device__ TileWalk(const MmaParams& p_, int pair, int npairs) : p(p_), unit(pair), step(npairs) {
     live = *p.live;
@@ -216,21 +224,21 @@ struct TileWalk {
       mt = tiles(p.cur);
       n_dw = p.has_dw ? (p.prev.nv + kPairRows - 1) / kPairRows * p.tiles_d * p.ks_w : 0;
       n_dx = p.has_dx ? mtx * p.tiles_d * p.ks_x : 0;
-      n_grad = p.has_grad ? mt * ((p.cur.nv + MmaCfg<SPLIT>::kBN - 1) / MmaCfg<SPLIT>::kBN) : 0;
+      n_grad = p.has_grad ? mt * ((p.cur.nv + kBN - 1) / kBN) : 0;
       units = n_dw + n_dx + n_grad;
     }
   }
   __device__ bool next(Tile& t) {
-    constexpr int BN = MmaCfg<SPLIT>::kBN;
     if (unit >= units) return false;
     if (FWD) {
-      const int m = unit % mt, s = unit / mt;
+      if (sub == 0) { us = unit / mt; um = unit - us * mt; }
+      const int m = um, s = us;
       const int v = s * p.per_split + sub;
       t.kind = kLse;
       t.m = m; t.n = v; t.ks = s;
       t.arow = (int64_t)m * kPairRows; t.ak = 0;
-      t.brow = (int64_t)v * BN; t.bk = 0;
-      t.nkb = p.kbD; t.bn = BN;
+      t.brow = (int64_t)v * kBN; t.bk = 0;
+      t.nkb = p.kbD; t.bn = kBN;
       ++sub;
       t.last = sub == p.per_split || v + 1 == p.vtiles;
       if (t.last) { sub = 0; unit += step; }
@@ -265,8 +273,8 @@ struct TileWalk {
       t.kind = kGrad;
       t.m = u % mt; t.n = u / mt; t.ks = 0;
       t.arow = p.cur.r0 + (int64_t)t.m * kPairRows; t.ak = 0;                // of Xp
-      t.brow = p.cur.v0 + (int64_t)t.n * BN; t.bk = 0;                       // of W
-      t.nkb = p.kbD; t.bn = BN;
+      t.brow = p.cur.v0 + (int64_t)t.n * kBN; t.bk = 0;                       // of W
+      t.nkb = p.kbD; t.bn = kBN;
     }
     return true;
   }
@@ -343,7 +351,7 @@ template <bool FWD, bool SPLIT, class T, class TO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1)
 xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ MmaMaps maps) {
   using Cfg = MmaCfg<SPLIT>;
-  constexpr int NS = Cfg::kStages, BN = Cfg::kBN;
+  constexpr int NS = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -434,7 +442,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
                                ((uint32_t)(t.bn >> 3) << 17) | (16u << 24);
         const int group = group_blocks<SPLIT, f16>(p, t);
         for (int k0 = 0; ok && k0 < t.nkb; k0 += group, ++ac) {
-          const uint32_t d = tmem + 256u * (ac & 1);
+          const uint32_t d = tmem + (uint32_t)kBN * (ac & 1);
           if (ac >= 2 && !wait(&ctl->acc_empty[ac & 1], ((ac >> 1) - 1) & 1, 4)) { ok = false; break; }
           tc_fence_after();
           const int k1 = min(t.nkb, k0 + group);
@@ -477,36 +485,47 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     TileWalk<FWD, SPLIT> walk(p, pair, npairs);
     Tile t;
     uint32_t ac = 0;
-    const int q = warp & 3, half = (warp - 4) >> 2;
+    const int q = warp & 3, wg = (warp - 4) >> 2;
     const int row_in = 128 * (int)rank + 32 * q + lane;     // row of the 256-row tile
     const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
     uint8_t* stage = out_stage + (warp - 4) * 4096;
-    const uint32_t empty_at[2] = {map_to_cta(smem_u32(&ctl->acc_empty[0]), 0),
-                                  map_to_cta(smem_u32(&ctl->acc_empty[1]), 0)};
+    const uint32_t empty0 = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
     constexpr bool f16 = std::is_same<T, __half>::value;
     const Scales scales(p.amax, f16, SPLIT);
     const float sc_s = scales.s;
     float m_run = -3.402823466e38f, s_run = 0.f;            // kLse, over the unit's tiles
     int target = -1;
-    constexpr int kChunks = BN / 2 / 32;                    // 32-column chunks per warp
+    constexpr int kCols = 128;                              // columns per warp
+    constexpr int kChunks = kCols / 32;
 
     auto release = [&](uint32_t a) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_cluster(empty_at[a & 1]);
+      if (lane == 0) arrive_cluster(empty0 + 8u * (a & 1));
+    };
+    auto wg_sync = [&] {   // the warpgroup's 128 threads
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
     };
     bool ok = true;
     while (ok && walk.next(t)) {
-      const int cols = t.bn / 2, col0 = half * cols;        // this warp's columns of the tile
-      const int chunks = cols / 32;
+      const int col0 = wg * (t.bn / 2);                     // this warp's columns of the tile
+      const int chunks = t.bn / 2 / 32;
+      const int group = group_blocks<SPLIT, f16>(p, t);
+      const int64_t row = t.arow + row_in;                  // kLse, kGrad: the live row
+      if (FWD && t.n == t.ks * p.per_split) {               // first tile of the unit
+        m_run = -3.402823466e38f;
+        s_run = 0.f;
+        target = p.target[row];
+      }
+      RowGrad rg;
+      if (!FWD && t.kind == kGrad) rg = p.rg[row];          // in flight while the MMAs run
       // The tile's products of this thread's row, in registers; the accumulator is given
       // back before they are worked on.
       float acc[kChunks][32];
-      const int group = group_blocks<SPLIT, f16>(p, t);
       for (int k0 = 0; ok && k0 < t.nkb; k0 += group, ++ac) {
         if (!__all_sync(0xffffffffu, wait(&ctl->acc_full[ac & 1], (ac >> 1) & 1, 32))) ok = false;
         tc_fence_after();
-        const uint32_t at = lanes + 256u * (ac & 1) + col0;
+        const uint32_t at = lanes + (uint32_t)kBN * (ac & 1) + col0;
         if (k0 == 0) {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
@@ -555,14 +574,8 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       }
 
       if (FWD) {
-        const int64_t row = t.arow + row_in;
         const int v0 = (int)t.brow + col0;
-        if (t.n == t.ks * p.per_split) {   // first tile of the unit
-          m_run = -3.402823466e38f;
-          s_run = 0.f;
-          target = p.target[row];
-        }
-        if (v0 + BN / 2 > p.V) {
+        if (v0 + kCols > p.V) {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -570,7 +583,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
               if (v0 + 32 * c + i >= p.V) acc[c][i] = __int_as_float(0xff800000);
         }
         const int tc = target - v0;
-        const bool mine = tc >= 0 && tc < BN / 2;
+        const bool mine = tc >= 0 && tc < kCols;
         if (__any_sync(0xffffffffu, mine)) {
           float x = 0.f;
 #pragma unroll
@@ -611,13 +624,11 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           unpack(add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])), sa, sb);
           s_run += sa + sb;
         }
-        if (t.last) p.part[(int64_t)(2 * t.ks + half) * p.Np + row] = make_float2(m_run, s_run);
+        if (t.last) p.part[(int64_t)(2 * t.ks + wg) * p.Np + row] = make_float2(m_run, s_run);
         continue;
       }
 
       if (t.kind == kGrad) {
-        const int64_t row = t.arow + row_in;
-        const RowGrad rg = p.rg[row];
         const int v0 = (int)t.brow + col0;
         const int vend = p.cur.v0 + p.cur.nv;
         const float ga = rg.a * scales.g, gb = rg.b * scales.g;
@@ -640,7 +651,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
             }
         }
         const int tc = rg.target - v0;
-        if (__any_sync(0xffffffffu, tc >= 0 && tc < BN / 2)) {
+        if (__any_sync(0xffffffffu, tc >= 0 && tc < kCols)) {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -649,7 +660,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         }
         // rows without a weight (padding) and entries behind the last: exactly zero
         const bool empty = rg.a == 0.f && rg.b == 0.f;
-        if (v0 + BN / 2 > vend || __any_sync(0xffffffffu, empty)) {
+        if (v0 + kCols > vend || __any_sync(0xffffffffu, empty)) {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -695,19 +706,17 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           }
         }
         if (p.dbias_part) {
-          // column sums of the unrounded g; the four quadrants' meet in the (now free)
-          // stages: [half][quadrant][BN / 2]
+          // column sums of the unrounded g; the four quadrants' meet in the warpgroup's
+          // (now free) stages
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
             reinterpret_cast<float*>(stage)[32 * c + lane] = column_sums(acc[c], lane);
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          const int e = (int)threadIdx.x - 128;
-          if (e < BN) {
-            const float* cs = reinterpret_cast<const float*>(out_stage + (e / (BN / 2)) * 16384) + e % (BN / 2);
-            const float s = (cs[0] + cs[1024]) + (cs[2048] + cs[3072]);
-            p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + e] = s;
-          }
-          asm volatile("bar.sync 1, 256;" ::: "memory");
+          wg_sync();
+          const int e = (int)threadIdx.x & 127;
+          const float* cs = reinterpret_cast<const float*>(out_stage + wg * 16384) + e;
+          const float s = (cs[0] + cs[1024]) + (cs[2048] + cs[3072]);
+          p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + col0 + e] = s;
+          wg_sync();
         }
         continue;
       }
