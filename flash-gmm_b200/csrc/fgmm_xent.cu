@@ -63,12 +63,13 @@ struct __align__(16) RowGrad {
 
 #include "fgmm_xent_mma.cuh"
 
-// First words of the workspace.
+// First words of the workspace.  Every word is written before it is read: err and
+// done by the tensor-core kernel's first launch, the others by rows_kernel.
 struct Header {
-  int err;        // a wait of the tensor-core kernel gave up
-  int amax[3];    // float bits of the largest finite |weight|, |x|, |w|
-  int done;       // blocks of the closing forward kernel that have finished
-  int live;       // rows that are not ignored
+  int err[kErrSlots];   // nonzero: a wait of that block of the tensor-core kernel gave up
+  int done;             // blocks of the closing forward kernel that have finished
+  int live;             // rows that are not ignored
+  int amax[3];          // float bits of the largest finite |weight|, |x|, |w|
 };
 
 constexpr int kRowsPerBlock = 4096;
@@ -81,7 +82,7 @@ struct XentWs {
   void *Xp, *Xp2, *Wp, *Wp2;      // packed operands (SPLIT: hi and lo words)
   float2* part;
   float* tlogit;
-  double* loss_part;
+  double* loss_part;               // [blocks][2] sum, count
   RowGrad* rg;
   void *G[2], *G2[2];
   float *dbias_part, *dx_slots, *dw_slots;
@@ -133,7 +134,7 @@ struct XentWs {
       }
       part = c.take<float2>((size_t)2 * splits * Np);
       tlogit = c.take<float>(Np);
-      loss_part = c.take<double>((N + 31) / 32);
+      loss_part = c.take<double>(2 * ((N + 31) / 32));
     } else {
       const int word = split ? 4 : 2;
       // column tiles of dX and dW: 128 wide where that pads D less
@@ -179,17 +180,18 @@ struct XentWs {
 // one launch does it without a second pass.  Ignored rows get loss = logZ = 0.
 // The last block pads the list to a multiple of kPairRows with -1.
 __global__ void __launch_bounds__(1024) rows_kernel(const XentArgs a, const XentWs w) {
+  pdl_trigger();
   __shared__ int wsum[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t base = (int64_t)blockIdx.x * kRowsPerBlock;
+  if (blockIdx.x == 0 && threadIdx.x < 3) w.hdr->amax[threadIdx.x] = 0;
   int before = 0;
 #pragma unroll 8
   for (int64_t i = threadIdx.x; i < base; i += 1024) before += a.targets[i] != a.ignore;
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) wsum[warp] = before;
   __syncthreads();
-  int at = 0;
-  for (int k = 0; k < 32; ++k) at += wsum[k];
+  int at = __reduce_add_sync(0xffffffffu, wsum[lane]);
   for (int r = 0; r < kRowsPerBlock && base + r < a.N; r += 1024) {
     const int64_t i = base + r + threadIdx.x;
     const int64_t t = i < a.N ? a.targets[i] : a.ignore;
@@ -198,11 +200,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(const XentArgs a, const Xent
     __syncthreads();
     if (lane == 0) wsum[warp] = __popc(m);
     __syncthreads();
-    int mine = at, all = 0;
-    for (int k = 0; k < 32; ++k) {
-      if (k < warp) mine += wsum[k];
-      all += wsum[k];
-    }
+    const int c = wsum[lane];
+    const int all = __reduce_add_sync(0xffffffffu, c);
+    int mine = at + __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);
     if (keep) {
       mine += __popc(m & ((1u << lane) - 1u));
       w.rows[mine] = (int)i;
@@ -223,20 +223,24 @@ __global__ void __launch_bounds__(1024) rows_kernel(const XentArgs a, const Xent
   }
 }
 
-// Largest finite magnitude of the listed rows (of every row without a list); a
-// warp takes four rows at a time, 16 bytes a lane where the layout allows (vec).
-__global__ void __launch_bounds__(256)
-amax_kernel(const float* __restrict__ A, int64_t s0, int64_t s1, int D, int64_t n,
-            const int* __restrict__ rows, const int* __restrict__ live, int vec,
-            int* __restrict__ amax) {
-  if (live) n = *live;
+// A share of a launch: its block number and how many blocks work on it.
+struct Share {
+  int block, blocks;
+};
+
+// Largest finite magnitude of the listed rows (of all n without a list); a warp
+// takes four rows at a time, 16 bytes a lane where the layout allows (vec).
+__device__ __forceinline__ void amax_rows(const Share sh, const float* __restrict__ A, int64_t s0,
+                                          int64_t s1, int D, int64_t n,
+                                          const int* __restrict__ rows, int vec,
+                                          int* __restrict__ amax) {
   const int lane = threadIdx.x & 31;
   float m = 0.f;
   auto see = [&](float x) {
     x = fabsf(x);
     if (x < INFINITY) m = fmaxf(m, x);
   };
-  for (int64_t i0 = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * 4; i0 < n; i0 += gridDim.x * 32ll) {
+  for (int64_t i0 = (sh.block * 8ll + (threadIdx.x >> 5)) * 4; i0 < n; i0 += sh.blocks * 32ll) {
     const float* row[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -262,67 +266,74 @@ amax_kernel(const float* __restrict__ A, int64_t s0, int64_t s1, int D, int64_t 
   if (lane == 0 && m > 0.f) atomicMax(amax, __float_as_int(m));
 }
 
+// fp32: the magnitudes that scale X (blocks before blocks_x) and W.
+__global__ void __launch_bounds__(256)
+amax_kernel(const XentArgs a, const XentWs w, int blocks_x, int vec_x, int vec_w) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x;
+  if (b < blocks_x)
+    amax_rows(Share{b, blocks_x}, static_cast<const float*>(a.X), a.sxn, a.sxd, a.D, w.hdr->live,
+              w.rows, vec_x, &w.hdr->amax[1]);
+  else
+    amax_rows(Share{b - blocks_x, (int)gridDim.x - blocks_x}, static_cast<const float*>(a.W), a.swv,
+              a.swd, a.D, a.V, nullptr, vec_w, &w.hdr->amax[2]);
+}
+
 // Dense copies of X's live rows (rows != null; zero rows up to a multiple of
 // kPairRows) or of W, D padded with zeros to Dp; fp32 becomes two fp16 words of
 // the value / 2^e.  8 elements a thread, `lanes` threads (a power of two) a row.
 template <class T>
-__global__ void __launch_bounds__(256)
-pack_kernel(const T* __restrict__ A, int64_t s0, int64_t s1, int D, int Dp, int64_t n,
-            const int* __restrict__ rows, const int* __restrict__ live, int vec, int lanes,
-            const int* __restrict__ amax, uint16_t* __restrict__ out, uint16_t* __restrict__ out2) {
+__device__ __forceinline__ void pack_rows(const Share sh, const T* __restrict__ A, int64_t s0,
+                                          int64_t s1, int D, int Dp, int64_t n,
+                                          const int* __restrict__ rows, int vec, int lanes,
+                                          const int* __restrict__ amax, uint16_t* __restrict__ out,
+                                          uint16_t* __restrict__ out2) {
   constexpr bool kSplit = sizeof(T) == 4;
-  if (live) n = ((int64_t)*live + kPairRows - 1) / kPairRows * kPairRows;
   const int per_row = Dp / 8, per_block = 256 / lanes;
   const float scale = kSplit ? ldexpf(1.f, -Scales::exponent(*amax, 14)) : 1.f;
-  for (int64_t i = blockIdx.x * (int64_t)per_block + threadIdx.x / lanes; i < n;
-       i += gridDim.x * (int64_t)per_block) {
+  for (int64_t i = sh.block * (int64_t)per_block + threadIdx.x / lanes; i < n;
+       i += sh.blocks * (int64_t)per_block) {
     const int64_t r = rows ? rows[i] : i;
     for (int c = threadIdx.x % lanes; c < per_row; c += lanes) {
-    const int64_t e = i * per_row + c;
-    const int d0 = c * 8;
-    uint4 w = make_uint4(0u, 0u, 0u, 0u), w2 = w;
-    if (r >= 0) {
-      const T* src = A + r * s0 + (int64_t)d0 * s1;
-      if (!kSplit && vec && d0 + 8 <= D) {
-        w = *reinterpret_cast<const uint4*>(src);
-      } else {
-        T v[8];
-        if (kSplit && vec && d0 + 8 <= D) {
-          reinterpret_cast<uint4*>(v)[0] = reinterpret_cast<const uint4*>(src)[0];
-          reinterpret_cast<uint4*>(v)[kSplit ? 1 : 0] = reinterpret_cast<const uint4*>(src)[kSplit ? 1 : 0];
+      const int64_t e = i * per_row + c;
+      const int d0 = c * 8;
+      uint4 w = make_uint4(0u, 0u, 0u, 0u), w2 = w;
+      if (r >= 0) {
+        const T* src = A + r * s0 + (int64_t)d0 * s1;
+        if (!kSplit && vec && d0 + 8 <= D) {
+          w = *reinterpret_cast<const uint4*>(src);
         } else {
+          T v[8];
+          if (kSplit && vec && d0 + 8 <= D) {
+            reinterpret_cast<uint4*>(v)[0] = reinterpret_cast<const uint4*>(src)[0];
+            reinterpret_cast<uint4*>(v)[kSplit ? 1 : 0] = reinterpret_cast<const uint4*>(src)[kSplit ? 1 : 0];
+          } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = d0 + k < D ? src[k * s1] : from_f32<T>(0.f);
-        }
-        uint32_t h[4], l[4];
+            for (int k = 0; k < 8; ++k) v[k] = d0 + k < D ? src[k * s1] : from_f32<T>(0.f);
+          }
+          uint32_t h[4], l[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (kSplit) split2(to_f32(v[2 * k]) * scale, to_f32(v[2 * k + 1]) * scale, h[k], l[k]);
-          else h[k] = pack2<T>(to_f32(v[2 * k]), to_f32(v[2 * k + 1]));
+          for (int k = 0; k < 4; ++k) {
+            if (kSplit) split2(to_f32(v[2 * k]) * scale, to_f32(v[2 * k + 1]) * scale, h[k], l[k]);
+            else h[k] = pack2<T>(to_f32(v[2 * k]), to_f32(v[2 * k + 1]));
+          }
+          w = make_uint4(h[0], h[1], h[2], h[3]);
+          if (kSplit) w2 = make_uint4(l[0], l[1], l[2], l[3]);
         }
-        w = make_uint4(h[0], h[1], h[2], h[3]);
-        if (kSplit) w2 = make_uint4(l[0], l[1], l[2], l[3]);
       }
-    }
-    reinterpret_cast<uint4*>(out)[e] = w;
-    if (kSplit) reinterpret_cast<uint4*>(out2)[e] = w2;
+      reinterpret_cast<uint4*>(out)[e] = w;
+      if (kSplit) reinterpret_cast<uint4*>(out2)[e] = w2;
     }
   }
 }
 
-__global__ void pad_bias_kernel(const float* __restrict__ bias, int V, int64_t Vp,
-                                float* __restrict__ out) {
-  for (int64_t v = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; v < Vp;
-       v += (int64_t)gridDim.x * blockDim.x)
-    out[v] = v < V ? bias[v] : -INFINITY;
-}
-
-__global__ void row_grad_kernel(const XentArgs a, const XentWs w) {
+// What the backward pass knows of the (padded) live rows, and the largest weight.
+__device__ __forceinline__ void row_weights(const Share sh, const XentArgs& a, const XentWs& w) {
   const int64_t n = ((int64_t)w.hdr->live + kPairRows - 1) / kPairRows * kPairRows;
   const float inv = a.count_in ? 1.f / *a.count_in : 1.f;
   float top = 0.f;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n;
-       i += (int64_t)gridDim.x * blockDim.x) {
+  for (int64_t i = sh.block * 256ll + threadIdx.x; i < n; i += sh.blocks * 256ll) {
     RowGrad r{0.f, 0.f, 0.f, -1};
     const int n0 = w.rows[i];
     if (n0 >= 0) {
@@ -341,20 +352,69 @@ __global__ void row_grad_kernel(const XentArgs a, const XentWs w) {
   if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&w.hdr->amax[0], __float_as_int(top));
 }
 
+// Blocks of prepare_kernel by what they do, in this order.
+struct PrepareShares {
+  int x, w, bias, rows;
+  int vec_x, vec_w, lanes;
+};
+
+// Everything the products need, in one launch: the packed rows of X, W where it
+// cannot be read in place, the bias padded with -inf, and the rows' weights.
+template <class T>
+__global__ void __launch_bounds__(256)
+prepare_kernel(const XentArgs a, const XentWs w, const PrepareShares sh) {
+  pdl_trigger();
+  pdl_wait();
+  int b = blockIdx.x;
+  if (b < sh.x) {
+    const int64_t n = ((int64_t)w.hdr->live + kPairRows - 1) / kPairRows * kPairRows;
+    pack_rows<T>(Share{b, sh.x}, static_cast<const T*>(a.X), a.sxn, a.sxd, a.D, w.Dp, n, w.rows,
+                 sh.vec_x, sh.lanes, &w.hdr->amax[1], static_cast<uint16_t*>(w.Xp),
+                 static_cast<uint16_t*>(w.Xp2));
+    return;
+  }
+  b -= sh.x;
+  if (b < sh.w) {
+    pack_rows<T>(Share{b, sh.w}, static_cast<const T*>(a.W), a.swv, a.swd, a.D, w.Dp, a.V, nullptr,
+                 sh.vec_w, sh.lanes, &w.hdr->amax[2], static_cast<uint16_t*>(w.Wp),
+                 static_cast<uint16_t*>(w.Wp2));
+    return;
+  }
+  b -= sh.w;
+  if (b < sh.bias) {
+    for (int64_t v = b * 256ll + threadIdx.x; v < w.Vp; v += sh.bias * 256ll)
+      w.bias[v] = v < a.V ? a.bias[v] : -INFINITY;
+    return;
+  }
+  row_weights(Share{b - sh.bias, sh.rows}, a, w);
+}
+
+// Whether a wait of the tensor-core kernel gave up (the same for all threads).
+__device__ __forceinline__ bool any_error(const Header* hdr) {
+  int e = 0;
+  for (int i = threadIdx.x; i < kErrSlots; i += blockDim.x) e |= hdr->err[i];
+  return __syncthreads_or(e) != 0;
+}
+
 // Joins a live row's parts (max, sum) into logZ and loss.  A block takes 32
-// rows (lane = row), its 8 warps the parts in turn; the last block to finish
-// adds the blocks' loss sums in order.
-__global__ void __launch_bounds__(256) finish_forward_kernel(const XentArgs a, const XentWs w) {
-  __shared__ float sm[8][32], ss[8][32];
+// rows (lane = row), its 32 warps the parts in turn; the last block to finish
+// adds the blocks' sums in order.  `direct`: row i of X is live row i, ignored
+// rows among them.
+__global__ void __launch_bounds__(1024)
+finish_forward_kernel(const XentArgs a, const XentWs w, int direct) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float sm[32][33], ss[32][33];
   __shared__ int last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t i = blockIdx.x * 32ll + lane;
-  const int live = w.hdr->live;
+  const int64_t live = direct ? a.N : w.hdr->live;
+  const bool bad = any_error(w.hdr);
   const bool on = i < live;
   float m = -3.402823466e38f, s = 0.f;
   if (on)
-#pragma unroll 8
-    for (int k = warp; k < 2 * w.splits; k += 8) {
+#pragma unroll 4
+    for (int k = warp; k < 2 * w.splits; k += 32) {
       const float2 p = __ldg(&w.part[(int64_t)k * w.Np + i]);
       const float mn = fmaxf(m, p.x);
       s = s * ex2((m - mn) * kLog2Ef) + p.y * ex2((p.x - mn) * kLog2Ef);
@@ -365,92 +425,100 @@ __global__ void __launch_bounds__(256) finish_forward_kernel(const XentArgs a, c
   __syncthreads();
   if (warp == 0) {
     float top = sm[0][lane];
-    for (int k = 1; k < 8; ++k) top = fmaxf(top, sm[k][lane]);
+#pragma unroll
+    for (int k = 1; k < 32; ++k) top = fmaxf(top, sm[k][lane]);
     float sum = 0.f;
-    for (int k = 0; k < 8; ++k) sum += ss[k][lane] * ex2((sm[k][lane] - top) * kLog2Ef);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) sum += ss[k][lane] * ex2((sm[k][lane] - top) * kLog2Ef);
     double mine = 0.0;
+    bool counted = false;
     if (on) {
-      const int r = w.rows[i];
-      float lz = top + logf(sum);
-      const float nan = __int_as_float(0x7fffffff);
-      if (w.hdr->err) lz = nan;
-      const float loss = w.target[i] < 0 ? nan : lz - w.tlogit[i];
+      const int64_t r = direct ? i : w.rows[i], t = a.targets[r];
+      counted = t != a.ignore;
+      float lz = 0.f, loss = 0.f;
+      if (counted) {
+        const float nan = __int_as_float(0x7fffffff);
+        lz = bad ? nan : top + logf(sum);
+        loss = t < 0 || t >= a.V ? nan : lz - w.tlogit[i];
+        mine = loss;
+      }
       a.logZ[r] = lz;
       a.loss[r] = loss;
-      mine = loss;
     }
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0 && a.reduction != FGMM_REDUCE_NONE) {
-      w.loss_part[blockIdx.x] = mine;
-      __threadfence();
-      last = atomicAdd(&w.hdr->done, 1) == (int)gridDim.x - 1;
+    if (a.reduction != FGMM_REDUCE_NONE) {
+      for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      const int n = __popc(__ballot_sync(0xffffffffu, counted));
+      if (lane == 0) {
+        w.loss_part[2 * blockIdx.x] = mine;
+        w.loss_part[2 * blockIdx.x + 1] = n;
+        __threadfence();
+        last = atomicAdd(&w.hdr->done, 1) == (int)gridDim.x - 1;
+      }
     }
   }
   if (a.reduction == FGMM_REDUCE_NONE) return;
   __syncthreads();
-  if (!last) return;
+  if (!last || warp != 0) return;
   __threadfence();
-  __shared__ double red[256];
-  double s64 = 0.0;
-  for (int k = threadIdx.x; k < (int)gridDim.x; k += 256) s64 += __ldcg(&w.loss_part[k]);
-  red[threadIdx.x] = s64;
-  __syncthreads();
-  for (int o = 128; o; o >>= 1) {
-    if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-    __syncthreads();
+  double total = 0.0, n = 0.0;
+  for (int k = lane; k < (int)gridDim.x; k += 32) {
+    total += __ldcg(&w.loss_part[2 * k]);
+    n += __ldcg(&w.loss_part[2 * k + 1]);
   }
-  if (threadIdx.x == 0) {
-    *a.count = (float)live;
-    *a.reduced = (float)(a.reduction == FGMM_REDUCE_MEAN ? red[0] / live : red[0]);
+  for (int o = 16; o; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if (lane == 0) {
+    *a.count = (float)n;
+    *a.reduced = (float)(a.reduction == FGMM_REDUCE_MEAN ? total / n : total);
   }
 }
 
 // out[r, :] = scale * sum of the slots' rows, in slot order; rows of dX without
-// a live row are zero.  If a wait gave up, every gradient becomes NaN instead.
+// a live row (inv < 0) are zero.
 template <class T>
-__global__ void __launch_bounds__(256)
-store_slots_kernel(const float* __restrict__ slots, int ks, int64_t slot_rows, int64_t ldS, int D,
-                   int64_t n, const int* __restrict__ inv, const Header* __restrict__ hdr,
-                   int is_dw, int split, T* __restrict__ out) {
-  const int per_row = (D + 3) / 4;
-  const Scales sc(hdr->amax, !std::is_same<T, __nv_bfloat16>::value, split);
-  const float scale = is_dw ? sc.dw : sc.dx;
+__device__ __forceinline__ void store_slots(const Share sh, const float* __restrict__ slots, int ks,
+                                            int64_t slot_rows, int64_t ldS, int D, int64_t n,
+                                            const int* __restrict__ inv, float scale, int lanes,
+                                            T* __restrict__ out) {
+  const int per_row = (D + 3) / 4, per_block = (int)blockDim.x / lanes;
   const bool vec = D % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0;
-  const bool bad = hdr->err != 0;
-  const int64_t total = n * per_row;
-  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
-    const int64_t r = e / per_row;
-    const int d0 = (int)(e - r * per_row) * 4;
+  for (int64_t r = sh.block * (int64_t)per_block + threadIdx.x / lanes; r < n;
+       r += sh.blocks * (int64_t)per_block) {
     const int64_t i = inv ? inv[r] : r;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (i >= 0) {
-      for (int k = 0; k < ks; ++k) {
-        const float4 x = *reinterpret_cast<const float4*>(slots + (k * slot_rows + i) * ldS + d0);
-        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    for (int c = threadIdx.x % lanes; c < per_row; c += lanes) {
+      const int d0 = c * 4;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i >= 0) {
+#pragma unroll 4
+        for (int k = 0; k < ks; ++k) {
+          const float4 x = *reinterpret_cast<const float4*>(slots + (k * slot_rows + i) * ldS + d0);
+          s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        }
+        s.x *= scale; s.y *= scale; s.z *= scale; s.w *= scale;
       }
-      s.x *= scale; s.y *= scale; s.z *= scale; s.w *= scale;
-    }
-    if (bad) s.x = s.y = s.z = s.w = __int_as_float(0x7fffffff);
-    T* dst = out + r * D + d0;
-    if (vec) {
-      T v[4] = {from_f32<T>(s.x), from_f32<T>(s.y), from_f32<T>(s.z), from_f32<T>(s.w)};
-      if (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
-      else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
-    } else {
-      const float f[4] = {s.x, s.y, s.z, s.w};
-      for (int k = 0; k < 4; ++k)
-        if (d0 + k < D) dst[k] = from_f32<T>(f[k]);
+      T* dst = out + r * D + d0;
+      if (vec) {
+        T v[4] = {from_f32<T>(s.x), from_f32<T>(s.y), from_f32<T>(s.z), from_f32<T>(s.w)};
+        if (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
+        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
+      } else {
+        const float f[4] = {s.x, s.y, s.z, s.w};
+        for (int k = 0; k < 4; ++k)
+          if (d0 + k < D) dst[k] = from_f32<T>(f[k]);
+      }
     }
   }
 }
 
-// dbias from the 128-row partial sums (NaN if a wait gave up): 32 entries a block,
-// 32 warps that take the parts in turn, joined in warp order.
-__global__ void __launch_bounds__(1024) store_dbias_kernel(const XentArgs a, const XentWs w) {
+// dbias from the 128-row partial sums: 32 entries a block, whose 32 warps take
+// the parts in turn and are joined in order.
+__device__ __forceinline__ void store_dbias(int block, const XentArgs& a, const XentWs& w) {
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nparts = (int)(((int64_t)w.hdr->live + kPairRows - 1) / kPairRows) * 2;
-  const int64_t v = blockIdx.x * 32ll + lane;      // < Vp
+  const int64_t v = block * 32ll + lane;      // < Vp
   float s = 0.f;
 #pragma unroll 4
   for (int k = warp; k < nparts; k += 32) s += w.dbias_part[(int64_t)k * w.Vp + v];
@@ -458,23 +526,82 @@ __global__ void __launch_bounds__(1024) store_dbias_kernel(const XentArgs a, con
   __syncthreads();
   if (warp == 0 && v < a.V) {
     s = red[0][lane];
+#pragma unroll
     for (int k = 1; k < 32; ++k) s += red[k][lane];
-    const float back = 1.f / Scales(w.hdr->amax, a.type != FGMM_T_BF16, a.type == FGMM_T_F32).g;
-    a.dbias[v] = w.hdr->err ? __int_as_float(0x7fffffff) : s * back;
+    a.dbias[v] = s / Scales(w.hdr->amax, a.type != FGMM_T_BF16, a.type == FGMM_T_F32).g;
   }
 }
 
-// After the last product: dW that was written directly becomes NaN if a wait gave up.
 template <class T>
-__global__ void poison_kernel(const Header* __restrict__ hdr, T* __restrict__ out, int64_t n) {
-  if (hdr->err == 0) return;
+__device__ __forceinline__ void fill_nan(T* out, int64_t n) {
   for (int64_t e = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; e < n;
        e += (int64_t)gridDim.x * blockDim.x)
     out[e] = from_f32<T>(__int_as_float(0x7fffffff));
 }
 
-int grid_for(int64_t threads) {
-  return (int)std::min<int64_t>(std::max<int64_t>((threads + 255) / 256, 1), 16 * num_sms());
+// Blocks of finish_backward_kernel by what they do, in this order.
+struct FinishShares {
+  int dx, dw, dbias;
+  int v0, nv;      // dW's rows from the slots
+  int lanes;
+};
+
+// Gradients from their fp32 sums.  If a wait gave up, the last launch makes all
+// of them NaN instead.
+template <class T>
+__global__ void __launch_bounds__(1024)
+finish_backward_kernel(const XentArgs a, const XentWs w, const FinishShares sh, int final_launch) {
+  pdl_trigger();
+  pdl_wait();
+  if (final_launch && any_error(w.hdr)) {
+    if (a.dX) fill_nan(static_cast<T*>(a.dX), a.N * a.D);
+    if (a.dW) fill_nan(static_cast<T*>(a.dW), (int64_t)a.V * a.D);
+    if (a.dbias) fill_nan(a.dbias, a.V);
+    return;
+  }
+  const Scales sc(w.hdr->amax, !std::is_same<T, __nv_bfloat16>::value, sizeof(T) == 4);
+  int b = blockIdx.x;
+  if (b < sh.dx) {
+    store_slots<T>(Share{b, sh.dx}, w.dx_slots, w.ks_x, w.Np, w.ldS, a.D, a.N, w.inv, sc.dx,
+                   sh.lanes, static_cast<T*>(a.dX));
+    return;
+  }
+  b -= sh.dx;
+  if (b < sh.dw) {
+    store_slots<T>(Share{b, sh.dw}, w.dw_slots, w.ks_w, w.piece, w.ldS, a.D, sh.nv, nullptr, sc.dw,
+                   sh.lanes, static_cast<T*>(a.dW) + (int64_t)sh.v0 * a.D);
+    return;
+  }
+  if (b - sh.dw < sh.dbias) store_dbias(b - sh.dw, a, w);
+}
+
+// Launches a kernel; `dependent`: it may be set up while the kernel before it (of this
+// call, on the same stream) still runs, and waits for its end itself (pdl_wait).
+template <class... P, class... A>
+cudaError_t launch(void (*kernel)(P...), int64_t grid, int threads, size_t smem,
+                   cudaStream_t stream, bool dependent, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+// Blocks of 256 threads for that many threads' work: all resident at once at most.
+int blocks_for(int64_t threads) {
+  return (int)std::min<int64_t>(std::max<int64_t>((threads + 255) / 256, 1), 8 * num_sms());
+}
+int row_lanes(int64_t pieces, int most) {
+  int lanes = 1;
+  while (lanes < most && lanes < pieces) lanes *= 2;
+  return lanes;
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -482,8 +609,15 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// The driver's encoder.  It needs the device's context current on the calling thread,
+// which a thread that has made no runtime call yet (autograd's, a new host thread) lacks
+// until cudaSetDevice binds it.
 cudaError_t encode_fn(EncodeTiled* out) {
   static std::atomic<void*> cached{nullptr};
+  int dev = 0;
+  cudaError_t bound = cudaGetDevice(&dev);
+  if (bound == cudaSuccess) bound = cudaSetDevice(dev);
+  if (bound != cudaSuccess) return bound;
   void* f = cached.load(std::memory_order_acquire);
   if (!f) {
     cudaDriverEntryPointQueryResult found;
@@ -499,11 +633,8 @@ cudaError_t encode_fn(EncodeTiled* out) {
 
 // 64 x 64 boxes of a row-major (rows, cols) matrix of 16-bit words, 128-byte
 // swizzle; elements outside read as zero.
-cudaError_t make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld,
-                     bool bf16) {
-  EncodeTiled encode;
-  cudaError_t e = encode_fn(&encode);
-  if (e != cudaSuccess) return e;
+cudaError_t make_map(EncodeTiled encode, CUtensorMap* m, const void* base, int64_t rows,
+                     int64_t cols, int64_t ld, bool bf16) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)std::max<int64_t>(rows, 1)};
   const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
   const cuuint32_t box[2] = {64, 64}, es[2] = {1, 1};
@@ -519,58 +650,64 @@ template <class T> struct Word { using type = T; };
 template <> struct Word<float> { using type = __half; };
 
 template <class T>
-cudaError_t prepare_operands(const XentArgs& a, const XentWs& w, MmaMaps* maps) {
+cudaError_t make_operand_maps(const XentArgs& a, const XentWs& w, bool direct, MmaMaps* maps) {
   constexpr bool kSplit = sizeof(T) == 4;
   constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value;
-  cudaError_t e = cudaMemsetAsync(w.hdr, 0, sizeof(Header), a.stream);
+  EncodeTiled enc;
+  cudaError_t e = encode_fn(&enc);
   if (e != cudaSuccess) return e;
-  rows_kernel<<<(unsigned)((a.N + kRowsPerBlock - 1) / kRowsPerBlock), 1024, 0, a.stream>>>(a, w);
-  const T* X = static_cast<const T*>(a.X);
-  const T* W = static_cast<const T*>(a.W);
-  const int* live = &w.hdr->live;
+  e = direct ? make_map(enc, &maps->X, a.X, a.N, a.D, a.sxn, kBf)
+                         : make_map(enc, &maps->X, w.Xp, w.Np, a.D, w.Dp, kBf);
+  if (e == cudaSuccess)
+    e = w.pack_w ? make_map(enc, &maps->W, w.Wp, a.V, a.D, w.Dp, kBf)
+                 : make_map(enc, &maps->W, a.W, a.V, a.D, a.swv, kBf);
+  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->X2, w.Xp2, w.Np, a.D, w.Dp, kBf);
+  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->W2, w.Wp2, a.V, a.D, w.Dp, kBf);
+  return e;
+}
+
+// The launches before the first product.  `direct`: X is read in place; *dependent
+// tells whether there was a launch.
+template <class T>
+cudaError_t prepare(const XentArgs& a, const XentWs& w, bool direct, bool backward, bool* dependent) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  *dependent = false;
+  cudaError_t e = cudaSuccess;
   auto vec = [&](const void* p, int64_t s0, int64_t s1, int whole) {
     return s1 == 1 && s0 * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 &&
            a.D % whole == 0;
   };
-  if (kSplit) {
-    auto blocks = [&](int64_t n) { return (int)std::min<int64_t>((n + 31) / 32, 8 * num_sms()); };
-    amax_kernel<<<blocks(a.N), 256, 0, a.stream>>>(
-        reinterpret_cast<const float*>(X), a.sxn, a.sxd, a.D, a.N, w.rows, live,
-        vec(X, a.sxn, a.sxd, 4), &w.hdr->amax[1]);
-    amax_kernel<<<blocks(a.V), 256, 0, a.stream>>>(
-        reinterpret_cast<const float*>(W), a.swv, a.swd, a.D, a.V, nullptr, nullptr,
-        vec(W, a.swv, a.swd, 4), &w.hdr->amax[2]);
-    count_launches(2);
+  if (!direct) {
+    e = launch(rows_kernel, (a.N + kRowsPerBlock - 1) / kRowsPerBlock, 1024, 0, a.stream, false, a, w);
+    *dependent = true;
   }
-  int lanes = 1;
-  while (lanes < 256 && lanes < w.Dp / 8) lanes *= 2;
-  pack_kernel<T><<<grid_for(w.Np * lanes), 256, 0, a.stream>>>(
-      X, a.sxn, a.sxd, a.D, w.Dp, 0, w.rows, live, vec(X, a.sxn, a.sxd, 1), lanes, &w.hdr->amax[1],
-      static_cast<uint16_t*>(w.Xp), static_cast<uint16_t*>(w.Xp2));
-  count_launches(2);
-  if (w.pack_w) {
-    pack_kernel<T><<<grid_for((int64_t)a.V * lanes), 256, 0, a.stream>>>(
-        W, a.swv, a.swd, a.D, w.Dp, a.V, nullptr, nullptr, vec(W, a.swv, a.swd, 1), lanes,
-        &w.hdr->amax[2], static_cast<uint16_t*>(w.Wp), static_cast<uint16_t*>(w.Wp2));
-    count_launches(1);
+  if constexpr (kSplit) {
+    const int bx = blocks_for(a.N * 8), bw = blocks_for((int64_t)a.V * 8);
+    if (e == cudaSuccess)
+      e = launch(amax_kernel, bx + bw, 256, 0, a.stream, true, a, w, bx, vec(a.X, a.sxn, a.sxd, 4),
+                 vec(a.W, a.swv, a.swd, 4));
   }
-  if (a.bias) {
-    pad_bias_kernel<<<grid_for(w.Vp), 256, 0, a.stream>>>(a.bias, a.V, w.Vp, w.bias);
-    count_launches(1);
+  PrepareShares sh{};
+  sh.lanes = row_lanes(w.Dp / 8, 256);
+  sh.x = direct ? 0 : blocks_for(w.Np * sh.lanes);
+  sh.w = w.pack_w ? blocks_for((int64_t)a.V * sh.lanes) : 0;
+  sh.bias = a.bias ? blocks_for(w.Vp) : 0;
+  sh.rows = backward ? blocks_for(w.Np) : 0;
+  sh.vec_x = vec(a.X, a.sxn, a.sxd, 1);
+  sh.vec_w = vec(a.W, a.swv, a.swd, 1);
+  const int grid = sh.x + sh.w + sh.bias + sh.rows;
+  if (e == cudaSuccess && grid > 0) {
+    e = launch(prepare_kernel<T>, grid, 256, 0, a.stream, *dependent, a, w, sh);
+    *dependent = true;
   }
-  e = make_map(&maps->X, w.Xp, w.Np, a.D, w.Dp, kBf);
-  if (e == cudaSuccess)
-    e = w.pack_w ? make_map(&maps->W, w.Wp, a.V, a.D, w.Dp, kBf)
-                 : make_map(&maps->W, a.W, a.V, a.D, a.swv, kBf);
-  if (kSplit && e == cudaSuccess) e = make_map(&maps->X2, w.Xp2, w.Np, a.D, w.Dp, kBf);
-  if (kSplit && e == cudaSuccess) e = make_map(&maps->W2, w.Wp2, a.V, a.D, w.Dp, kBf);
   return e;
 }
 
 MmaParams common_params(const XentArgs& a, const XentWs& w) {
   MmaParams p{};
   p.live = &w.hdr->live;
-  p.err = &w.hdr->err;
+  p.err = w.hdr->err;
+  p.done = &w.hdr->done;
   p.amax = w.hdr->amax;
   p.N = a.N;
   p.D = a.D;
@@ -583,22 +720,28 @@ MmaParams common_params(const XentArgs& a, const XentWs& w) {
 }
 
 template <bool FWD, class T>
-cudaError_t launch_mma(const XentArgs& a, const MmaParams& p, const MmaMaps& maps, int64_t units) {
+cudaError_t launch_mma(const XentArgs& a, const MmaParams& p, const MmaMaps& maps, int64_t units,
+                       bool dependent) {
   constexpr bool kSplit = sizeof(T) == 4;
   auto* kernel = xent_mma_kernel<FWD, kSplit, typename Word<T>::type, T>;
   constexpr size_t smem = MmaCfg<kSplit>::kSmem;
   cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  const int pairs = (int)std::min<int64_t>(units, num_sms() / 2);
-  kernel<<<2 * pairs, kMmaThreads, smem, a.stream>>>(p, maps);
-  count_launches(1);
-  return cudaGetLastError();
+  const int64_t pairs = std::min<int64_t>(units, std::min(num_sms(), kErrSlots) / 2);
+  return launch(kernel, 2 * pairs, kMmaThreads, smem, a.stream, dependent, p, maps);
 }
 
 template <class T>
 cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
   MmaMaps maps{};
-  cudaError_t e = prepare_operands<T>(a, w, &maps);
+  // Up to one tile of rows that TMA can read is used in place: no list, no copy, and
+  // the ignored rows among them cost nothing.
+  const bool direct = sizeof(T) == 2 && a.N <= kPairRows && a.sxd == 1 && a.sxn >= a.D &&
+                      a.sxn % 8 == 0 && a.sxn < (int64_t(1) << 38) &&
+                      (reinterpret_cast<uintptr_t>(a.X) & 15) == 0;
+  cudaError_t e = make_operand_maps<T>(a, w, direct, &maps);
+  bool dependent;
+  if (e == cudaSuccess) e = prepare<T>(a, w, direct, false, &dependent);
   if (e != cudaSuccess) return e;
   MmaParams p = common_params(a, w);
   p.vtiles = w.vtiles;
@@ -606,26 +749,27 @@ cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
   p.splits = w.splits;
   p.part = w.part;
   p.tlogit = w.tlogit;
-  p.target = w.target;
-  e = launch_mma<true, T>(a, p, maps, w.Np / kPairRows * w.splits);
+  p.target = direct ? nullptr : w.target;
+  p.targets = a.targets;
+  p.first = 1;
+  e = launch_mma<true, T>(a, p, maps, w.Np / kPairRows * w.splits, dependent);
   if (e != cudaSuccess) return e;
-  finish_forward_kernel<<<(unsigned)((a.N + 31) / 32), 256, 0, a.stream>>>(a, w);
-  count_launches(1);
-  return cudaSuccess;
+  return launch(finish_forward_kernel, (a.N + 31) / 32, 1024, 0, a.stream, true, a, w, (int)direct);
 }
 
 template <class T>
 cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
   constexpr bool kSplit = sizeof(T) == 4;
   MmaMaps maps{};
-  cudaError_t e = prepare_operands<T>(a, w, &maps);
-  if (e != cudaSuccess) return e;
-  row_grad_kernel<<<grid_for(w.Np), 256, 0, a.stream>>>(a, w);
-  count_launches(1);
+  cudaError_t e = make_operand_maps<T>(a, w, false, &maps);
+  bool dependent;
+  if (e == cudaSuccess) e = prepare<T>(a, w, false, true, &dependent);
   CUtensorMap gmap[2], gmap2[2];
+  EncodeTiled enc;
+  if (e == cudaSuccess) e = encode_fn(&enc);
   for (int b = 0; b < 2 && e == cudaSuccess; ++b) {
-    e = make_map(&gmap[b], w.G[b], w.row_chunk, w.piece, w.piece, std::is_same<T, __nv_bfloat16>::value);
-    if (kSplit && e == cudaSuccess) e = make_map(&gmap2[b], w.G2[b], w.row_chunk, w.piece, w.piece, false);
+    e = make_map(enc, &gmap[b], w.G[b], w.row_chunk, w.piece, w.piece, std::is_same<T, __nv_bfloat16>::value);
+    if (kSplit && e == cudaSuccess) e = make_map(enc, &gmap2[b], w.G2[b], w.row_chunk, w.piece, w.piece, false);
   }
   if (e != cudaSuccess) return e;
   MmaParams p = common_params(a, w);
@@ -658,7 +802,11 @@ cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
     p.has_grad = j < total;
     p.has_dx = j > 0 && a.dX != nullptr;
     p.has_dw = j > 0 && a.dW != nullptr;
-    if (!p.has_grad && !p.has_dx && !p.has_dw) break;
+    if (!p.has_grad && !p.has_dx && !p.has_dw) {   // dbias alone: its sums are complete
+      FinishShares sh{};
+      sh.dbias = (a.V + 31) / 32;
+      return launch(finish_backward_kernel<T>, sh.dbias, 1024, 0, a.stream, true, a, w, sh, 1);
+    }
     p.cur = piece_at(std::min(j, total - 1));
     p.prev = piece_at(std::max(j - 1, 0));
     p.dx_add = j - 1 >= w.n_chunks;
@@ -671,27 +819,29 @@ cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
         (p.has_grad ? (int64_t)(p.cur.rows / 256) * ((p.cur.nv + kBN - 1) / kBN) : 0) +
         (p.has_dx ? (int64_t)(p.prev.rows / 256) * w.tiles_d * w.ks_x : 0) +
         (p.has_dw ? (int64_t)((p.prev.nv + 255) / 256) * w.tiles_d * w.ks_w : 0);
-    e = launch_mma<false, T>(a, p, maps, units);
+    p.first = j == 0;
+    e = launch_mma<false, T>(a, p, maps, units, true);
     if (e != cudaSuccess) return e;
-    if (p.has_dw && !w.dw_direct && j % w.n_chunks == 0) {   // the piece's last row chunk
-      store_slots_kernel<T><<<grid_for((int64_t)p.prev.nv * ((a.D + 3) / 4)), 256, 0, a.stream>>>(
-          w.dw_slots, w.ks_w, w.piece, w.ldS, a.D, p.prev.nv, nullptr, w.hdr, 1, kSplit,
-          static_cast<T*>(a.dW) + (int64_t)p.prev.v0 * a.D);
-      count_launches(1);
+    // dW's slots are complete after the piece's last row chunk; with the last piece, all
+    // sums are
+    const bool last = j == total;
+    const bool dw = p.has_dw && !w.dw_direct && j % w.n_chunks == 0;
+    if (dw || last) {
+      FinishShares sh{};
+      const int pieces = (a.D + 3) / 4;
+      sh.lanes = row_lanes(pieces, 1024);
+      auto blocks = [&](int64_t rows) {
+        return (int)std::min<int64_t>((rows * sh.lanes + 1023) / 1024, 2 * num_sms());
+      };
+      sh.dx = last && a.dX ? blocks(a.N) : 0;
+      sh.dw = dw ? blocks(p.prev.nv) : 0;
+      sh.dbias = last && a.dbias ? (a.V + 31) / 32 : 0;
+      sh.v0 = p.prev.v0;
+      sh.nv = p.prev.nv;
+      e = launch(finish_backward_kernel<T>, std::max(sh.dx + sh.dw + sh.dbias, 1), 1024, 0, a.stream,
+                 true, a, w, sh, (int)last);
+      if (e != cudaSuccess) return e;
     }
-  }
-  if (a.dX) {
-    store_slots_kernel<T><<<grid_for(a.N * ((a.D + 3) / 4)), 256, 0, a.stream>>>(
-        w.dx_slots, w.ks_x, w.Np, w.ldS, a.D, a.N, w.inv, w.hdr, 0, kSplit, static_cast<T*>(a.dX));
-    count_launches(1);
-  }
-  if (a.dbias) {
-    store_dbias_kernel<<<(unsigned)((a.V + 31) / 32), 1024, 0, a.stream>>>(a, w);
-    count_launches(1);
-  }
-  if (a.dW) {
-    poison_kernel<T><<<num_sms(), 256, 0, a.stream>>>(w.hdr, static_cast<T*>(a.dW), (int64_t)a.V * a.D);
-    count_launches(1);
   }
   return cudaSuccess;
 }
@@ -812,6 +962,7 @@ int fgmm_xent_bwd(int type, const void* X, int64_t x_stride_n, int64_t x_stride_
     rc = check_device_and_workspace(a, w.bytes);
     if (rc != FGMM_OK) return rc;
     cudaError_t e = cudaSuccess;
+    if (!dX && !dW && !dbias) return FGMM_OK;
     if (N == 0) {
       if (dW) e = cudaMemsetAsync(dW, 0, (size_t)V * D * type_size(type), a.stream);
       if (e == cudaSuccess && dbias) e = cudaMemsetAsync(dbias, 0, (size_t)V * 4, a.stream);

@@ -37,6 +37,7 @@
 // bound by its dependent latencies, not by the special-function unit (50% busy).
 
 constexpr int kPairRows = 256;
+constexpr int kErrSlots = 256;    // blocks of this kernel, at most
 constexpr int kBoxBytes = 64 * 128;
 constexpr int kEpiWarps = 8;
 constexpr int kMmaThreads = (4 + kEpiWarps) * 32;
@@ -53,8 +54,9 @@ struct Piece {
 };
 
 struct MmaParams {
-  const int* live;
-  int* err;
+  const int* live;         // unused where target is null
+  int *err, *done;         // Header
+  int first;               // first launch of the call: err and done start at 0
   int64_t N;
   int D, V, kbD;           // kbD = ceil(D / 64)
   int bn_d, tiles_d;       // column tiles of dX and dW: width 128 or 256, count
@@ -62,7 +64,8 @@ struct MmaParams {
   int vtiles, per_split, splits;
   float2* part;            // [2 splits][Np] (max, sum of exp(S - max)), natural units
   float* tlogit;           // [Np] S at the target
-  const int* target;       // [Np] compact targets (-1: none)
+  const int* target;       // [Np] the live rows' targets (-1: none); null: X is read in place,
+  const int64_t* targets;  // row i's target is targets[i]
   int64_t Np;
   const float* bias;       // padded to 256 with -inf, or null
   const int* amax;         // float bits of the largest |g weight|, |x|, |w| (Scales)
@@ -101,6 +104,7 @@ struct Scales {
     return max(-100, min(100, scale_exp_to(__int_as_float(bits), target)));
   }
   __device__ Scales(const int* amax, bool f16, bool split) {
+    if (!amax) { s = g = dx = dw = 1.f; return; }   // 16-bit logits: nothing is scaled
     const float top = __int_as_float(amax[0]);
     const float unit = f16 ? 4096.f : 1.f;
     // weights outside 2^-100 .. 2^100: their reciprocal would leave fp32
@@ -123,6 +127,15 @@ struct Tile {
   int m, n, ks;         // tile indices
   int last;             // kLse: last tile of the unit
 };
+
+// Programmatic dependent launch: let the next kernel of the stream be set up, and wait
+// for the end of the one before (no-ops in a launch without the attribute).
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
                                               uint32_t bar) {
@@ -211,7 +224,7 @@ struct TileWalk {
   int unit, step, sub = 0, um = 0, us = 0;
   int mt, mtx, n_dw, n_dx, n_grad, units;
   __device__ TileWalk(const MmaParams& p_, int pair, int npairs) : p(p_), unit(pair), step(npairs) {
-    live = *p.live;
+    live = FWD && !p.target ? p.N : *p.live;
     if (FWD) {
       mt = (int)((live + kPairRows - 1) / kPairRows);
       units = mt * p.splits;
@@ -385,8 +398,18 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
   cluster_sync_all();   // the other SM's barriers are ready before anything arrives there
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
+  // set up; now what the launches before this one write
+  pdl_trigger();
+  pdl_wait();
+  int* err = p.err + blockIdx.x;
+  if (p.first) {
+    if (threadIdx.x == 0)
+      for (int i = blockIdx.x; i < kErrSlots; i += gridDim.x) p.err[i] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
+    __syncthreads();
+  }
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-    return mbar_wait_flag(bar, parity, &ctl->abort_flag, p.err, code);
+    return mbar_wait_flag(bar, parity, &ctl->abort_flag, err, code);
   };
 
   if (warp < 4) {
@@ -491,7 +514,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     uint8_t* stage = out_stage + (warp - 4) * 4096;
     const uint32_t empty0 = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
     constexpr bool f16 = std::is_same<T, __half>::value;
-    const Scales scales(p.amax, f16, SPLIT);
+    const Scales scales(FWD && !SPLIT ? nullptr : p.amax, f16, SPLIT);
     const float sc_s = scales.s;
     float m_run = -3.402823466e38f, s_run = 0.f;            // kLse, over the unit's tiles
     int target = -1;
@@ -515,7 +538,12 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       if (FWD && t.n == t.ks * p.per_split) {               // first tile of the unit
         m_run = -3.402823466e38f;
         s_run = 0.f;
-        target = p.target[row];
+        if (p.target) {
+          target = p.target[row];
+        } else {
+          const int64_t x = row < p.N ? p.targets[row] : -1;
+          target = x >= 0 && x < p.V ? (int)x : -1;
+        }
       }
       RowGrad rg;
       if (!FWD && t.kind == kGrad) rg = p.rg[row];          // in flight while the MMAs run

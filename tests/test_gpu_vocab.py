@@ -276,6 +276,33 @@ def test_xent_other_stream_and_two_at_once():
         assert torch.equal(a, want) and torch.equal(b, want2)
 
 
+def test_xent_from_new_host_threads():
+    """The backward call as the first CUDA call of its host thread (as autograd's worker
+    makes it), and two threads on one stream at once."""
+    import threading
+    X, W, t, _ = R.problem(300, 500, 64, BF)
+    loss, logZ, reduced, count = L.xent_fwd(X, W, t, None, R.IGNORE, "mean")
+    one = torch.ones((), device=DEV)
+    want = L.xent_bwd(X, W, t, None, R.IGNORE, logZ, one, count, None, (True, True, False))
+    got, failed = {}, []
+
+    def work(k):
+        try:
+            for _ in range(10):
+                got[k] = L.xent_bwd(X, W, t, None, R.IGNORE, logZ, one, count, None,
+                                    (True, True, False))
+                assert torch.equal(L.xent_fwd(X, W, t, None, R.IGNORE, "none")[0], loss)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    [th.start() for th in threads]
+    [th.join() for th in threads]
+    assert not failed, failed
+    for g in got.values():
+        assert torch.equal(g[0], want[0]) and torch.equal(g[1], want[1])
+
+
 def test_training_step_captured_into_graphs():
     """Lookup, loss and both gradients, captured twice and replayed on new data."""
     X, W, t, _ = R.problem(300, 700, 64, BF, ignored=0.1)
