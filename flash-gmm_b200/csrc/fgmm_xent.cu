@@ -9,8 +9,8 @@
 // first ("live" rows, in their order): ignored rows cost no products, and what
 // they hold never meets a product.  Forward, logits stay in TMEM and registers and
 // leave as a (max, sum) per row and range of the vocabulary.  Backward, they are
-// computed again in pieces of the vocabulary; a piece's g goes to the workspace
-// and is multiplied with W and X while the next piece's is made.
+// computed again in pieces; a piece's g goes to a small ring of buffers and is
+// multiplied with W and X, out of the L2, while the next pieces' are made.
 #include <cuda.h>
 
 #include <algorithm>
@@ -84,7 +84,8 @@ struct XentWs {
   float* tlogit;
   double* loss_part;               // [blocks][2] sum, count
   RowGrad* rg;
-  void *G[2], *G2[2];
+  uint32_t* sync;
+  void *G, *G2;
   float *dbias_part, *dx_slots, *dw_slots;
 
   int64_t Np, Vp;
@@ -94,11 +95,11 @@ struct XentWs {
   int bn_d, tiles_d;
   int64_t ldS;
   int row_chunk, piece, n_chunks, n_pieces, ks_x, ks_w;
-  bool dw_direct;
+  int64_t sync_words;
   size_t bytes;
 
   static constexpr int kPairs = 74;                        // SM pairs the plan is made for
-  static constexpr int64_t kPieceBytes = int64_t(1) << 28; // one buffer of G
+  static constexpr int64_t kPieceBytes = int64_t(1) << 25; // one buffer of G: kRing stay in the L2
   static constexpr int64_t kSlotBytes = int64_t(1) << 28;
 
   XentWs(void* p, bool backward, int type, int64_t N, int V, int D, const void* W, int64_t swv,
@@ -141,35 +142,36 @@ struct XentWs {
       bn_d = (D + 127) / 128 * 128 < (D + 255) / 256 * 256 ? 128 : 256;
       tiles_d = (D + bn_d - 1) / bn_d;
       ldS = (int64_t)tiles_d * bn_d;
-      // G in pieces of at most kPieceBytes: all rows x at least 2048 entries if possible
-      const int64_t wide = std::min<int64_t>(Vp, 2048);
+      // Pieces of G: wide ones, so that dX's slots are added to rarely, and all rows of a
+      // short batch.
+      piece = (int)std::min<int64_t>(Vp, 4096);
       row_chunk = (int)std::max<int64_t>(
-          256, std::min<int64_t>(Np, kPieceBytes / (wide * word) / 256 * 256));
-      piece = (int)std::max<int64_t>(
-          256, std::min<int64_t>(Vp, kPieceBytes / ((int64_t)row_chunk * word) / 256 * 256));
+          256, std::min<int64_t>(Np, kPieceBytes / ((int64_t)piece * word) / 256 * 256));
+      if (row_chunk == Np)
+        piece = (int)std::max<int64_t>(
+            piece, std::min<int64_t>(Vp, kPieceBytes / ((int64_t)row_chunk * word) / 256 * 256));
       n_chunks = (int)((Np + row_chunk - 1) / row_chunk);
       n_pieces = (int)((Vp + piece - 1) / piece);
-      // Splits of K, where a product's tiles alone cannot occupy the pairs
-      const int64_t dx_tiles = (int64_t)(row_chunk / 256) * tiles_d, dx_kb = piece / 64;
-      const int64_t dw_tiles = (int64_t)(piece / 256) * tiles_d, dw_kb = row_chunk / 64;
-      auto pick = [](int64_t tiles, int64_t kb, int64_t slot_bytes) {
-        int64_t ks = 1;
-        if (tiles < 2 * kPairs) ks = (3 * kPairs + tiles - 1) / tiles;
+      // Splits of K: products of at most kUnit blocks, shorter where a product's tiles
+      // could not occupy the pairs twice; dW's only where its slots hold all of V.
+      const int64_t unit = split ? 24 : 64;
+      auto pick = [&](int64_t tiles, int64_t kb, int64_t slot_bytes) {
+        int64_t ks = std::max<int64_t>((kb + unit - 1) / unit, (2 * kPairs + tiles - 1) / tiles);
         ks = std::min(ks, std::max<int64_t>(1, kb / 8));
         return (int)std::max<int64_t>(1, std::min(ks, kSlotBytes / std::max<int64_t>(slot_bytes, 1)));
       };
-      ks_x = pick(dx_tiles, dx_kb, Np * ldS * 4);
-      ks_w = pick(dw_tiles, dw_kb, (int64_t)piece * ldS * 4);
-      dw_direct = n_chunks == 1 && ks_w == 1;
+      const int64_t steps = (int64_t)n_chunks * n_pieces;
+      ks_x = pick((int64_t)(row_chunk / 256) * tiles_d * steps, piece / 64, Np * ldS * 4);
+      ks_w = n_pieces > 1 ? 1 : pick((int64_t)(piece / 256) * tiles_d * steps, row_chunk / 64,
+                                     (int64_t)piece * ldS * 4);
       rg = c.take<RowGrad>(Np);
-      const bool two = n_chunks * n_pieces > 1;
-      for (int b = 0; b < 2; ++b) {
-        G[b] = c.take<uint16_t>(b == 0 || two ? (size_t)row_chunk * piece : 0);
-        G2[b] = c.take<uint16_t>(split && (b == 0 || two) ? (size_t)row_chunk * piece : 0);
-      }
+      sync_words = 1 + 2 * steps + (Np / kPairRows * ks_x + (int64_t)(piece / 256) * ks_w) * tiles_d;
+      sync = c.take<uint32_t>(sync_words);
+      G = c.take<uint16_t>((size_t)kRing * row_chunk * piece);
+      G2 = c.take<uint16_t>(split ? (size_t)kRing * row_chunk * piece : 0);
       dbias_part = c.take<float>(want_bias ? (size_t)(Np / 128) * Vp : 0);
       dx_slots = c.take<float>((size_t)ks_x * Np * ldS);
-      dw_slots = c.take<float>(dw_direct ? 0 : (size_t)ks_w * piece * ldS);
+      dw_slots = c.take<float>(n_chunks == 1 && ks_w == 1 ? 0 : (size_t)ks_w * piece * ldS);
     }
     bytes = c.used;
   }
@@ -185,6 +187,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(const XentArgs a, const Xent
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t base = (int64_t)blockIdx.x * kRowsPerBlock;
   if (blockIdx.x == 0 && threadIdx.x < 3) w.hdr->amax[threadIdx.x] = 0;
+  if (a.logZ_in)   // backward: the product kernel's counts
+    for (int64_t i = blockIdx.x * 1024 + threadIdx.x; i < w.sync_words; i += gridDim.x * 1024)
+      w.sync[i] = 0;
   int before = 0;
 #pragma unroll 8
   for (int64_t i = threadIdx.x; i < base; i += 1024) before += a.targets[i] != a.ignore;
@@ -542,18 +547,16 @@ __device__ __forceinline__ void fill_nan(T* out, int64_t n) {
 // Blocks of finish_backward_kernel by what they do, in this order.
 struct FinishShares {
   int dx, dw, dbias;
-  int v0, nv;      // dW's rows from the slots
   int lanes;
 };
 
-// Gradients from their fp32 sums.  If a wait gave up, the last launch makes all
-// of them NaN instead.
+// Gradients from their fp32 sums.  If a wait gave up, all of them become NaN instead.
 template <class T>
 __global__ void __launch_bounds__(1024)
-finish_backward_kernel(const XentArgs a, const XentWs w, const FinishShares sh, int final_launch) {
+finish_backward_kernel(const XentArgs a, const XentWs w, const FinishShares sh) {
   pdl_trigger();
   pdl_wait();
-  if (final_launch && any_error(w.hdr)) {
+  if (any_error(w.hdr)) {
     if (a.dX) fill_nan(static_cast<T*>(a.dX), a.N * a.D);
     if (a.dW) fill_nan(static_cast<T*>(a.dW), (int64_t)a.V * a.D);
     if (a.dbias) fill_nan(a.dbias, a.V);
@@ -568,8 +571,8 @@ finish_backward_kernel(const XentArgs a, const XentWs w, const FinishShares sh, 
   }
   b -= sh.dx;
   if (b < sh.dw) {
-    store_slots<T>(Share{b, sh.dw}, w.dw_slots, w.ks_w, w.piece, w.ldS, a.D, sh.nv, nullptr, sc.dw,
-                   sh.lanes, static_cast<T*>(a.dW) + (int64_t)sh.v0 * a.D);
+    store_slots<T>(Share{b, sh.dw}, w.dw_slots, w.ks_w, w.piece, w.ldS, a.D, a.V, nullptr, sc.dw,
+                   sh.lanes, static_cast<T*>(a.dW));
     return;
   }
   if (b - sh.dw < sh.dbias) store_dbias(b - sh.dw, a, w);
@@ -751,7 +754,6 @@ cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
   p.tlogit = w.tlogit;
   p.target = direct ? nullptr : w.target;
   p.targets = a.targets;
-  p.first = 1;
   e = launch_mma<true, T>(a, p, maps, w.Np / kPairRows * w.splits, dependent);
   if (e != cudaSuccess) return e;
   return launch(finish_forward_kernel, (a.N + 31) / 32, 1024, 0, a.stream, true, a, w, (int)direct);
@@ -764,86 +766,47 @@ cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
   cudaError_t e = make_operand_maps<T>(a, w, false, &maps);
   bool dependent;
   if (e == cudaSuccess) e = prepare<T>(a, w, false, true, &dependent);
-  CUtensorMap gmap[2], gmap2[2];
   EncodeTiled enc;
   if (e == cudaSuccess) e = encode_fn(&enc);
-  for (int b = 0; b < 2 && e == cudaSuccess; ++b) {
-    e = make_map(enc, &gmap[b], w.G[b], w.row_chunk, w.piece, w.piece, std::is_same<T, __nv_bfloat16>::value);
-    if (kSplit && e == cudaSuccess) e = make_map(enc, &gmap2[b], w.G2[b], w.row_chunk, w.piece, w.piece, false);
-  }
+  const int64_t ring_rows = (int64_t)kRing * w.row_chunk;
+  if (e == cudaSuccess)
+    e = make_map(enc, &maps.G, w.G, ring_rows, w.piece, w.piece, std::is_same<T, __nv_bfloat16>::value);
+  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps.G2, w.G2, ring_rows, w.piece, w.piece, false);
   if (e != cudaSuccess) return e;
   MmaParams p = common_params(a, w);
   p.bn_d = w.bn_d;
   p.tiles_d = w.tiles_d;
+  p.has_dx = a.dX != nullptr;
+  p.has_dw = a.dW != nullptr;
+  p.row_chunk = w.row_chunk;
+  p.piece = w.piece;
+  p.n_chunks = w.n_chunks;
+  p.n_pieces = w.n_pieces;
+  p.sync = w.sync;
   p.rg = w.rg;
-  p.ldG = w.piece;
+  p.G = w.G;
+  p.G2 = w.G2;
   p.dbias_part = a.dbias ? w.dbias_part : nullptr;
   p.ks_x = w.ks_x;
   p.ks_w = w.ks_w;
   p.dx_slots = w.dx_slots;
-  p.dw_slots = w.dw_direct ? nullptr : w.dw_slots;
+  p.dw_slots = w.dw_slots;
   p.ldS = w.ldS;
-  p.dw_rows = w.piece;
   p.dW = a.dW;
-  p.dw_vec = a.D % 8 == 0 && sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(a.dW) & 15) == 0;
-  // The vocabulary's pieces, each over the row chunks: launch j makes piece j's g
-  // while it multiplies piece j - 1's.
-  const int total = w.n_pieces * w.n_chunks;
-  auto piece_at = [&](int j) {
-    const int vp = j / w.n_chunks, rc = j % w.n_chunks;
-    Piece q;
-    q.r0 = (int64_t)rc * w.row_chunk;
-    q.rows = (int)std::min<int64_t>(w.row_chunk, w.Np - q.r0);
-    q.v0 = (int)((int64_t)vp * w.piece);
-    q.nv = std::min(w.piece, a.V - q.v0);
-    return q;
+  p.dw_vec = a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(a.dW) & (4 * sizeof(T) - 1)) == 0;
+  const int64_t units = (int64_t)(w.row_chunk / 256) * (w.piece / 256) * w.n_chunks * w.n_pieces;
+  e = launch_mma<false, T>(a, p, maps, std::max<int64_t>(units, XentWs::kPairs), true);
+  if (e != cudaSuccess) return e;
+  FinishShares sh{};
+  sh.lanes = row_lanes((a.D + 3) / 4, 1024);
+  auto blocks = [&](int64_t rows) {
+    return (int)std::min<int64_t>((rows * sh.lanes + 1023) / 1024, 2 * num_sms());
   };
-  for (int j = 0; j <= total; ++j) {
-    p.has_grad = j < total;
-    p.has_dx = j > 0 && a.dX != nullptr;
-    p.has_dw = j > 0 && a.dW != nullptr;
-    if (!p.has_grad && !p.has_dx && !p.has_dw) {   // dbias alone: its sums are complete
-      FinishShares sh{};
-      sh.dbias = (a.V + 31) / 32;
-      return launch(finish_backward_kernel<T>, sh.dbias, 1024, 0, a.stream, true, a, w, sh, 1);
-    }
-    p.cur = piece_at(std::min(j, total - 1));
-    p.prev = piece_at(std::max(j - 1, 0));
-    p.dx_add = j - 1 >= w.n_chunks;
-    p.dw_add = p.prev.r0 > 0;
-    p.G = w.G[j & 1];
-    p.G2 = w.G2[j & 1];
-    maps.G = gmap[(j & 1) ^ 1];
-    maps.G2 = gmap2[(j & 1) ^ 1];
-    const int64_t units =
-        (p.has_grad ? (int64_t)(p.cur.rows / 256) * ((p.cur.nv + kBN - 1) / kBN) : 0) +
-        (p.has_dx ? (int64_t)(p.prev.rows / 256) * w.tiles_d * w.ks_x : 0) +
-        (p.has_dw ? (int64_t)((p.prev.nv + 255) / 256) * w.tiles_d * w.ks_w : 0);
-    p.first = j == 0;
-    e = launch_mma<false, T>(a, p, maps, units, true);
-    if (e != cudaSuccess) return e;
-    // dW's slots are complete after the piece's last row chunk; with the last piece, all
-    // sums are
-    const bool last = j == total;
-    const bool dw = p.has_dw && !w.dw_direct && j % w.n_chunks == 0;
-    if (dw || last) {
-      FinishShares sh{};
-      const int pieces = (a.D + 3) / 4;
-      sh.lanes = row_lanes(pieces, 1024);
-      auto blocks = [&](int64_t rows) {
-        return (int)std::min<int64_t>((rows * sh.lanes + 1023) / 1024, 2 * num_sms());
-      };
-      sh.dx = last && a.dX ? blocks(a.N) : 0;
-      sh.dw = dw ? blocks(p.prev.nv) : 0;
-      sh.dbias = last && a.dbias ? (a.V + 31) / 32 : 0;
-      sh.v0 = p.prev.v0;
-      sh.nv = p.prev.nv;
-      e = launch(finish_backward_kernel<T>, std::max(sh.dx + sh.dw + sh.dbias, 1), 1024, 0, a.stream,
-                 true, a, w, sh, (int)last);
-      if (e != cudaSuccess) return e;
-    }
-  }
-  return cudaSuccess;
+  sh.dx = a.dX ? blocks(a.N) : 0;
+  sh.dw = a.dW && w.ks_w > 1 ? blocks(a.V) : 0;
+  sh.dbias = a.dbias ? (a.V + 31) / 32 : 0;
+  return launch(finish_backward_kernel<T>, std::max(sh.dx + sh.dw + sh.dbias, 1), 1024, 0, a.stream,
+                true, a, w, sh);
 }
 
 int check_common(const XentArgs& a) {

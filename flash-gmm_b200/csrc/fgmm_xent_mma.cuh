@@ -46,17 +46,9 @@ constexpr int kLogitBlocks = 4;   // 16 steps
 
 enum TileKind { kLse = 0, kGrad = 1, kDx = 2, kDw = 3 };
 
-// A rectangle of live rows x vocabulary.
-struct Piece {
-  int64_t r0;   // first live row (multiple of 256)
-  int rows;     // rows at most (multiple of 256); the last live row may end it earlier
-  int v0, nv;   // vocabulary [v0, v0 + nv); v0 multiple of 256
-};
-
 struct MmaParams {
   const int* live;         // unused where target is null
   int *err, *done;         // Header
-  int first;               // first launch of the call: err and done start at 0
   int64_t N;
   int D, V, kbD;           // kbD = ceil(D / 64)
   int bn_d, tiles_d;       // column tiles of dX and dW: width 128 or 256, count
@@ -70,21 +62,21 @@ struct MmaParams {
   const float* bias;       // padded to 256 with -inf, or null
   const int* amax;         // float bits of the largest |g weight|, |x|, |w| (Scales)
   // backward
-  int has_grad, has_dx, has_dw;
-  Piece cur, prev;         // of kGrad, and of kDx / kDw
+  int has_dx, has_dw;
+  int row_chunk, piece;    // rows x entries of a piece of G (multiples of 256)
+  int n_chunks, n_pieces;  // row chunks at most, pieces of the vocabulary
+  uint32_t* sync;          // from 0: units claimed, then marks of kGrad and of the products by
+                           // piece, then of each tile of dX's and of dW's slots
   const RowGrad* rg;
-  void *G, *G2;            // written by kGrad (G2: lo words)
-  int64_t ldG;
+  void *G, *G2;            // [kRing row_chunk][piece] words (G2: lo words)
   float* dbias_part;       // [2 Np / 256][Vp], or null
   int64_t Vp;
   int ks_x, ks_w;          // splits of K
   float* dx_slots;         // [ks_x][Np][ldS]
-  float* dw_slots;         // [ks_w][piece rows][ldS], or null: written to dW
+  float* dw_slots;         // [ks_w][piece][ldS]
   int64_t ldS;
-  int64_t dw_rows;
-  int dx_add, dw_add;      // add to the slots (a later piece / row chunk)
   void* dW;
-  int dw_vec;              // dW's rows take 16-byte stores
+  int dw_vec;              // dW's rows take stores of four elements
 };
 
 struct MmaMaps {
@@ -118,14 +110,19 @@ struct Scales {
   }
 };
 
-struct Tile {
-  int kind;
-  int64_t arow, brow;   // first A / B row (K-major) or column (MN-major) of the pair's tile
-  int64_t ak, bk;       // first K of A / B
-  int nkb;              // K blocks
-  int bn;
-  int m, n, ks;         // tile indices
-  int last;             // kLse: last tile of the unit
+// One tile, as every role gets it (16 words).
+struct __align__(16) Tile {
+  int kind;             // TileKind, or -1: no more
+  int arow, brow;       // first A / B row (K-major) or column (MN-major) of the pair's tile
+  int ak, bk;           // first K of A / B
+  int nkb, bn;          // K blocks, columns
+  int ks;               // split of K; kLse: the unit's range of the vocabulary
+  int flags;            // kLse: 1 last, 2 first tile of its unit; products: 1 add, 2 final
+  int j;                // backward: the piece
+  int x0, x1;           // kGrad: row, column of G; kDx: row of dX; kDw: row of the piece, v0
+  uint32_t w0, w1;      // marks to wait for (wait_marks)
+  int cell;             // products: their tile of the slots
+  int pad;
 };
 
 // Programmatic dependent launch: let the next kernel of the stream be set up, and wait
@@ -204,94 +201,222 @@ struct MmaCfg {
   static constexpr int kB = (kBN / 2 / 64) * kBoxBytes;      // this SM's half of B
   static constexpr int kStage = (SPLIT ? 2 : 1) * (kA + kB);
   static constexpr int kStageOut = kEpiWarps * 4096;         // 32 rows x 128 B per warp
-  static constexpr int kCtl = 256;
+  static constexpr int kCtl = 512;
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStageOut + kCtl;
   static_assert(kSmem <= 232448, "shared memory budget");
 };
 
+constexpr int kFeed = 3;          // tiles handed out ahead of the slowest role
+
 struct MmaCtl {
+  Tile feed[kFeed];
   uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
+  uint64_t feed_full[kFeed], feed_empty[kFeed], unit_done[kFeed];
   uint32_t tmem;
   volatile int abort_flag;
 };
-static_assert(sizeof(MmaCtl) <= 256, "control block");
+static_assert(sizeof(MmaCtl) <= 512, "control block");
 
-// The pair's tiles in order: the same sequence for every role.
-template <bool FWD, bool SPLIT>
-struct TileWalk {
+// The forward tiles of a pair in order: units of per_split vocabulary tiles of a row
+// tile, dealt in turn (rows fastest: pairs at work share the vocabulary's tiles).
+struct ForwardWalk {
   const MmaParams& p;
-  int64_t live;
-  int unit, step, sub = 0, um = 0, us = 0;
-  int mt, mtx, n_dw, n_dx, n_grad, units;
-  __device__ TileWalk(const MmaParams& p_, int pair, int npairs) : p(p_), unit(pair), step(npairs) {
-    live = FWD && !p.target ? p.N : *p.live;
-    if (FWD) {
-      mt = (int)((live + kPairRows - 1) / kPairRows);
-      units = mt * p.splits;
-    } else {
-      auto tiles = [&](const Piece& q) {
-        const int64_t r = live - q.r0;
-        return (int)((max((int64_t)0, min(r, (int64_t)q.rows)) + kPairRows - 1) / kPairRows);
-      };
-      mtx = tiles(p.prev);
-      mt = tiles(p.cur);
-      n_dw = p.has_dw ? (p.prev.nv + kPairRows - 1) / kPairRows * p.tiles_d * p.ks_w : 0;
-      n_dx = p.has_dx ? mtx * p.tiles_d * p.ks_x : 0;
-      n_grad = p.has_grad ? mt * ((p.cur.nv + kBN - 1) / kBN) : 0;
-      units = n_dw + n_dx + n_grad;
-    }
+  int unit, step, sub = 0, m = 0, s = 0, mt;
+  int64_t units;
+  __device__ ForwardWalk(const MmaParams& p_, int pair, int npairs) : p(p_), unit(pair), step(npairs) {
+    const int64_t live = p.target ? *p.live : p.N;
+    mt = (int)((live + kPairRows - 1) / kPairRows);
+    units = (int64_t)mt * p.splits;
   }
   __device__ bool next(Tile& t) {
     if (unit >= units) return false;
-    if (FWD) {
-      if (sub == 0) { us = unit / mt; um = unit - us * mt; }
-      const int m = um, s = us;
-      const int v = s * p.per_split + sub;
-      t.kind = kLse;
-      t.m = m; t.n = v; t.ks = s;
-      t.arow = (int64_t)m * kPairRows; t.ak = 0;
-      t.brow = (int64_t)v * kBN; t.bk = 0;
-      t.nkb = p.kbD; t.bn = kBN;
-      ++sub;
-      t.last = sub == p.per_split || v + 1 == p.vtiles;
-      if (t.last) { sub = 0; unit += step; }
-      return true;
-    }
-    int u = unit;
-    unit += step;
-    t.last = 0;
-    if (u < n_dw) {          // column tiles fastest: they share G's columns
-      t.kind = kDw;
-      t.n = u % p.tiles_d; u /= p.tiles_d;
-      t.ks = u % p.ks_w; t.m = u / p.ks_w;
-      const int64_t rows = max((int64_t)0, min(live - p.prev.r0, (int64_t)p.prev.rows));
-      const int nkb = (int)((rows + 63) / 64), per = (nkb + p.ks_w - 1) / p.ks_w;
-      const int k0 = t.ks * per;
-      t.nkb = max(0, min(per, nkb - k0));
-      t.arow = (int64_t)t.m * kPairRows; t.ak = (int64_t)k0 * 64;            // of G
-      t.brow = (int64_t)t.n * p.bn_d; t.bk = p.prev.r0 + (int64_t)k0 * 64;   // of Xp
-      t.bn = p.bn_d;
-    } else if ((u -= n_dw) < n_dx) {
-      t.kind = kDx;
-      t.n = u % p.tiles_d; u /= p.tiles_d;
-      t.ks = u % p.ks_x; t.m = u / p.ks_x;
-      const int nkb = (p.prev.nv + 63) / 64, per = (nkb + p.ks_x - 1) / p.ks_x;
-      const int k0 = t.ks * per;
-      t.nkb = max(0, min(per, nkb - k0));
-      t.arow = (int64_t)t.m * kPairRows; t.ak = (int64_t)k0 * 64;            // of G
-      t.brow = (int64_t)t.n * p.bn_d; t.bk = p.prev.v0 + (int64_t)k0 * 64;   // of W
-      t.bn = p.bn_d;
-    } else {
-      u -= n_dx;
-      t.kind = kGrad;
-      t.m = u % mt; t.n = u / mt; t.ks = 0;
-      t.arow = p.cur.r0 + (int64_t)t.m * kPairRows; t.ak = 0;                // of Xp
-      t.brow = p.cur.v0 + (int64_t)t.n * kBN; t.bk = 0;                       // of W
-      t.nkb = p.kbD; t.bn = kBN;
+    if (sub == 0) { s = unit / mt; m = unit - s * mt; }
+    const int v = s * p.per_split + sub;
+    t.kind = kLse;
+    t.ks = s;
+    t.arow = m * kPairRows; t.ak = 0;
+    t.brow = v * kBN; t.bk = 0;
+    t.nkb = p.kbD; t.bn = kBN;
+    t.flags = sub == 0 ? 2 : 0;
+    ++sub;
+    if (sub == p.per_split || v + 1 == p.vtiles) {
+      t.flags |= 1;
+      sub = 0;
+      unit += step;
     }
     return true;
   }
 };
+
+// The backward tiles.  G runs through a ring of kRing pieces (row chunk x piece of the
+// vocabulary, the chunks of one piece of the vocabulary in a row) that stays in the L2:
+// step j makes piece j's g (kGrad) and multiplies piece j - kLag's (kDx, kDw), the two
+// kinds mixed, since one is bound by its epilogue and the other by its products.  Pairs
+// claim units in this one order, and a unit waits only for units before it in the order,
+// so whichever pairs are resident make progress.  What a unit needs of others:
+//   kGrad j       the products of piece j - kRing (the ring's buffer is free)
+//   products i    all of piece i's g, and the unit before it on the same tile of the slots
+// Each is a count of marks, one per SM that has finished its half of a unit (mark role).
+constexpr int kRing = 4;
+constexpr int kLag = 2;
+constexpr uint32_t kMarks = 2;
+
+struct BackwardList {
+  const MmaParams& p;
+  int live, chunks, pieces;              // row chunks that hold live rows, pieces in all
+  int step = 0, base = 0, n_grad = 0, n_prod = 0;
+  struct Size { int rows, mt, v0, nv, vt; };
+  __device__ explicit BackwardList(const MmaParams& p_) : p(p_) {
+    live = *p.live;
+    chunks = max(1, (live + p.row_chunk - 1) / p.row_chunk);
+    pieces = chunks * p.n_pieces;
+    load();
+  }
+  __device__ Size size(int j) const {
+    const int vp = j / chunks, rc = j - vp * chunks;
+    Size s;
+    s.rows = min(live - rc * p.row_chunk, p.row_chunk);
+    s.mt = (s.rows + kPairRows - 1) / kPairRows;
+    s.v0 = vp * p.piece;
+    s.nv = min(p.piece, p.V - s.v0);
+    s.vt = (s.nv + 255) / 256;
+    return s;
+  }
+  __device__ int grads(int j) const {
+    if (j < 0 || j >= pieces) return 0;
+    const Size s = size(j);
+    return s.mt * s.vt;
+  }
+  __device__ int products(int j) const {
+    if (j < 0 || j >= pieces) return 0;
+    const Size s = size(j);
+    return (p.has_dx ? s.mt * p.tiles_d * p.ks_x : 0) + (p.has_dw ? s.vt * p.tiles_d * p.ks_w : 0);
+  }
+  uint64_t share = 0;
+  __device__ void load() {
+    n_grad = grads(step);
+    n_prod = products(step - kLag);
+    const int n = n_grad + n_prod;
+    share = n > 0 ? ((uint64_t)n_prod << 32) / (uint64_t)n : 0;
+  }
+  // Products among the step's first i of n units, floor(i n_prod / n): in steps of 0 or 1.
+  // The multiplication errs by less than n 2^-32 downwards, the quotients below n_prod are
+  // at least 1/n off a whole number or exactly one: right for n < 2^15.
+  __device__ int upto(int i) const {
+    const int n = n_grad + n_prod;
+    if (i >= n) return n_prod;
+    if (n >= 1 << 15) return (int)((uint64_t)i * n_prod / n);
+    return (int)(((uint64_t)(uint32_t)i * share + (1u << 16)) >> 32);
+  }
+  // Unit u (never smaller than the one before); kind -1 behind the last.
+  __device__ void get(int u, Tile& t) {
+    while (step < pieces + kLag && u >= base + n_grad + n_prod) {
+      base += n_grad + n_prod;
+      ++step;
+      load();
+    }
+    if (step >= pieces + kLag) { t.kind = -1; return; }
+    // products spread evenly among the step's units
+    const int i = u - base;
+    const int prod = upto(i);
+    if (upto(i + 1) == prod) {
+      const Size s = size(step);
+      const int g = i - prod, vt = g / s.mt, m = g - vt * s.mt;
+      t.kind = kGrad;
+      t.j = step;
+      t.arow = (step % chunks) * p.row_chunk + m * kPairRows; t.ak = 0;   // of Xp
+      t.brow = s.v0 + vt * kBN; t.bk = 0;                                 // of W
+      t.nkb = p.kbD; t.bn = kBN;
+      t.ks = 0; t.flags = 0;
+      t.x0 = (step % kRing) * p.row_chunk + m * kPairRows;
+      t.x1 = vt * kBN;
+      t.w0 = kMarks * (uint32_t)products(step - kRing);
+      t.w1 = 0;
+      return;
+    }
+    const int j = step - kLag;
+    const Size s = size(j);
+    const int rc = j % chunks, g0 = (j % kRing) * p.row_chunk;
+    const int n_dx = p.has_dx ? s.mt * p.tiles_d * p.ks_x : 0;
+    t.j = j;
+    t.bn = p.bn_d;
+    t.w0 = kMarks * (uint32_t)(s.mt * s.vt);
+    if (prod < n_dx) {
+      int u2 = prod;
+      const int tn = u2 % p.tiles_d;
+      u2 /= p.tiles_d;
+      t.ks = u2 % p.ks_x;
+      const int m = u2 / p.ks_x;
+      const int nkb = (s.nv + 63) / 64, per = (nkb + p.ks_x - 1) / p.ks_x, k0 = t.ks * per;
+      t.kind = kDx;
+      t.nkb = max(0, min(per, nkb - k0));
+      t.arow = g0 + m * kPairRows; t.ak = k0 * 64;                        // of G
+      t.brow = tn * p.bn_d; t.bk = s.v0 + k0 * 64;                        // of W
+      t.flags = j >= chunks ? 1 : 0;
+      t.x0 = rc * p.row_chunk + m * kPairRows;
+      t.x1 = 0;
+      t.w1 = kMarks * (uint32_t)(j / chunks);
+      t.cell = ((t.x0 / kPairRows) * p.ks_x + t.ks) * p.tiles_d + tn;
+    } else {
+      int u2 = prod - n_dx;
+      const int tn = u2 % p.tiles_d;
+      u2 /= p.tiles_d;
+      t.ks = u2 % p.ks_w;
+      const int m = u2 / p.ks_w;
+      const int nkb = (s.rows + 63) / 64, per = (nkb + p.ks_w - 1) / p.ks_w, k0 = t.ks * per;
+      t.kind = kDw;
+      t.nkb = max(0, min(per, nkb - k0));
+      t.arow = m * kPairRows; t.ak = g0 + k0 * 64;                        // of G
+      t.brow = tn * p.bn_d; t.bk = rc * p.row_chunk + k0 * 64;            // of Xp
+      t.flags = (rc > 0 ? 1 : 0) | (rc == chunks - 1 && p.ks_w == 1 ? 2 : 0);
+      t.x0 = m * kPairRows;
+      t.x1 = s.v0;
+      t.w1 = kMarks * (uint32_t)j;
+      t.cell = ((int)(p.Np / kPairRows) * p.ks_x + m * p.ks_w + t.ks) * p.tiles_d + tn;
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void fence_async_all() {
+  asm volatile("fence.proxy.async;" ::: "memory");
+}
+// One lane's bounded wait until *count reaches `need`.
+__device__ __forceinline__ bool wait_marks(const uint32_t* count, uint32_t need,
+                                           volatile int* abort_flag, int* err, int code) {
+  if (need == 0 || ld_acquire(count) >= need) return true;
+  const long long t0 = clock64();
+  while (ld_acquire(count) < need) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kTimeoutCycles) {
+      *abort_flag = 1;
+      atomicOr(err, code);
+      return false;
+    }
+    __nanosleep(32);
+  }
+  return true;
+}
+// Writes a tile into the feed of an SM of the pair; its barrier completes when all 64
+// bytes are there (no fence: a release at cluster scope took most of the claim's time).
+__device__ __forceinline__ void send_tile(uint32_t dst, uint32_t bar, const Tile& t) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar),
+               "r"((uint32_t)sizeof(Tile))
+               : "memory");
+  const uint4* v = reinterpret_cast<const uint4*>(&t);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    asm volatile(
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+            dst + 16u * k),
+        "r"(v[k].x), "r"(v[k].y), "r"(v[k].z), "r"(v[k].w), "r"(bar)
+        : "memory");
+}
+static_assert(sizeof(Tile) == 64, "a feed entry");
 
 // Sums the 32 values of each column over the warp's 32 rows: lane c gets column c.
 __device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
@@ -383,6 +508,11 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       mbar_init(&ctl->acc_full[b], 1);                // commit
       mbar_init(&ctl->acc_empty[b], 2 * kEpiWarps);   // both SMs' epilogue warps
     }
+    for (int b = 0; b < kFeed; ++b) {
+      mbar_init(&ctl->feed_full[b], 1);
+      mbar_init(&ctl->feed_empty[b], 2 * (kEpiWarps + 2) + 1);   // epilogue, loads, marks; MMA
+      mbar_init(&ctl->unit_done[b], kEpiWarps);
+    }
     mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -402,32 +532,47 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
   pdl_trigger();
   pdl_wait();
   int* err = p.err + blockIdx.x;
-  if (p.first) {
-    if (threadIdx.x == 0)
-      for (int i = blockIdx.x; i < kErrSlots; i += gridDim.x) p.err[i] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
-    __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = blockIdx.x; i < kErrSlots; i += gridDim.x) p.err[i] = 0;
+    if (FWD && blockIdx.x == 0) *p.done = 0;
   }
+  __syncthreads();
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     return mbar_wait_flag(bar, parity, &ctl->abort_flag, err, code);
   };
+  // Backward: tile number n of the feed, for one lane; false after the last and on abort.
+  const uint32_t feed_empty0 = map_to_cta(smem_u32(&ctl->feed_empty[0]), 0);
+  auto take = [&](uint32_t n, Tile& t) {
+    const uint32_t s = n % kFeed;
+    if (!wait(&ctl->feed_full[s], (n / kFeed) & 1, 64)) return false;
+    t = ctl->feed[s];
+    arrive_cluster(feed_empty0 + 8u * s);
+    return t.kind >= 0;
+  };
+  uint32_t* grad_marks = p.sync + 1;
+  uint32_t* prod_marks = grad_marks + p.n_chunks * p.n_pieces;
+  uint32_t* cell_marks = prod_marks + p.n_chunks * p.n_pieces;
 
   if (warp < 4) {
     regs_down<72>();
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ loads
-      TileWalk<FWD, SPLIT> walk(p, pair, npairs);
+      ForwardWalk walk(p, pair, npairs);
       Tile t;
       uint32_t it = 0;
       bool ok = true;
-      while (ok && walk.next(t)) {
+      for (uint32_t n = 0; ok && (FWD ? walk.next(t) : take(n, t)); ++n) {
+        if (!FWD && t.kind >= kDx) {   // its G was written by other SMs' plain stores
+          if (!wait_marks(grad_marks + t.j, t.w0, &ctl->abort_flag, err, 128)) { ok = false; break; }
+          fence_async_all();
+        }
         const bool a_mn = t.kind == kDw, b_mn = t.kind >= kDx;
         const CUtensorMap* ma = t.kind <= kGrad ? &maps.X : &maps.G;
         const CUtensorMap* mb = t.kind == kDw ? &maps.X : &maps.W;
         const CUtensorMap* ma2 = t.kind <= kGrad ? &maps.X2 : &maps.G2;
         const CUtensorMap* mb2 = t.kind == kDw ? &maps.X2 : &maps.W2;
         const int bboxes = t.bn / 128;                       // 64-row boxes of B per SM
-        const int ar = (int)t.arow + 128 * (int)rank, br = (int)t.brow + t.bn / 2 * (int)rank;
+        const int ar = t.arow + 128 * (int)rank, br = t.brow + t.bn / 2 * (int)rank;
         const uint32_t bytes = (uint32_t)((SPLIT ? 2 : 1) * (2 + bboxes) * kBoxBytes);
         for (int kb = 0; kb < t.nkb; ++kb, ++it) {
           const int s = it % NS;
@@ -435,7 +580,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * bytes);
           const uint32_t bar = map_to_cta(smem_u32(&ctl->full[s]), 0);
           uint32_t dst = smem_u32(smem + s * Cfg::kStage);
-          const int ka = (int)t.ak + kb * 64, kbb = (int)t.bk + kb * 64;
+          const int ka = t.ak + kb * 64, kbb = t.bk + kb * 64;
           for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
             const CUtensorMap* a = h ? ma2 : ma;
             const CUtensorMap* b = h ? mb2 : mb;
@@ -450,50 +595,71 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       // every stage handed back; after a timeout, time for the copies in flight to land
       for (uint32_t k = it > NS ? it - NS : 0; ok && k < it; ++k)
         ok = wait(&ctl->empty[k % NS], (k / NS) & 1, 2);
-      if (!ok) idle_cycles(4000000);
-    } else if (warp == 1 && rank == 0 && lane == 0) {
+      if (!ok || ctl->abort_flag) idle_cycles(4000000);
+    } else if (warp == 1 && rank == 0) {
       // ------------------------------------------------------------ MMA
-      TileWalk<FWD, SPLIT> walk(p, pair, npairs);
+      // The whole warp runs the loop, so that addresses and descriptors are warp-uniform
+      // values; an elected lane issues each K-block.  Issued from one lane's branch, a
+      // block of four MMAs took about 750 cycles to issue, whatever its width.
+      ForwardWalk walk(p, pair, npairs);
       Tile t;
       uint32_t it = 0, ac = 0;
       bool ok = true;
       constexpr bool f16 = std::is_same<T, __half>::value;
-      while (ok && walk.next(t)) {
+      auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
+        return (bool)__all_sync(0xffffffffu, wait(bar, parity, code));
+      };
+      auto take_all = [&](uint32_t n) {
+        if (FWD) return walk.next(t);
+        const uint32_t s = n % kFeed;
+        if (!wait_all(&ctl->feed_full[s], (n / kFeed) & 1, 64)) return false;
+        t = ctl->feed[s];
+        __syncwarp();
+        if (lane == 0) arrive_cluster(feed_empty0 + 8u * s);
+        return t.kind >= 0;
+      };
+      const uint32_t smem0 = smem_u32(smem);
+      for (uint32_t n = 0; ok && take_all(n); ++n) {
         const bool a_mn = t.kind == kDw, b_mn = t.kind >= kDx;
         const uint32_t idesc = (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) |
                                (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
                                ((uint32_t)(t.bn >> 3) << 17) | (16u << 24);
+        // K-major: 16 K are 32 bytes of a row; MN-major: 16 rows of 128 bytes
+        const uint32_t as = a_mn ? 2048 >> 4 : 32 >> 4, bs = b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint32_t alo = a_mn ? (uint32_t)(kBoxBytes >> 4) << 16 : 1u << 16;
+        const uint32_t blo = b_mn ? (uint32_t)(kBoxBytes >> 4) << 16 : 1u << 16;
         const int group = group_blocks<SPLIT, f16>(p, t);
         for (int k0 = 0; ok && k0 < t.nkb; k0 += group, ++ac) {
           const uint32_t d = tmem + (uint32_t)kBN * (ac & 1);
-          if (ac >= 2 && !wait(&ctl->acc_empty[ac & 1], ((ac >> 1) - 1) & 1, 4)) { ok = false; break; }
+          if (ac >= 2 && !wait_all(&ctl->acc_empty[ac & 1], ((ac >> 1) - 1) & 1, 4)) { ok = false; break; }
           tc_fence_after();
           const int k1 = min(t.nkb, k0 + group);
           for (int kb = k0; kb < k1; ++kb, ++it) {
             const int s = it % NS;
-            if (!wait(&ctl->full[s], (it / NS) & 1, 8)) { ok = false; break; }
+            if (!wait_all(&ctl->full[s], (it / NS) & 1, 8)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t a0 = smem_u32(smem + s * Cfg::kStage);
-            const uint32_t b0 = a0 + Cfg::kA;
-            constexpr uint32_t lo = Cfg::kA + Cfg::kB;
+            const uint32_t a0 = (smem0 + (uint32_t)(s * Cfg::kStage)) >> 4;
+            const uint32_t ad = a0 | alo, bd = (a0 + (Cfg::kA >> 4)) | blo;
+            constexpr uint32_t lo = (Cfg::kA + Cfg::kB) >> 4;
+            const uint32_t more = kb > k0 ? 1u : 0u;
+            if (elect_one()) {
 #pragma unroll
-            for (int term = SPLIT ? 0 : 2; term < 3; ++term) {   // lo hi, hi lo, hi hi
-              const uint32_t a = a0 + (term == 0 ? lo : 0u), b = b0 + (term == 1 ? lo : 0u);
-              const uint32_t ad = a_mn ? desc_lo_mnmajor(a, kBoxBytes) : desc_lo_kmajor(a);
-              const uint32_t bd = b_mn ? desc_lo_mnmajor(b, kBoxBytes) : desc_lo_kmajor(b);
-              const uint32_t as = a_mn ? 2048 >> 4 : 32 >> 4, bs = b_mn ? 2048 >> 4 : 32 >> 4;
+              for (int term = SPLIT ? 0 : 2; term < 3; ++term) {   // lo hi, hi lo, hi hi
+                const uint32_t at = ad + (term == 0 ? lo : 0u), bt = bd + (term == 1 ? lo : 0u);
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_pair(d, ad + k * as, bd + k * bs, idesc,
-                         (kb > k0 || k > 0 || term > (SPLIT ? 0 : 2)) ? 1u : 0u);
+                for (int k = 0; k < 4; ++k)
+                  mma_pair(d, at + k * as, bt + k * bs, idesc,
+                           (k > 0 || term > (SPLIT ? 0 : 2)) ? 1u : more);
+              }
+              commit_pair(&ctl->empty[s]);
+              if (kb + 1 == k1) commit_pair(&ctl->acc_full[ac & 1]);
             }
-            commit_pair(&ctl->empty[s]);
+            __syncwarp();
           }
-          if (ok) commit_pair(&ctl->acc_full[ac & 1]);
         }
       }
       // after a timeout: let what was issued finish (bounded) before TMEM is freed
-      if (!ok) {
+      if (!ok && lane == 0) {
         asm volatile(
             "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                 smem_u32(&ctl->drain))
@@ -501,11 +667,48 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         const long long t0 = clock64();
         while (!mbar_try(smem_u32(&ctl->drain), 0) && clock64() - t0 < 100000000LL) {}
       }
+    } else if (!FWD && warp == 2 && lane == 0) {
+      // ------------------------------------------------------------ marks
+      // The fence that makes a unit's stores visible to other SMs waits for them to land:
+      // here, not in the epilogue.  The feed's place is kept until then, which bounds how
+      // far the epilogue can run ahead of its marks.
+      for (uint32_t n = 0;; ++n) {
+        const uint32_t s = n % kFeed, parity = (n / kFeed) & 1;
+        if (!wait(&ctl->feed_full[s], parity, 64)) break;
+        const int kind = ctl->feed[s].kind, j = ctl->feed[s].j, cell = ctl->feed[s].cell;
+        if (kind < 0) break;
+        if (!wait(&ctl->unit_done[s], parity, 1024)) break;
+        arrive_cluster(feed_empty0 + 8u * s);
+        __threadfence();
+        fence_async_all();
+        if (kind == kGrad) {
+          atomicAdd(grad_marks + j, 1u);
+        } else {
+          atomicAdd(prod_marks + j, 1u);
+          atomicAdd(cell_marks + cell, 1u);
+        }
+      }
+    } else if (!FWD && warp == 3 && rank == 0 && lane == 0) {
+      // ------------------------------------------------------------ claims
+      BackwardList list(p);
+      uint32_t claim = atomicAdd(p.sync, 1u);
+      for (uint32_t n = 0;; ++n) {
+        const uint32_t s = n % kFeed;
+        if (n >= kFeed && !wait(&ctl->feed_empty[s], (n / kFeed - 1) & 1, 256)) break;
+        Tile t = {};
+        list.get((int)claim, t);
+        if (t.kind >= 0) claim = atomicAdd(p.sync, 1u);   // the next, on its way meanwhile
+#pragma unroll
+        for (uint32_t c = 0; c < 2; ++c)
+          send_tile(map_to_cta(smem_u32(&ctl->feed[s]), c),
+                    map_to_cta(smem_u32(&ctl->feed_full[s]), c), t);
+        if (t.kind < 0) break;
+      }
     }
   } else {
     regs_up<216>();
     // -------------------------------------------------------------- epilogue
-    TileWalk<FWD, SPLIT> walk(p, pair, npairs);
+    ForwardWalk walk(p, pair, npairs);
     Tile t;
     uint32_t ac = 0;
     const int q = warp & 3, wg = (warp - 4) >> 2;
@@ -526,16 +729,36 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       __syncwarp();
       if (lane == 0) arrive_cluster(empty0 + 8u * (a & 1));
     };
+    auto unit_done = [&](uint32_t n) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->unit_done[n % kFeed]);
+    };
     auto wg_sync = [&] {   // the warpgroup's 128 threads
       asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
     };
+    auto wait_warp = [&](const uint32_t* count, uint32_t need) {
+      bool there = true;
+      if (lane == 0) there = wait_marks(count, need, &ctl->abort_flag, err, 512);
+      return (bool)__all_sync(0xffffffffu, there);
+    };
+    auto next = [&](uint32_t n) {
+      if (FWD) return walk.next(t);
+      const uint32_t s = n % kFeed, parity = (n / kFeed) & 1;
+      bool there = true;
+      if (lane == 0) there = wait(&ctl->feed_full[s], parity, 64);
+      if (!__all_sync(0xffffffffu, there)) return false;
+      t = ctl->feed[s];
+      __syncwarp();
+      if (lane == 0) arrive_cluster(feed_empty0 + 8u * s);
+      return t.kind >= 0;
+    };
     bool ok = true;
-    while (ok && walk.next(t)) {
+    for (uint32_t n = 0; ok && next(n); ++n) {
       const int col0 = wg * (t.bn / 2);                     // this warp's columns of the tile
       const int chunks = t.bn / 2 / 32;
       const int group = group_blocks<SPLIT, f16>(p, t);
       const int64_t row = t.arow + row_in;                  // kLse, kGrad: the live row
-      if (FWD && t.n == t.ks * p.per_split) {               // first tile of the unit
+      if (FWD && (t.flags & 2)) {                           // first tile of the unit
         m_run = -3.402823466e38f;
         s_run = 0.f;
         if (p.target) {
@@ -573,6 +796,12 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         release(ac);
       }
       if (!ok) break;
+      if (!FWD) {
+        // the ring's buffer is free; the slots' tile holds the sums so far
+        ok = t.kind == kGrad ? wait_warp(prod_marks + t.j - kRing, t.w0)
+                             : wait_warp(cell_marks + t.cell, t.w1);
+        if (!ok) break;
+      }
       if (t.nkb == 0) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
@@ -652,13 +881,12 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           unpack(add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])), sa, sb);
           s_run += sa + sb;
         }
-        if (t.last) p.part[(int64_t)(2 * t.ks + wg) * p.Np + row] = make_float2(m_run, s_run);
+        if (t.flags & 1) p.part[(int64_t)(2 * t.ks + wg) * p.Np + row] = make_float2(m_run, s_run);
         continue;
       }
 
       if (t.kind == kGrad) {
         const int v0 = (int)t.brow + col0;
-        const int vend = p.cur.v0 + p.cur.nv;
         const float ga = rg.a * scales.g, gb = rg.b * scales.g;
         if (p.bias) {
 #pragma unroll
@@ -688,16 +916,16 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         }
         // rows without a weight (padding) and entries behind the last: exactly zero
         const bool empty = rg.a == 0.f && rg.b == 0.f;
-        if (v0 + kCols > vend || __any_sync(0xffffffffu, empty)) {
+        if (v0 + kCols > p.V || __any_sync(0xffffffffu, empty)) {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (empty || v0 + 32 * c + i >= vend) acc[c][i] = 0.f;
+              if (empty || v0 + 32 * c + i >= p.V) acc[c][i] = 0.f;
         }
         // 128-byte staged rows: 64 columns of 16-bit words, or 32 of hi and lo words
-        const int64_t grow0 = row - lane - p.cur.r0;        // rows of the G buffer
-        const int64_t gcol0 = t.brow - p.cur.v0 + col0;
+        const int64_t grow0 = t.x0 + row_in - lane;
+        const int64_t gcol0 = t.x1 + col0;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
@@ -725,9 +953,9 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
               const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
               uint16_t* dst;
               if (SPLIT)
-                dst = static_cast<uint16_t*>(g < 4 ? p.G : p.G2) + (grow0 + r) * p.ldG + gcol + 8 * (g & 3);
+                dst = static_cast<uint16_t*>(g < 4 ? p.G : p.G2) + (grow0 + r) * p.piece + gcol + 8 * (g & 3);
               else
-                dst = static_cast<uint16_t*>(p.G) + (grow0 + r) * p.ldG + gcol + 8 * g;
+                dst = static_cast<uint16_t*>(p.G) + (grow0 + r) * p.piece + gcol + 8 * g;
               *reinterpret_cast<uint4*>(dst) = x;
             }
             __syncwarp();
@@ -746,65 +974,62 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + col0 + e] = s;
           wg_sync();
         }
+        unit_done(n);
         continue;
       }
 
-      // kDx, kDw: fp32 slots, or dW rows in their type
-      const bool dw = t.kind == kDw;
-      const bool direct = dw && !p.dw_slots;
-      const int64_t row0 = (dw ? t.arow : p.prev.r0 + t.arow) + 128 * (int)rank + 32 * q;
-      float* slots = dw ? p.dw_slots + (int64_t)t.ks * p.dw_rows * p.ldS
+      // kDx, kDw: into fp32 slots, or (the last sum of a dW tile) dW in its type
+      const bool dw = t.kind == kDw, add = t.flags & 1, direct = t.flags & 2;
+      const int64_t row0 = t.x0 + 128 * (int)rank + 32 * q;
+      float* slots = dw ? p.dw_slots + (int64_t)t.ks * p.piece * p.ldS
                         : p.dx_slots + (int64_t)t.ks * p.Np * p.ldS;
-      const int add = dw ? p.dw_add : p.dx_add;
       const float so = scales.dw;
+      const int64_t rows_left = (int64_t)p.V - t.x1 - row0;   // kDw: rows of dW from row0
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         if (c >= chunks) break;
         const float (&v)[32] = acc[c];
-        const int64_t col = t.brow + col0 + 32 * c;
-        // 32 fp32 columns = a 128-byte staged row
+        const int col = t.brow + col0 + 32 * c;
+        // 32 fp32 columns = a 128-byte staged row; then 8 lanes a row
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
               make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         __syncwarp();
-        if (!direct) {
+        const int g = lane & 7, at = col + 4 * g;
+        float4* slot0 = reinterpret_cast<float4*>(slots + (row0 + (lane >> 3)) * p.ldS + at);
+        float4 old[8];
+        if (add) {   // all in flight at once; written by other SMs
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + (lane >> 3), g = lane & 7;
-            float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
-            float4* dst = reinterpret_cast<float4*>(slots + (row0 + r) * p.ldS + col + 4 * g);
-            if (add) {
-              const float4 o = *dst;
-              x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w;
-            }
-            *dst = x;
-          }
-        } else if (p.dw_vec && col + 32 <= p.D) {
-          // 16-byte stores: 4 lanes a row, 8 rows at a time
+          for (int i = 0; i < 8; ++i) old[i] = __ldcg(slot0 + i * p.ldS);   // 4 rows of floats
+        }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 8 * i + (lane >> 2), g = 2 * (lane & 3);
-            const float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
-            const float4 y = *reinterpret_cast<const float4*>(stage + r * 128 + (((g + 1) ^ (r & 7)) << 4));
-            const int64_t vrow = row0 + r;
-            if (vrow < p.prev.nv) {
-              const uint4 w = make_uint4(pack2<TO>(x.x * so, x.y * so), pack2<TO>(x.z * so, x.w * so),
-                                         pack2<TO>(y.x * so, y.y * so), pack2<TO>(y.z * so, y.w * so));
-              *reinterpret_cast<uint4*>(static_cast<TO*>(p.dW) + (p.prev.v0 + vrow) * p.D + col + 4 * g) = w;
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3);
+          float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
+          float4* slot = slot0 + i * p.ldS;
+          if (add) { x.x += old[i].x; x.y += old[i].y; x.z += old[i].z; x.w += old[i].w; }
+          if (!direct) {
+            *slot = x;
+          } else if (r < rows_left) {
+            TO* dst = static_cast<TO*>(p.dW) + (t.x1 + row0 + r) * p.D + at;
+            TO y[4] = {from_f32<TO>(x.x * so), from_f32<TO>(x.y * so), from_f32<TO>(x.z * so),
+                       from_f32<TO>(x.w * so)};
+            if (p.dw_vec) {
+              if (at < p.D) {
+                if (sizeof(TO) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(y);
+                else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (at + k < p.D) dst[k] = y[k];
             }
-          }
-        } else {
-          for (int r = 0; r < 32; ++r) {
-            const float x = *reinterpret_cast<const float*>(
-                stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3));
-            const int64_t vrow = row0 + r;
-            if (vrow < p.prev.nv && col + lane < p.D)
-              static_cast<TO*>(p.dW)[(p.prev.v0 + vrow) * p.D + col + lane] = from_f32<TO>(x * so);
           }
         }
         __syncwarp();
       }
+      unit_done(n);
     }
   }
   __syncwarp();

@@ -55,7 +55,8 @@ def test_xent_matches_64_bits(N, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("N,V,D", [(5, 70001, 96), (2500, 9001, 320), (9000, 600, 64)])
+@pytest.mark.parametrize("N,V,D", [(5, 70001, 96), (2500, 9001, 320), (9000, 600, 64),
+                                   (6000, 12300, 40)])
 def test_xent_larger(N, V, D, dtype):
     X, W, t, c = R.problem(N, V, D, dtype, seed=7, ignored=0.3, bias=True)
     check_xent(X, W, t, c)
