@@ -540,30 +540,39 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     return mbar_wait_flag(bar, parity, &ctl->abort_flag, err, code);
   };
-  // Backward: tile number n of the feed, for one lane; false after the last and on abort.
   const uint32_t feed_empty0 = map_to_cta(smem_u32(&ctl->feed_empty[0]), 0);
-  auto take = [&](uint32_t n, Tile& t) {
-    const uint32_t s = n % kFeed;
-    if (!wait(&ctl->feed_full[s], (n / kFeed) & 1, 64)) return false;
-    t = ctl->feed[s];
-    arrive_cluster(feed_empty0 + 8u * s);
-    return t.kind >= 0;
-  };
   uint32_t* grad_marks = p.sync + 1;
   uint32_t* prod_marks = grad_marks + p.n_chunks * p.n_pieces;
   uint32_t* cell_marks = prod_marks + p.n_chunks * p.n_pieces;
 
   if (warp < 4) {
     regs_down<72>();
-    if (warp == 0 && lane == 0) {
+    // Loads and MMAs: the whole warp runs the loop, so that addresses, descriptors and
+    // coordinates are warp-uniform values, and an elected lane issues.  From one lane's
+    // branch, a block of four MMAs took about 750 cycles to issue, whatever its width.
+    auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
+      return (bool)__all_sync(0xffffffffu, wait(bar, parity, code));
+    };
+    // Backward: tile number n of the feed; false after the last and on abort.
+    auto take = [&](uint32_t n, Tile& t) {
+      const uint32_t s = n % kFeed;
+      if (!wait_all(&ctl->feed_full[s], (n / kFeed) & 1, 64)) return false;
+      t = ctl->feed[s];
+      __syncwarp();
+      if (lane == 0) arrive_cluster(feed_empty0 + 8u * s);
+      return t.kind >= 0;
+    };
+    if (warp == 0) {
       // ------------------------------------------------------------ loads
       ForwardWalk walk(p, pair, npairs);
       Tile t;
       uint32_t it = 0;
       bool ok = true;
+      const uint32_t smem0 = smem_u32(smem), full0 = map_to_cta(smem_u32(&ctl->full[0]), 0);
       for (uint32_t n = 0; ok && (FWD ? walk.next(t) : take(n, t)); ++n) {
         if (!FWD && t.kind >= kDx) {   // its G was written by other SMs' plain stores
-          if (!wait_marks(grad_marks + t.j, t.w0, &ctl->abort_flag, err, 128)) { ok = false; break; }
+          const bool there = wait_marks(grad_marks + t.j, t.w0, &ctl->abort_flag, err, 128);
+          if (!__all_sync(0xffffffffu, there)) { ok = false; break; }
           fence_async_all();
         }
         const bool a_mn = t.kind == kDw, b_mn = t.kind >= kDx;
@@ -571,55 +580,46 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         const CUtensorMap* mb = t.kind == kDw ? &maps.X : &maps.W;
         const CUtensorMap* ma2 = t.kind <= kGrad ? &maps.X2 : &maps.G2;
         const CUtensorMap* mb2 = t.kind == kDw ? &maps.X2 : &maps.W2;
-        const int bboxes = t.bn / 128;                       // 64-row boxes of B per SM
+        const bool wide = t.bn == 256;                       // two 64-row boxes of B per SM
         const int ar = t.arow + 128 * (int)rank, br = t.brow + t.bn / 2 * (int)rank;
-        const uint32_t bytes = (uint32_t)((SPLIT ? 2 : 1) * (2 + bboxes) * kBoxBytes);
+        const uint32_t bytes = (uint32_t)((SPLIT ? 4 : 2) * (wide ? 4 : 3) * kBoxBytes);
+        // coordinates of the boxes at K-block 0, and what a K-block and a box add to them
+        int ax = a_mn ? ar : t.ak, ay = a_mn ? t.ak : ar, bx = b_mn ? br : t.bk, by = b_mn ? t.bk : br;
+        const int akx = a_mn ? 0 : 64, aky = 64 - akx, bkx = b_mn ? 0 : 64, bky = 64 - bkx;
         for (int kb = 0; kb < t.nkb; ++kb, ++it) {
-          const int s = it % NS;
-          if (it >= NS && !wait(&ctl->empty[s], ((it / NS) - 1) & 1, 1)) { ok = false; break; }
-          if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * bytes);
-          const uint32_t bar = map_to_cta(smem_u32(&ctl->full[s]), 0);
-          uint32_t dst = smem_u32(smem + s * Cfg::kStage);
-          const int ka = t.ak + kb * 64, kbb = t.bk + kb * 64;
-          for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
-            const CUtensorMap* a = h ? ma2 : ma;
-            const CUtensorMap* b = h ? mb2 : mb;
-            for (int j = 0; j < 2; ++j, dst += kBoxBytes)
-              tma_load_pair(dst, a, a_mn ? ar + 64 * j : ka, a_mn ? ka : ar + 64 * j, bar);
-            for (int j = 0; j < bboxes; ++j, dst += kBoxBytes)
-              tma_load_pair(dst, b, b_mn ? br + 64 * j : kbb, b_mn ? kbb : br + 64 * j, bar);
-            if (SPLIT) dst = smem_u32(smem + s * Cfg::kStage) + Cfg::kA + Cfg::kB;
+          const uint32_t s = it % NS;
+          if (it >= NS && !wait_all(&ctl->empty[s], ((it / NS) - 1) & 1, 1)) { ok = false; break; }
+          const uint32_t dst = smem0 + s * Cfg::kStage, bar = full0 + 8u * s;
+          if (elect_one()) {
+            if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], bytes);
+#pragma unroll
+            for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
+              const CUtensorMap* a = h ? ma2 : ma;
+              const CUtensorMap* b = h ? mb2 : mb;
+              const uint32_t d = dst + h * (Cfg::kA + Cfg::kB);
+              tma_load_pair(d, a, ax, ay, bar);
+              tma_load_pair(d + kBoxBytes, a, ax + aky, ay + akx, bar);
+              tma_load_pair(d + 2 * kBoxBytes, b, bx, by, bar);
+              if (wide) tma_load_pair(d + 3 * kBoxBytes, b, bx + bky, by + bkx, bar);
+            }
           }
+          __syncwarp();
+          ax += akx; ay += aky; bx += bkx; by += bky;
         }
       }
       // every stage handed back; after a timeout, time for the copies in flight to land
       for (uint32_t k = it > NS ? it - NS : 0; ok && k < it; ++k)
-        ok = wait(&ctl->empty[k % NS], (k / NS) & 1, 2);
+        ok = wait_all(&ctl->empty[k % NS], (k / NS) & 1, 2);
       if (!ok || ctl->abort_flag) idle_cycles(4000000);
     } else if (warp == 1 && rank == 0) {
       // ------------------------------------------------------------ MMA
-      // The whole warp runs the loop, so that addresses and descriptors are warp-uniform
-      // values; an elected lane issues each K-block.  Issued from one lane's branch, a
-      // block of four MMAs took about 750 cycles to issue, whatever its width.
       ForwardWalk walk(p, pair, npairs);
       Tile t;
       uint32_t it = 0, ac = 0;
       bool ok = true;
       constexpr bool f16 = std::is_same<T, __half>::value;
-      auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
-        return (bool)__all_sync(0xffffffffu, wait(bar, parity, code));
-      };
-      auto take_all = [&](uint32_t n) {
-        if (FWD) return walk.next(t);
-        const uint32_t s = n % kFeed;
-        if (!wait_all(&ctl->feed_full[s], (n / kFeed) & 1, 64)) return false;
-        t = ctl->feed[s];
-        __syncwarp();
-        if (lane == 0) arrive_cluster(feed_empty0 + 8u * s);
-        return t.kind >= 0;
-      };
       const uint32_t smem0 = smem_u32(smem);
-      for (uint32_t n = 0; ok && take_all(n); ++n) {
+      for (uint32_t n = 0; ok && (FWD ? walk.next(t) : take(n, t)); ++n) {
         const bool a_mn = t.kind == kDw, b_mn = t.kind >= kDx;
         const uint32_t idesc = (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) |
                                (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
