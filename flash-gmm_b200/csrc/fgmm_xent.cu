@@ -634,18 +634,23 @@ cudaError_t encode_fn(EncodeTiled* out) {
   return cudaSuccess;
 }
 
-// 64 x 64 boxes of a row-major (rows, cols) matrix of 16-bit words, 128-byte
+// Boxes of 128 bytes x box_rows of a row-major (rows, cols) matrix, 128-byte
 // swizzle; elements outside read as zero.
-cudaError_t make_map(EncodeTiled encode, CUtensorMap* m, const void* base, int64_t rows,
-                     int64_t cols, int64_t ld, bool bf16) {
+cudaError_t make_map(EncodeTiled encode, CUtensorMap* m, CUtensorMapDataType type, const void* base,
+                     int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  const int size = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)std::max<int64_t>(rows, 1)};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, 64}, es[2] = {1, 1};
-  const CUresult r = encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                            2, const_cast<void*>(base), dims, strides, box, es,
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, es[2] = {1, 1};
+  const CUresult r = encode(m, type, 2, const_cast<void*>(base), dims, strides, box, es,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+template <class T>
+constexpr CUtensorMapDataType word_type() {
+  return std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
 
 // Operand word of each element type, and what dW is stored as.
@@ -655,17 +660,35 @@ template <> struct Word<float> { using type = __half; };
 template <class T>
 cudaError_t make_operand_maps(const XentArgs& a, const XentWs& w, bool direct, MmaMaps* maps) {
   constexpr bool kSplit = sizeof(T) == 4;
-  constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value;
+  constexpr CUtensorMapDataType type = word_type<T>();
   EncodeTiled enc;
   cudaError_t e = encode_fn(&enc);
   if (e != cudaSuccess) return e;
-  e = direct ? make_map(enc, &maps->X, a.X, a.N, a.D, a.sxn, kBf)
-                         : make_map(enc, &maps->X, w.Xp, w.Np, a.D, w.Dp, kBf);
+  e = direct ? make_map(enc, &maps->X, type, a.X, a.N, a.D, a.sxn, 64)
+             : make_map(enc, &maps->X, type, w.Xp, w.Np, a.D, w.Dp, 64);
   if (e == cudaSuccess)
-    e = w.pack_w ? make_map(enc, &maps->W, w.Wp, a.V, a.D, w.Dp, kBf)
-                 : make_map(enc, &maps->W, a.W, a.V, a.D, a.swv, kBf);
-  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->X2, w.Xp2, w.Np, a.D, w.Dp, kBf);
-  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->W2, w.Wp2, a.V, a.D, w.Dp, kBf);
+    e = w.pack_w ? make_map(enc, &maps->W, type, w.Wp, a.V, a.D, w.Dp, 64)
+                 : make_map(enc, &maps->W, type, a.W, a.V, a.D, a.swv, 64);
+  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->X2, type, w.Xp2, w.Np, a.D, w.Dp, 64);
+  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->W2, type, w.Wp2, a.V, a.D, w.Dp, 64);
+  return e;
+}
+
+// Maps of G, loaded and stored, and of the fp32 slots.
+template <class T>
+cudaError_t make_backward_maps(const XentWs& w, MmaMaps* maps) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  constexpr CUtensorMapDataType type = word_type<T>(), f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const int64_t rows = (int64_t)kRing * w.row_chunk;
+  EncodeTiled enc;
+  cudaError_t e = encode_fn(&enc);
+  if (e == cudaSuccess) e = make_map(enc, &maps->G, type, w.G, rows, w.piece, w.piece, 64);
+  if (e == cudaSuccess) e = make_map(enc, &maps->Gs, type, w.G, rows, w.piece, w.piece, 32);
+  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->G2, type, w.G2, rows, w.piece, w.piece, 64);
+  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->G2s, type, w.G2, rows, w.piece, w.piece, 32);
+  if (e == cudaSuccess) e = make_map(enc, &maps->dxs, f32, w.dx_slots, w.ks_x * w.Np, w.ldS, w.ldS, 32);
+  if (e == cudaSuccess)
+    e = make_map(enc, &maps->dws, f32, w.dw_slots, (int64_t)w.ks_w * w.piece, w.ldS, w.ldS, 32);
   return e;
 }
 
@@ -761,17 +784,11 @@ cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
 
 template <class T>
 cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
-  constexpr bool kSplit = sizeof(T) == 4;
   MmaMaps maps{};
   cudaError_t e = make_operand_maps<T>(a, w, false, &maps);
+  if (e == cudaSuccess) e = make_backward_maps<T>(w, &maps);
   bool dependent;
   if (e == cudaSuccess) e = prepare<T>(a, w, false, true, &dependent);
-  EncodeTiled enc;
-  if (e == cudaSuccess) e = encode_fn(&enc);
-  const int64_t ring_rows = (int64_t)kRing * w.row_chunk;
-  if (e == cudaSuccess)
-    e = make_map(enc, &maps.G, w.G, ring_rows, w.piece, w.piece, std::is_same<T, __nv_bfloat16>::value);
-  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps.G2, w.G2, ring_rows, w.piece, w.piece, false);
   if (e != cudaSuccess) return e;
   MmaParams p = common_params(a, w);
   p.bn_d = w.bn_d;
@@ -789,7 +806,6 @@ cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
   p.dbias_part = a.dbias ? w.dbias_part : nullptr;
   p.ks_x = w.ks_x;
   p.ks_w = w.ks_w;
-  p.dx_slots = w.dx_slots;
   p.dw_slots = w.dw_slots;
   p.ldS = w.ldS;
   p.dW = a.dW;

@@ -72,15 +72,16 @@ struct MmaParams {
   float* dbias_part;       // [2 Np / 256][Vp], or null
   int64_t Vp;
   int ks_x, ks_w;          // splits of K
-  float* dx_slots;         // [ks_x][Np][ldS]
-  float* dw_slots;         // [ks_w][piece][ldS]
+  const float* dw_slots;   // [ks_w][piece][ldS]
   int64_t ldS;
   void* dW;
   int dw_vec;              // dW's rows take stores of four elements
 };
 
 struct MmaMaps {
-  CUtensorMap X, W, G, X2, W2, G2;
+  CUtensorMap X, W, G, X2, W2, G2;    // 64 x 64 boxes of words, loaded
+  CUtensorMap Gs, G2s;                // 64 x 32 boxes of words, stored
+  CUtensorMap dxs, dws;               // 32 x 32 boxes of fp32, stored or added
 };
 
 // Scales of the stored words.  G is stored over the largest row weight: with equal
@@ -141,6 +142,29 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
       "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
+}
+// An epilogue warp's staged 32 rows x 128 bytes, stored to (x, y) or added to it in the
+// L2; one bulk group of the issuing thread.
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\t"
+      "cp.async.bulk.commit_group;" ::"l"(map),
+      "r"(x), "r"(y), "r"(src)
+      : "memory");
+}
+__device__ __forceinline__ void tma_add(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];\n\t"
+      "cp.async.bulk.commit_group;" ::"l"(map),
+      "r"(x), "r"(y), "r"(src)
+      : "memory");
+}
+// All groups of this thread: their shared memory has been read / their writes are done.
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_done() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 __device__ __forceinline__ void mma_pair(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
                                          uint32_t accumulate) {
@@ -669,8 +693,8 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       }
     } else if (!FWD && warp == 2 && lane == 0) {
       // ------------------------------------------------------------ marks
-      // The fence that makes a unit's stores visible to other SMs waits for them to land:
-      // here, not in the epilogue.  The feed's place is kept until then, which bounds how
+      // The fence that makes a unit's stores visible to other SMs takes its time here, not
+      // in the epilogue.  The feed's place is kept until the unit is done, which bounds how
       // far the epilogue can run ahead of its marks.
       for (uint32_t n = 0;; ++n) {
         const uint32_t s = n % kFeed, parity = (n / kFeed) & 1;
@@ -729,10 +753,27 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       __syncwarp();
       if (lane == 0) arrive_cluster(empty0 + 8u * (a & 1));
     };
-    auto unit_done = [&](uint32_t n) {
+    // A unit is reported when its bulk stores are done: not at once, but in the middle of
+    // the next unit or before anything is waited for.
+    int to_report = -1;
+    auto report = [&] {
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->unit_done[n % kFeed]);
+      if (to_report >= 0 && lane == 0) {
+        bulk_wait_done();
+        mbar_arrive(&ctl->unit_done[to_report]);
+      }
+      to_report = -1;
     };
+    // The warp's stage is free to be written / holds data for the bulk store to come.
+    auto stage_free = [&] {
+      if (lane == 0) bulk_wait_read();
+      __syncwarp();
+    };
+    auto stage_full = [&] {
+      fence_async_smem();
+      __syncwarp();
+    };
+    const uint32_t stage_at = smem_u32(stage);
     auto wg_sync = [&] {   // the warpgroup's 128 threads
       asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
     };
@@ -744,6 +785,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     auto next = [&](uint32_t n) {
       if (FWD) return walk.next(t);
       const uint32_t s = n % kFeed, parity = (n / kFeed) & 1;
+      if (!__all_sync(0xffffffffu, mbar_try(smem_u32(&ctl->feed_full[s]), parity))) report();
       bool there = true;
       if (lane == 0) there = wait(&ctl->feed_full[s], parity, 64);
       if (!__all_sync(0xffffffffu, there)) return false;
@@ -774,6 +816,9 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       // back before they are worked on.
       float acc[kChunks][32];
       for (int k0 = 0; ok && k0 < t.nkb; k0 += group, ++ac) {
+        if (!FWD && to_report >= 0 &&
+            !__all_sync(0xffffffffu, mbar_try(smem_u32(&ctl->acc_full[ac & 1]), (ac >> 1) & 1)))
+          report();
         if (!__all_sync(0xffffffffu, wait(&ctl->acc_full[ac & 1], (ac >> 1) & 1, 32))) ok = false;
         tc_fence_after();
         const uint32_t at = lanes + (uint32_t)kBN * (ac & 1) + col0;
@@ -797,6 +842,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       }
       if (!ok) break;
       if (!FWD) {
+        report();
         // the ring's buffer is free; the slots' tile holds the sums so far
         ok = t.kind == kGrad ? wait_warp(prod_marks + t.j - kRing, t.w0)
                              : wait_warp(cell_marks + t.cell, t.w1);
@@ -923,47 +969,35 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
             for (int i = 0; i < 32; ++i)
               if (empty || v0 + 32 * c + i >= p.V) acc[c][i] = 0.f;
         }
-        // 128-byte staged rows: 64 columns of 16-bit words, or 32 of hi and lo words
-        const int64_t grow0 = t.x0 + row_in - lane;
-        const int64_t gcol0 = t.x1 + col0;
+        // 64 columns of words at a time are a warp's stage (SPLIT: their hi words, then
+        // their lo words)
+        const int gx = t.x1 + col0, gy = t.x0 + 128 * (int)rank + 32 * q;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < kChunks; c += 2) {
 #pragma unroll
           for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
-            uint32_t w[16];
+            stage_free();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float a = acc[c][2 * i], bb = acc[c][2 * i + 1];
-              uint32_t hi = pack2<T>(a, bb);
-              if (SPLIT && h) hi = pack_f16(a - f16lo_f(hi), bb - f16hi_f(hi));
-              w[i] = hi;
+            for (int g = 0; g < 8; ++g) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int e = 8 * g + 2 * i;
+                const float a = acc[c + e / 32][e % 32], bb = acc[c + e / 32][e % 32 + 1];
+                w[i] = pack2<T>(a, bb);
+                if (SPLIT && h) w[i] = pack_f16(a - f16lo_f(w[i]), bb - f16hi_f(w[i]));
+              }
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((g ^ (lane & 7)) << 4)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
             }
-            const int g0 = SPLIT ? h * 4 : (c & 1) * 4;       // first 16-byte granule
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<uint4*>(stage + lane * 128 + (((g0 + i) ^ (lane & 7)) << 4)) =
-                  make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-          }
-          if (SPLIT || (c & 1)) {
-            __syncwarp();
-            const int64_t gcol = gcol0 + 32 * (SPLIT ? c : c - 1);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 4 * i + (lane >> 3), g = lane & 7;
-              const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
-              uint16_t* dst;
-              if (SPLIT)
-                dst = static_cast<uint16_t*>(g < 4 ? p.G : p.G2) + (grow0 + r) * p.piece + gcol + 8 * (g & 3);
-              else
-                dst = static_cast<uint16_t*>(p.G) + (grow0 + r) * p.piece + gcol + 8 * g;
-              *reinterpret_cast<uint4*>(dst) = x;
-            }
-            __syncwarp();
+            stage_full();
+            if (lane == 0) tma_store(h ? &maps.G2s : &maps.Gs, gx + 32 * c, gy, stage_at);
           }
         }
         if (p.dbias_part) {
           // column sums of the unrounded g; the four quadrants' meet in the warpgroup's
-          // (now free) stages
+          // stages
+          stage_free();
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
             reinterpret_cast<float*>(stage)[32 * c + lane] = column_sums(acc[c], lane);
@@ -974,45 +1008,51 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + col0 + e] = s;
           wg_sync();
         }
-        unit_done(n);
+        to_report = (int)(n % kFeed);
         continue;
       }
 
       // kDx, kDw: into fp32 slots, or (the last sum of a dW tile) dW in its type
       const bool dw = t.kind == kDw, add = t.flags & 1, direct = t.flags & 2;
-      const int64_t row0 = t.x0 + 128 * (int)rank + 32 * q;
-      float* slots = dw ? p.dw_slots + (int64_t)t.ks * p.piece * p.ldS
-                        : p.dx_slots + (int64_t)t.ks * p.Np * p.ldS;
+      const int row0 = t.x0 + 128 * (int)rank + 32 * q;
+      const int slot_row = dw ? t.ks * p.piece + row0 : t.ks * (int)p.Np + row0;
       const float so = scales.dw;
-      const int64_t rows_left = (int64_t)p.V - t.x1 - row0;   // kDw: rows of dW from row0
+      const int rows_left = p.V - t.x1 - row0;                // kDw: rows of dW from row0
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         if (c >= chunks) break;
         const float (&v)[32] = acc[c];
         const int col = t.brow + col0 + 32 * c;
-        // 32 fp32 columns = a 128-byte staged row; then 8 lanes a row
+        // 32 fp32 columns = a 128-byte staged row
+        stage_free();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
               make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        if (!direct) {
+          stage_full();
+          if (lane == 0) {
+            if (add) tma_add(dw ? &maps.dws : &maps.dxs, col, slot_row, stage_at);
+            else tma_store(dw ? &maps.dws : &maps.dxs, col, slot_row, stage_at);
+          }
+          continue;
+        }
         __syncwarp();
-        const int g = lane & 7, at = col + 4 * g;
-        float4* slot0 = reinterpret_cast<float4*>(slots + (row0 + (lane >> 3)) * p.ldS + at);
+        const int g = lane & 7, at = col + 4 * g;             // 8 lanes a row
         float4 old[8];
         if (add) {   // all in flight at once; written by other SMs
+          const float4* slot = reinterpret_cast<const float4*>(
+              p.dw_slots + (int64_t)(slot_row + (lane >> 3)) * p.ldS + at);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) old[i] = __ldcg(slot0 + i * p.ldS);   // 4 rows of floats
+          for (int i = 0; i < 8; ++i) old[i] = __ldcg(slot + i * p.ldS);   // 4 rows of floats
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int r = 4 * i + (lane >> 3);
           float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
-          float4* slot = slot0 + i * p.ldS;
           if (add) { x.x += old[i].x; x.y += old[i].y; x.z += old[i].z; x.w += old[i].w; }
-          if (!direct) {
-            *slot = x;
-          } else if (r < rows_left) {
-            TO* dst = static_cast<TO*>(p.dW) + (t.x1 + row0 + r) * p.D + at;
+          if (r < rows_left) {
+            TO* dst = static_cast<TO*>(p.dW) + (int64_t)(t.x1 + row0 + r) * p.D + at;
             TO y[4] = {from_f32<TO>(x.x * so), from_f32<TO>(x.y * so), from_f32<TO>(x.z * so),
                        from_f32<TO>(x.w * so)};
             if (p.dw_vec) {
@@ -1029,8 +1069,10 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         }
         __syncwarp();
       }
-      unit_done(n);
+      to_report = (int)(n % kFeed);
     }
+    if (!FWD) report();
+    if (lane == 0) bulk_wait_done();
   }
   __syncwarp();
   tc_fence_before();
