@@ -217,29 +217,30 @@ __device__ __forceinline__ void idle_cycles(long long n) {
 }
 
 constexpr int kBN = 256;          // widest tile: the width of logits
+constexpr int kFeedMax = 4;       // places of the feed
 
 template <bool SPLIT>
 struct MmaCfg {
   static constexpr int kStages = SPLIT ? 3 : 6;
+  static constexpr int kFeed = SPLIT ? 3 : kFeedMax;         // tiles handed out ahead
   static constexpr int kA = 2 * kBoxBytes;                   // 128 rows x 64
   static constexpr int kB = (kBN / 2 / 64) * kBoxBytes;      // this SM's half of B
   static constexpr int kStage = (SPLIT ? 2 : 1) * (kA + kB);
   static constexpr int kStageOut = kEpiWarps * 4096;         // 32 rows x 128 B per warp
-  static constexpr int kCtl = 512;
+  static constexpr int kCtl = 768;
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStageOut + kCtl;
   static_assert(kSmem <= 232448, "shared memory budget");
 };
 
-constexpr int kFeed = 3;          // tiles handed out ahead of the slowest role
 
 struct MmaCtl {
-  Tile feed[kFeed];
+  Tile feed[kFeedMax];
   uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
-  uint64_t feed_full[kFeed], feed_empty[kFeed], unit_done[kFeed];
+  uint64_t feed_full[kFeedMax], feed_empty[kFeedMax], unit_done[kFeedMax];
   uint32_t tmem;
   volatile int abort_flag;
 };
-static_assert(sizeof(MmaCtl) <= 512, "control block");
+static_assert(sizeof(MmaCtl) <= 768, "control block");
 
 // The forward tiles of a pair in order: units of per_split vocabulary tiles of a row
 // tile, dealt in turn (rows fastest: pairs at work share the vocabulary's tiles).
@@ -513,7 +514,7 @@ template <bool FWD, bool SPLIT, class T, class TO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1)
 xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ MmaMaps maps) {
   using Cfg = MmaCfg<SPLIT>;
-  constexpr int NS = Cfg::kStages;
+  constexpr int NS = Cfg::kStages, kFeed = Cfg::kFeed;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -727,6 +728,10 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           send_tile(map_to_cta(smem_u32(&ctl->feed[s]), c),
                     map_to_cta(smem_u32(&ctl->feed_full[s]), c), t);
         if (t.kind < 0) break;
+        // products are long: no others are claimed until the unit before this one is done
+        if (!SPLIT && t.kind >= kDx && n > 0 &&
+            !wait(&ctl->feed_empty[(n - 1) % kFeed], ((n - 1) / kFeed) & 1, 256))
+          break;
       }
     }
   } else {
