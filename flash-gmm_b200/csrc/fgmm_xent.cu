@@ -77,7 +77,7 @@ constexpr int kBadTarget = -2;
 
 struct XentWs {
   Header* hdr;
-  int *rows, *inv, *target;
+  int *rows, *inv, *target, *counts;
   float* bias;
   void *Xp, *Xp2, *Wp, *Wp2;      // packed operands (SPLIT: hi and lo words)
   float2* part;
@@ -100,6 +100,7 @@ struct XentWs {
 
   static constexpr int kPairs = 74;                        // SM pairs the plan is made for
   static constexpr int64_t kPieceBytes = int64_t(1) << 25; // one buffer of G: kRing stay in the L2
+  static constexpr int kPiecesWanted = 4;   // of a short batch: products begin while g is made
   static constexpr int64_t kSlotBytes = int64_t(1) << 28;
 
   XentWs(void* p, bool backward, int type, int64_t N, int V, int D, const void* W, int64_t swv,
@@ -116,6 +117,7 @@ struct XentWs {
     rows = c.take<int>(Np);
     inv = c.take<int>(Np);
     target = c.take<int>(Np);
+    counts = c.take<int>((N + kRowsPerBlock - 1) / kRowsPerBlock);
     bias = c.take<float>(want_bias ? Vp : 0);
     Xp = c.take<uint16_t>((size_t)Np * Dp);
     Xp2 = c.take<uint16_t>(split ? (size_t)Np * Dp : 0);
@@ -138,8 +140,8 @@ struct XentWs {
       loss_part = c.take<double>(2 * ((N + 31) / 32));
     } else {
       const int word = split ? 4 : 2;
-      // column tiles of dX and dW: 128 wide where that pads D less
-      bn_d = (D + 127) / 128 * 128 < (D + 255) / 256 * 256 ? 128 : 256;
+      // column tiles of dX and dW: a 128-wide block takes about 0.7 of a 256-wide one's time
+      bn_d = D <= 128 ? 128 : 256;
       tiles_d = (D + bn_d - 1) / bn_d;
       ldS = (int64_t)tiles_d * bn_d;
       // Pieces of G: wide ones, so that dX's slots are added to rarely, and all rows of a
@@ -149,7 +151,8 @@ struct XentWs {
           256, std::min<int64_t>(Np, kPieceBytes / ((int64_t)piece * word) / 256 * 256));
       if (row_chunk == Np)
         piece = (int)std::max<int64_t>(
-            piece, std::min<int64_t>(Vp, kPieceBytes / ((int64_t)row_chunk * word) / 256 * 256));
+            piece, std::min<int64_t>((Vp / kPiecesWanted + 255) / 256 * 256,
+                                     kPieceBytes / ((int64_t)row_chunk * word) / 256 * 256));
       n_chunks = (int)((Np + row_chunk - 1) / row_chunk);
       n_pieces = (int)((Vp + piece - 1) / piece);
       // Splits of K: products of at most kUnit blocks, shorter where a product's tiles
@@ -177,12 +180,34 @@ struct XentWs {
   }
 };
 
-// Lists the live rows in their order, with their targets; block b counts the
-// live rows before its own 4096 by reading all earlier labels (from L2), so
-// one launch does it without a second pass.  Ignored rows get loss = logZ = 0.
-// The last block pads the list to a multiple of kPairRows with -1.
-__global__ void __launch_bounds__(1024) rows_kernel(const XentArgs a, const XentWs w) {
+// Live rows among each 4096 labels, for long batches (rows_kernel).
+__global__ void __launch_bounds__(1024) count_kernel(const XentArgs a, const XentWs w) {
   pdl_trigger();
+  __shared__ int wsum[32];
+  const int64_t base = (int64_t)blockIdx.x * kRowsPerBlock;
+  int n = 0;
+#pragma unroll
+  for (int r = 0; r < kRowsPerBlock; r += 1024) {
+    const int64_t i = base + r + threadIdx.x;
+    n += i < a.N && a.targets[i] != a.ignore;
+  }
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) wsum[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    n = __reduce_add_sync(0xffffffffu, wsum[threadIdx.x]);
+    if (threadIdx.x == 0) w.counts[blockIdx.x] = n;
+  }
+}
+
+// Lists the live rows in their order, with their targets.  Block b needs the live
+// rows before its own 4096: from count_kernel's sums where that ran (`counted`), else
+// it reads all earlier labels.  Ignored rows get loss = logZ = 0.
+// The last block pads the list to a multiple of kPairRows with -1.
+__global__ void __launch_bounds__(1024)
+rows_kernel(const XentArgs a, const XentWs w, int counted) {
+  pdl_trigger();
+  pdl_wait();
   __shared__ int wsum[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t base = (int64_t)blockIdx.x * kRowsPerBlock;
@@ -191,8 +216,12 @@ __global__ void __launch_bounds__(1024) rows_kernel(const XentArgs a, const Xent
     for (int64_t i = blockIdx.x * 1024 + threadIdx.x; i < w.sync_words; i += gridDim.x * 1024)
       w.sync[i] = 0;
   int before = 0;
+  if (counted) {
+    for (int k = threadIdx.x; k < (int)blockIdx.x; k += 1024) before += w.counts[k];
+  } else {
 #pragma unroll 8
-  for (int64_t i = threadIdx.x; i < base; i += 1024) before += a.targets[i] != a.ignore;
+    for (int64_t i = threadIdx.x; i < base; i += 1024) before += a.targets[i] != a.ignore;
+  }
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) wsum[warp] = before;
   __syncthreads();
@@ -401,40 +430,45 @@ __device__ __forceinline__ bool any_error(const Header* hdr) {
   return __syncthreads_or(e) != 0;
 }
 
-// Joins a live row's parts (max, sum) into logZ and loss.  A block takes 32
-// rows (lane = row), its 32 warps the parts in turn; the last block to finish
-// adds the blocks' sums in order.  `direct`: row i of X is live row i, ignored
-// rows among them.
+// Joins a live row's parts (max, sum) into logZ and loss.  With many parts a block
+// takes 32 rows (lane = row) and its 32 warps the parts in turn; with few (`few`)
+// every thread takes a row.  The last block to finish adds the blocks' sums in order.
+// `direct`: row i of X is live row i, ignored rows among them.
 __global__ void __launch_bounds__(1024)
-finish_forward_kernel(const XentArgs a, const XentWs w, int direct) {
+finish_forward_kernel(const XentArgs a, const XentWs w, int direct, int few) {
   pdl_trigger();
   pdl_wait();
   __shared__ float sm[32][33], ss[32][33];
+  __shared__ double block_sum[32];
+  __shared__ int block_count[32];
   __shared__ int last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t i = blockIdx.x * 32ll + lane;
+  const int64_t i = few ? blockIdx.x * 1024ll + threadIdx.x : blockIdx.x * 32ll + lane;
   const int64_t live = direct ? a.N : w.hdr->live;
   const bool bad = any_error(w.hdr);
   const bool on = i < live;
   float m = -3.402823466e38f, s = 0.f;
   if (on)
 #pragma unroll 4
-    for (int k = warp; k < 2 * w.splits; k += 32) {
+    for (int k = few ? 0 : warp; k < 2 * w.splits; k += few ? 1 : 32) {
       const float2 p = __ldg(&w.part[(int64_t)k * w.Np + i]);
       const float mn = fmaxf(m, p.x);
       s = s * ex2((m - mn) * kLog2Ef) + p.y * ex2((p.x - mn) * kLog2Ef);
       m = mn;
     }
-  sm[warp][lane] = m;
-  ss[warp][lane] = s;
-  __syncthreads();
-  if (warp == 0) {
-    float top = sm[0][lane];
+  if (!few) {
+    sm[warp][lane] = m;
+    ss[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0) {
 #pragma unroll
-    for (int k = 1; k < 32; ++k) top = fmaxf(top, sm[k][lane]);
-    float sum = 0.f;
+      for (int k = 1; k < 32; ++k) m = fmaxf(m, sm[k][lane]);
+      s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) sum += ss[k][lane] * ex2((sm[k][lane] - top) * kLog2Ef);
+      for (int k = 0; k < 32; ++k) s += ss[k][lane] * ex2((sm[k][lane] - m) * kLog2Ef);
+    }
+  }
+  if (few || warp == 0) {
     double mine = 0.0;
     bool counted = false;
     if (on) {
@@ -443,25 +477,28 @@ finish_forward_kernel(const XentArgs a, const XentWs w, int direct) {
       float lz = 0.f, loss = 0.f;
       if (counted) {
         const float nan = __int_as_float(0x7fffffff);
-        lz = bad ? nan : top + logf(sum);
+        lz = bad ? nan : m + logf(s);
         loss = t < 0 || t >= a.V ? nan : lz - w.tlogit[i];
         mine = loss;
       }
       a.logZ[r] = lz;
       a.loss[r] = loss;
     }
-    if (a.reduction != FGMM_REDUCE_NONE) {
-      for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-      const int n = __popc(__ballot_sync(0xffffffffu, counted));
-      if (lane == 0) {
-        w.loss_part[2 * blockIdx.x] = mine;
-        w.loss_part[2 * blockIdx.x + 1] = n;
-        __threadfence();
-        last = atomicAdd(&w.hdr->done, 1) == (int)gridDim.x - 1;
-      }
-    }
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    const int n = __popc(__ballot_sync(0xffffffffu, counted));
+    if (lane == 0) { block_sum[warp] = mine; block_count[warp] = n; }
   }
   if (a.reduction == FGMM_REDUCE_NONE) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double total = 0.0;
+    int n = 0;
+    for (int k = 0; k < (few ? 32 : 1); ++k) { total += block_sum[k]; n += block_count[k]; }
+    w.loss_part[2 * blockIdx.x] = total;
+    w.loss_part[2 * blockIdx.x + 1] = n;
+    __threadfence();
+    last = atomicAdd(&w.hdr->done, 1) == (int)gridDim.x - 1;
+  }
   __syncthreads();
   if (!last || warp != 0) return;
   __threadfence();
@@ -480,7 +517,7 @@ finish_forward_kernel(const XentArgs a, const XentWs w, int direct) {
   }
 }
 
-// out[r, :] = scale * sum of the slots' rows, in slot order; rows of dX without
+// out[r, :] = scale * sum of the ks slots' rows, in slot order; rows of dX without
 // a live row (inv < 0) are zero.
 template <class T>
 __device__ __forceinline__ void store_slots(const Share sh, const float* __restrict__ slots, int ks,
@@ -704,7 +741,10 @@ cudaError_t prepare(const XentArgs& a, const XentWs& w, bool direct, bool backwa
            a.D % whole == 0;
   };
   if (!direct) {
-    e = launch(rows_kernel, (a.N + kRowsPerBlock - 1) / kRowsPerBlock, 1024, 0, a.stream, false, a, w);
+    const int64_t blocks = (a.N + kRowsPerBlock - 1) / kRowsPerBlock;
+    const bool counted = blocks > 4;
+    if (counted) e = launch(count_kernel, blocks, 1024, 0, a.stream, false, a, w);
+    if (e == cudaSuccess) e = launch(rows_kernel, blocks, 1024, 0, a.stream, counted, a, w, (int)counted);
     *dependent = true;
   }
   if constexpr (kSplit) {
@@ -779,7 +819,9 @@ cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
   p.targets = a.targets;
   e = launch_mma<true, T>(a, p, maps, w.Np / kPairRows * w.splits, dependent);
   if (e != cudaSuccess) return e;
-  return launch(finish_forward_kernel, (a.N + 31) / 32, 1024, 0, a.stream, true, a, w, (int)direct);
+  const bool few = w.splits <= 8 && a.N > 32;   // up to 16 parts a row
+  return launch(finish_forward_kernel, few ? (a.N + 1023) / 1024 : (a.N + 31) / 32, 1024, 0, a.stream,
+                true, a, w, (int)direct, (int)few);
 }
 
 template <class T>

@@ -1023,6 +1023,17 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       const int slot_row = dw ? t.ks * p.piece + row0 : t.ks * (int)p.Np + row0;
       const float so = scales.dw;
       const int rows_left = p.V - t.x1 - row0;                // kDw: rows of dW from row0
+      const int g = lane & 7;                                 // direct: 8 lanes a row
+      // the sums so far of a chunk's rows r = 4 i + lane / 8, written by other SMs: all in
+      // flight at once, and the next chunk's while one is worked on
+      float4 old[2][8];
+      auto fetch = [&](int c, float4 (&o)[8]) {
+        const float4* slot = reinterpret_cast<const float4*>(
+            p.dw_slots + (int64_t)(slot_row + (lane >> 3)) * p.ldS + t.brow + col0 + 32 * c + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = __ldcg(slot + i * p.ldS);   // 4 rows of floats
+      };
+      if (direct && add) fetch(0, old[0]);
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         if (c >= chunks) break;
@@ -1043,32 +1054,36 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           continue;
         }
         __syncwarp();
-        const int g = lane & 7, at = col + 4 * g;             // 8 lanes a row
-        float4 old[8];
-        if (add) {   // all in flight at once; written by other SMs
-          const float4* slot = reinterpret_cast<const float4*>(
-              p.dw_slots + (int64_t)(slot_row + (lane >> 3)) * p.ldS + at);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) old[i] = __ldcg(slot + i * p.ldS);   // 4 rows of floats
-        }
+        if (add && c + 1 < chunks) fetch(c + 1, old[(c + 1) & 1]);
+        const int at = col + 4 * g;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int r = 4 * i + (lane >> 3);
           float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
-          if (add) { x.x += old[i].x; x.y += old[i].y; x.z += old[i].z; x.w += old[i].w; }
-          if (r < rows_left) {
+          if (add) {
+            const float4 o = old[c & 1][i];
+            x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w;
+          }
+          if (!p.dw_vec) {   // rows of dW start anywhere: stored below
+            *reinterpret_cast<float4*>(stage + r * 128 + ((g ^ (r & 7)) << 4)) = x;
+          } else if (r < rows_left && at < p.D) {
             TO* dst = static_cast<TO*>(p.dW) + (int64_t)(t.x1 + row0 + r) * p.D + at;
             TO y[4] = {from_f32<TO>(x.x * so), from_f32<TO>(x.y * so), from_f32<TO>(x.z * so),
                        from_f32<TO>(x.w * so)};
-            if (p.dw_vec) {
-              if (at < p.D) {
-                if (sizeof(TO) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(y);
-                else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (at + k < p.D) dst[k] = y[k];
+            if (sizeof(TO) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(y);
+            else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
+          }
+        }
+        if (!p.dw_vec) {     // lane = column
+          __syncwarp();
+          TO* dst = static_cast<TO*>(p.dW) + (int64_t)(t.x1 + row0) * p.D + col + lane;
+          if (col + lane < p.D) {
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r) {
+              if (r >= rows_left) break;
+              const float x = *reinterpret_cast<const float*>(
+                  stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3));
+              dst[(int64_t)r * p.D] = from_f32<TO>(x * so);
             }
           }
         }
