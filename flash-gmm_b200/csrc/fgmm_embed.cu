@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(kClusterSortThreads)
 cluster_sort_kernel(const int64_t* __restrict__ ids, int64_t ignore, int V, int N, int bits,
                     int digit_bits, uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
                     uint32_t* __restrict__ joins) {
+  pdl_trigger();
   if (blockIdx.x == 0 && threadIdx.x == 0) joins[0] = 0;
   extern __shared__ uint32_t sm[];
   constexpr int kMine = kClusterSortThreads * ITEMS;               // places of a block
@@ -258,7 +259,7 @@ sort_count_kernel(SortIn in, int64_t N, int shift, uint32_t mask, uint32_t* __re
 // Exclusive prefix sum of hist[0, n) by one block.
 __global__ void __launch_bounds__(1024)
 sort_scan_kernel(uint32_t* __restrict__ hist, int64_t n, uint32_t* __restrict__ joins) {
-  if (threadIdx.x == 0) joins[0] = 0;
+  if (threadIdx.x == 0) joins[0] = 0;   // (before the next kernel may start)
   __shared__ uint32_t warp_sum[32];
   uint32_t carry = 0;
   for (int64_t base = 0; base < n; base += 8192) {   // 8 consecutive values a thread
@@ -385,6 +386,8 @@ run_sum_kernel(const T* __restrict__ g, int64_t dsn, int64_t dsd, const uint32_t
                const uint32_t* __restrict__ pos, int64_t N, int V, int D, float scale,
                int accumulate, int col_blocks, int64_t sums, T* __restrict__ dtable,
                float* __restrict__ parts, uint32_t* __restrict__ joins) {
+  pdl_trigger();
+  pdl_wait();
   if (blockIdx.x >= sums) {
     clear_rows<T>(key, N, (blockIdx.x - sums) * (int64_t)kClearRows, V, D, VEC > 1, dtable);
     return;
@@ -445,6 +448,8 @@ __global__ void __launch_bounds__(512)
 join_runs_kernel(const uint32_t* __restrict__ key, int64_t N, int V, int D, float scale,
                  int accumulate, T* __restrict__ dtable, const float* __restrict__ parts,
                  const uint32_t* __restrict__ joins) {
+  pdl_trigger();
+  pdl_wait();
   __shared__ int64_t s_last;
   __shared__ float red[8][64][4];
   const int tiles = (D + 255) / 256;
@@ -454,17 +459,15 @@ join_runs_kernel(const uint32_t* __restrict__ key, int64_t N, int V, int D, floa
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int64_t j = u / tiles, b = joins[1 + j], end = (b + 1) * kRun;
     const uint32_t v = key[end];
-    if (threadIdx.x < 32) {   // first position with another id, 32 probes a round
-      int64_t lo = end, hi = N;
-      while (lo < hi) {
-        const int64_t step = (hi - lo + 31) / 32, at = lo + threadIdx.x * step;
-        const uint32_t same = __ballot_sync(0xffffffffu, at < hi && key[at] == v);
-        const int n = __popc(same);                     // probes of the id: a prefix of the lanes
-        if (n == 0) break;
-        hi = min(hi, lo + n * step);
-        lo += (n - 1) * step + 1;
+    if (threadIdx.x < 32) {   // the block in which the run ends: the last whose first key is v
+      int64_t last = b;
+      for (;;) {
+        const int64_t at = (last + 1 + threadIdx.x) * kRun;
+        const int n = __popc(__ballot_sync(0xffffffffu, at < N && key[at] == v));
+        last += n;                                      // a prefix of the lanes
+        if (n < 32) break;
       }
-      if (threadIdx.x == 0) s_last = (lo - 1) / kRun;
+      if (threadIdx.x == 0) s_last = last;
     }
     __syncthreads();
     const int64_t count = s_last - b + 1;
@@ -682,15 +685,13 @@ int fgmm_embed_bwd(int type, const void* dout, int64_t d_stride_n, int64_t d_str
         const int cols = 256 * (vec ? VEC : 1), col_blocks = (D + cols - 1) / cols;
         const int64_t sums = (int64_t)runs * col_blocks;
         const unsigned grid = (unsigned)(sums + (accumulate ? 0 : ((int64_t)V + kClearRows - 1) / kClearRows));
-        auto* kernel = vec ? run_sum_kernel<T, VEC> : run_sum_kernel<T, 1>;
-        kernel<<<grid, 256, 0, st>>>(g, d_stride_n, d_stride_d, ws.key[at], ws.pos[at], N, V, D,
-                                     scale, accumulate, col_blocks, sums, out, ws.parts, ws.joins);
-        count_launches(1);
-        if (runs > 1) {
+        e = launch(vec ? run_sum_kernel<T, VEC> : run_sum_kernel<T, 1>, grid, 256, 0, st, true, g,
+                   d_stride_n, d_stride_d, ws.key[at], ws.pos[at], N, V, D, scale, accumulate,
+                   col_blocks, sums, out, ws.parts, ws.joins);
+        if (runs > 1 && e == cudaSuccess) {
           const int64_t most = (int64_t)(runs - 1) * ((D + 255) / 256);
-          join_runs_kernel<T><<<(unsigned)std::min<int64_t>(most, 4 * num_sms()), 512, 0, st>>>(
-              ws.key[at], N, V, D, scale, accumulate, out, ws.parts, ws.joins);
-          count_launches(1);
+          e = launch(join_runs_kernel<T>, std::min<int64_t>(most, 4 * num_sms()), 512, 0, st, true,
+                     ws.key[at], N, V, D, scale, accumulate, out, ws.parts, ws.joins);
         }
       });
     }

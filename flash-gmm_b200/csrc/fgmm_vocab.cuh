@@ -51,6 +51,34 @@ decltype(auto) with_type(int type, F&& f) {
   return f(static_cast<float*>(nullptr));
 }
 
+// Programmatic dependent launch: let the next kernel of the stream be set up, and wait
+// for the end of the one before (no-ops in a launch without the attribute).
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Launches a kernel; `dependent`: it may be set up while the kernel before it (of this
+// call, on the same stream) still runs, and waits for its end itself (pdl_wait).
+template <class... P, class... A>
+cudaError_t launch(void (*kernel)(P...), int64_t grid, int threads, size_t smem,
+                   cudaStream_t stream, bool dependent, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  count_launches(1);
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // FGMM_OK, or the status of a refused type or shape with its message recorded.
 inline int vocab_check_shape(const char* name, int type, int64_t N, int32_t V, int32_t D) {
   char buf[200];

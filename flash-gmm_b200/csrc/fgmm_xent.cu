@@ -615,25 +615,6 @@ finish_backward_kernel(const XentArgs a, const XentWs w, const FinishShares sh) 
   if (b - sh.dw < sh.dbias) store_dbias(b - sh.dw, a, w);
 }
 
-// Launches a kernel; `dependent`: it may be set up while the kernel before it (of this
-// call, on the same stream) still runs, and waits for its end itself (pdl_wait).
-template <class... P, class... A>
-cudaError_t launch(void (*kernel)(P...), int64_t grid, int threads, size_t smem,
-                   cudaStream_t stream, bool dependent, A&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  count_launches(1);
-  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
-}
-
 // Blocks of 256 threads for that many threads' work: all resident at once at most.
 int blocks_for(int64_t threads) {
   return (int)std::min<int64_t>(std::max<int64_t>((threads + 255) / 256, 1), 8 * num_sms());

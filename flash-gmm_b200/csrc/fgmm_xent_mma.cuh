@@ -126,15 +126,6 @@ struct __align__(16) Tile {
   int pad;
 };
 
-// Programmatic dependent launch: let the next kernel of the stream be set up, and wait
-// for the end of the one before (no-ops in a launch without the attribute).
-__device__ __forceinline__ void pdl_trigger() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void pdl_wait() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
                                               uint32_t bar) {
   asm volatile(
