@@ -95,7 +95,7 @@ struct XentWs {
   int bn_d, tiles_d;
   int64_t ldS;
   int row_chunk, piece, n_chunks, n_pieces, ks_x, ks_w;
-  int64_t sync_words;
+  int64_t sync_words, units = 0;
   size_t bytes;
 
   static constexpr int kPairs = 74;                        // SM pairs the plan is made for
@@ -167,6 +167,9 @@ struct XentWs {
       ks_x = pick((int64_t)(row_chunk / 256) * tiles_d * steps, piece / 64, Np * ldS * 4);
       ks_w = n_pieces > 1 ? 1 : pick((int64_t)(piece / 256) * tiles_d * steps, row_chunk / 64,
                                      (int64_t)piece * ldS * 4);
+      // tiles of all kinds, which the product kernel counts in 32 bits
+      units = Np / 256 * (Vp / 256) + steps * tiles_d *
+              ((int64_t)(row_chunk / 256) * ks_x + (int64_t)(piece / 256) * ks_w);
       rg = c.take<RowGrad>(Np);
       sync_words = 1 + 2 * steps + (Np / kPairRows * ks_x + (int64_t)(piece / 256) * ks_w) * tiles_d;
       sync = c.take<uint32_t>(sync_words);
@@ -961,6 +964,8 @@ int fgmm_xent_bwd(int type, const void* X, int64_t x_stride_n, int64_t x_stride_
     if (rc == FGMM_OK) rc = vocab_check_array(name, "dW", dW, type_size(type), 0, 0);
     if (rc != FGMM_OK) return rc;
     const XentWs w(workspace, true, type, N, V, D, W, w_stride_v, w_stride_d, bias != nullptr);
+    if (w.units >= (int64_t(1) << 31) - (1 << 16))
+      return entry_fail(FGMM_ERR_UNSUPPORTED, std::string(name) + ": N * V exceeds what one call counts; split the rows");
     rc = check_device_and_workspace(a, w.bytes);
     if (rc != FGMM_OK) return rc;
     cudaError_t e = cudaSuccess;

@@ -215,7 +215,8 @@ FGMM_API int fgmm_generate_iso_rows(float* X, const int64_t* row_ids, int64_t ro
  *  - Workspaces are 256-byte aligned, as for the E-step; nothing in them has
  *    to be initialised and nothing is kept in them between calls.  Results
  *    are bitwise reproducible run to run.
- *  - Limits: N < 2^30, V < 2^30, D <= 2^16.
+ *  - Limits: N < 2^30, V < 2^30, D <= 2^16; the gradient of the loss also
+ *    about N * V < 2^46 (FGMM_ERR_UNSUPPORTED beyond).
  * ------------------------------------------------------------------------- */
 #define FGMM_T_F32 0
 #define FGMM_T_BF16 1

@@ -252,7 +252,7 @@ def test_xent_only_what_is_asked():
 
 
 def test_xent_same_bits_every_run():
-    X, W, t, c = R.problem(3000, 5000, 136, BF, ignored=0.1, bias=True)
+    X, W, t, c = R.problem(6000, 12300, 136, BF, ignored=0.1, bias=True)
     X.requires_grad_(), W.requires_grad_(), c.requires_grad_()
     runs = []
     for _ in range(3):
@@ -275,6 +275,63 @@ def test_xent_other_stream_and_two_at_once():
             b = F.linear_cross_entropy(X2, W2, t2, reduction="none")
         torch.cuda.synchronize()
         assert torch.equal(a, want) and torch.equal(b, want2)
+
+
+def test_backward_calls_on_two_streams_at_once():
+    """Each call's pairs of SMs wait for one another; two calls share the SMs."""
+    probs = [R.problem(2500, 9000, 128, BF, seed=k, bias=True) for k in (0, 1)]
+    args = []
+    for X, W, t, c in probs:
+        loss, logZ, _, count = L.xent_fwd(X, W, t, c, R.IGNORE, "mean")
+        args.append((X, W, t, c, R.IGNORE, logZ, torch.ones((), device=DEV), count, None,
+                     (True, True, True)))
+    want = [L.xent_bwd(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(L.xent_bwd(*args[k]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for out in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
+
+
+@pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
+def test_xent_mean_with_a_penalty_on_logz(dtype):
+    X, W, t, c = R.problem(400, 900, 56, dtype, ignored=0.2, bias=True, seed=4)
+    leaves = [x.clone().requires_grad_() for x in (X, W, c)]
+    loss, logZ = F.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], return_logZ=True)
+    (loss + 1e-3 * logZ.square().sum()).backward()
+    count = int((t != R.IGNORE).sum())
+    w = torch.full((400,), 1.0 / count, device=DEV)
+    z = R.xent(X, W, t, c)["logZ"] * 2e-3
+    ref = R.xent(X, W, t, c, w=w, dlogZ=z)
+    # the penalty's weight is made of the float32 logZ: 2^-17 + 2^-22 of it at most (e_logZ)
+    off = 2e-3 * ref["e_logZ"].max() / z.abs().max().clamp_min(1e-6) + 2 ** -20
+    for leaf, name in zip(leaves, ("dX", "dW", "dbias")):
+        slack = off * {"dX": (z + 1)[:, None] * W.double().abs().max(),
+                       "dW": (z.abs().sum() + 1) * X.double().abs().max(),
+                       "dbias": z.abs().sum() + 1}[name]
+        R.assert_within(leaf.grad, ref[name], ref["e_" + name] * (1 + 2 ** -18) + slack, name)
+
+
+@pytest.mark.parametrize("N", [255, 256, 257])
+def test_xent_rows_read_in_place_or_copied(N):
+    """Up to 256 16-bit rows are read in place, with their ignored rows among them."""
+    X, W, t, _ = R.problem(N, 5000, 96, BF, ignored=0.3, seed=N)
+    wide = torch.cat([X, X], 1)
+    X[t == R.IGNORE] = float("nan")
+    wide[t == R.IGNORE] = float("nan")
+    a = F.linear_cross_entropy(X, W, t, reduction="none")
+    b = F.linear_cross_entropy(wide[:, 96:], W, t, reduction="none")
+    c = F.linear_cross_entropy(wide[:, 96:].contiguous()[:, :], W, t, reduction="sum")
+    ref = R.xent(X.nan_to_num(0), W, t, None)
+    R.assert_within(a, ref["loss"], ref["e_loss"], "loss")
+    assert torch.equal(a, b)
+    assert abs(c.item() - ref["loss"].sum().item()) <= ref["e_loss"].sum().item() + 2 ** -20 * c.item()
 
 
 def test_xent_from_new_host_threads():

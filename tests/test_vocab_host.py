@@ -87,6 +87,7 @@ class C:
     ("fgmm_xent_bwd", C.BWD, dict(ds=2), 1, "dloss_stride"),
     ("fgmm_xent_bwd", C.BWD, dict(logZ=None), 1, "null pointer"),
     ("fgmm_xent_bwd", C.BWD, dict(dX=257), 1, "not aligned"),
+    ("fgmm_xent_bwd", C.BWD, dict(N=(1 << 30) - 1, V=(1 << 30) - 1), 3, "split the rows"),
     ("fgmm_embed_fwd", C.EFWD, dict(out=None), 1, "null pointer"),
     ("fgmm_embed_fwd", C.EFWD, dict(tsd=-1), 1, "negative stride"),
     ("fgmm_embed_bwd", C.EBWD, dict(dtable=None), 1, "null pointer"),
