@@ -266,26 +266,27 @@ struct ForwardWalk {
 
 // The backward tiles.  G runs through a ring of kRing pieces (row chunk x piece of the
 // vocabulary, the chunks of one piece of the vocabulary in a row) that stays in the L2:
-// step j makes piece j's g (kGrad) and multiplies piece j - kLag's (kDx, kDw), the two
+// step j makes piece j's g (kGrad) and multiplies piece j - lag's (kDx, kDw), the two
 // kinds mixed, since one is bound by its epilogue and the other by its products.  Pairs
 // claim units in this one order, and a unit waits only for units before it in the order,
 // so whichever pairs are resident make progress.  What a unit needs of others:
 //   kGrad j       the products of piece j - kRing (the ring's buffer is free)
 //   products i    all of piece i's g, and the unit before it on the same tile of the slots
 // Each is a count of marks, one per SM that has finished its half of a unit (mark role).
-constexpr int kRing = 4;
+constexpr int kRing = 5;
 constexpr int kLag = 2;
 constexpr uint32_t kMarks = 2;
 
 struct BackwardList {
   const MmaParams& p;
-  int live, chunks, pieces;              // row chunks that hold live rows, pieces in all
+  int live, chunks, pieces, lag;         // row chunks that hold live rows, pieces in all
   int step = 0, base = 0, n_grad = 0, n_prod = 0;
   struct Size { int rows, mt, v0, nv, vt; };
   __device__ explicit BackwardList(const MmaParams& p_) : p(p_) {
     live = *p.live;
     chunks = max(1, (live + p.row_chunk - 1) / p.row_chunk);
     pieces = chunks * p.n_pieces;
+    lag = pieces <= kRing ? pieces : kLag;   // few pieces: all of g first
     load();
   }
   __device__ Size size(int j) const {
@@ -311,7 +312,7 @@ struct BackwardList {
   uint64_t share = 0;
   __device__ void load() {
     n_grad = grads(step);
-    n_prod = products(step - kLag);
+    n_prod = products(step - lag);
     const int n = n_grad + n_prod;
     share = n > 0 ? ((uint64_t)n_prod << 32) / (uint64_t)n : 0;
   }
@@ -326,12 +327,12 @@ struct BackwardList {
   }
   // Unit u (never smaller than the one before); kind -1 behind the last.
   __device__ void get(int u, Tile& t) {
-    while (step < pieces + kLag && u >= base + n_grad + n_prod) {
+    while (step < pieces + lag && u >= base + n_grad + n_prod) {
       base += n_grad + n_prod;
       ++step;
       load();
     }
-    if (step >= pieces + kLag) { t.kind = -1; return; }
+    if (step >= pieces + lag) { t.kind = -1; return; }
     // products spread evenly among the step's units
     const int i = u - base;
     const int prod = upto(i);
@@ -350,7 +351,7 @@ struct BackwardList {
       t.w1 = 0;
       return;
     }
-    const int j = step - kLag;
+    const int j = step - lag;
     const Size s = size(j);
     const int rc = j % chunks, g0 = (j % kRing) * p.row_chunk;
     const int n_dx = p.has_dx ? s.mt * p.tiles_d * p.ks_x : 0;
