@@ -75,6 +75,28 @@ struct Header {
 constexpr int kRowsPerBlock = 4096;
 constexpr int kBadTarget = -2;
 
+// The launches of fgmm_xent_small.cuh.
+constexpr int kSmallRows = 16;             // rows at most
+constexpr int kSmallCols = 512;            // columns of a products block: 128 threads x 4
+struct SmallPlan {
+  int nb;            // rows the kernels are made for: 1, 8 or 16
+  int blocks;        // of small_logits_kernel; its parts
+  int splits;        // ranges of the vocabulary of the products
+  int per_split;     // entries of one
+};
+
+SmallPlan small_plan(int64_t N, int V, int D) {
+  SmallPlan p;
+  p.nb = N <= 1 ? 1 : N <= 8 ? 8 : 16;
+  const int rows = p.nb == 16 ? 2 : p.nb == 8 ? 4 : 8;       // of W, per warp
+  p.blocks = (int)std::min<int64_t>(((int64_t)V + 8 * rows - 1) / (8 * rows), 4 * 148);
+  const int64_t tiles = (D + kSmallCols - 1) / kSmallCols;
+  const int64_t want = std::max<int64_t>(1, (6 * 148 + tiles - 1) / tiles);
+  p.per_split = (int)std::max<int64_t>(64, (V + want - 1) / want);
+  p.splits = (V + p.per_split - 1) / p.per_split;
+  return p;
+}
+
 struct XentWs {
   Header* hdr;
   int *rows, *inv, *target, *counts;
@@ -87,10 +109,11 @@ struct XentWs {
   uint32_t* sync;
   void *G, *G2;
   float *dbias_part, *dx_slots, *dw_slots;
+  float *small_g, *small_dx;       // of a few rows: g [V][nb], parts of dX [splits][nb][D]
 
   int64_t Np, Vp;
   int Dp;                          // row length of the packed operands
-  bool split, pack_w;
+  bool split, pack_w, small;
   int vtiles, per_split, splits;
   int bn_d, tiles_d;
   int64_t ldS;
@@ -114,6 +137,23 @@ struct XentWs {
     pack_w = split || swd != 1 || swv < D || swv % 8 != 0 || swv >= (int64_t(1) << 38) ||
              (reinterpret_cast<uintptr_t>(W) & 15) != 0;
     hdr = c.take<Header>(1);
+    // fp32 rows of W that do not take 16-byte loads: 8 rows at most (12 of 100000 x 999: 390 us
+    // against 320 as words on the tensor cores)
+    const bool w16 = swd == 1 && swv % 4 == 0 && D % 4 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0;
+    small = split && N <= (w16 ? kSmallRows : 8);
+    if (small) {
+      const SmallPlan sp = small_plan(N, V, D);
+      if (!backward) {
+        part = c.take<float2>((size_t)sp.blocks * Np);
+        tlogit = c.take<float>(Np);
+        loss_part = c.take<double>(2);
+      } else {
+        small_g = c.take<float>((size_t)V * sp.nb);
+        small_dx = c.take<float>((size_t)sp.splits * sp.nb * D);
+      }
+      bytes = c.used;
+      return;
+    }
     rows = c.take<int>(Np);
     inv = c.take<int>(Np);
     target = c.take<int>(Np);
@@ -182,6 +222,8 @@ struct XentWs {
     bytes = c.used;
   }
 };
+
+#include "fgmm_xent_small.cuh"
 
 // Live rows among each 4096 labels, for long batches (rows_kernel).
 __global__ void __launch_bounds__(1024) count_kernel(const XentArgs a, const XentWs w) {
@@ -438,7 +480,7 @@ __device__ __forceinline__ bool any_error(const Header* hdr) {
 // every thread takes a row.  The last block to finish adds the blocks' sums in order.
 // `direct`: row i of X is live row i, ignored rows among them.
 __global__ void __launch_bounds__(1024)
-finish_forward_kernel(const XentArgs a, const XentWs w, int direct, int few) {
+finish_forward_kernel(const XentArgs a, const XentWs w, int parts, int direct, int few) {
   pdl_trigger();
   pdl_wait();
   __shared__ float sm[32][33], ss[32][33];
@@ -453,7 +495,7 @@ finish_forward_kernel(const XentArgs a, const XentWs w, int direct, int few) {
   float m = -3.402823466e38f, s = 0.f;
   if (on)
 #pragma unroll 4
-    for (int k = few ? 0 : warp; k < 2 * w.splits; k += few ? 1 : 32) {
+    for (int k = few ? 0 : warp; k < parts; k += few ? 1 : 32) {
       const float2 p = __ldg(&w.part[(int64_t)k * w.Np + i]);
       const float mn = fmaxf(m, p.x);
       s = s * ex2((m - mn) * kLog2Ef) + p.y * ex2((p.x - mn) * kLog2Ef);
@@ -781,8 +823,76 @@ cudaError_t launch_mma(const XentArgs& a, const MmaParams& p, const MmaMaps& map
   return launch(kernel, 2 * pairs, kMmaThreads, smem, a.stream, dependent, p, maps);
 }
 
+// How X, W (and `out`, contiguous rows) can be accessed.
+template <class T>
+int small_mode(const XentArgs& a, const void* out) {
+  auto four = [&](const void* p, int64_t s0) {
+    return s0 % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0;
+  };
+  if (a.sxd != 1 || a.swd != 1) return kAnyStride;
+  return a.D % 4 == 0 && four(a.X, a.sxn) && four(a.W, a.swv) && four(out, a.D) ? kVector : kUnitStride;
+}
+template <class F>
+cudaError_t with_mode(int mode, F&& f) {
+  if (mode == kVector) return f(std::integral_constant<int, kVector>{});
+  if (mode == kUnitStride) return f(std::integral_constant<int, kUnitStride>{});
+  return f(std::integral_constant<int, kAnyStride>{});
+}
+
+template <class T, bool GRAD>
+cudaError_t small_logits(const XentArgs& a, const XentWs& w, const SmallPlan& p) {
+  auto run = [&](auto nb, auto r, auto mode) {
+    return launch(small_logits_kernel<T, nb, r, mode, GRAD>, p.blocks, 32 * kSmallWarps, 0, a.stream, false,
+                  a, w, p);
+  };
+  return with_mode(small_mode<T>(a, nullptr), [&](auto mode) {
+    using std::integral_constant;
+    if (p.nb == 1) return run(integral_constant<int, 1>{}, integral_constant<int, 8>{}, mode);
+    if (p.nb == 8) return run(integral_constant<int, 8>{}, integral_constant<int, 4>{}, mode);
+    return run(integral_constant<int, 16>{}, integral_constant<int, 2>{}, mode);
+  });
+}
+
+template <class T>
+cudaError_t small_forward(const XentArgs& a, const XentWs& w) {
+  const SmallPlan p = small_plan(a.N, a.V, a.D);
+  cudaError_t e = small_logits<T, false>(a, w, p);
+  if (e != cudaSuccess) return e;
+  return launch(finish_forward_kernel, 1, 1024, 0, a.stream, true, a, w, p.blocks, 1, 0);
+}
+
+template <class T>
+cudaError_t small_backward(const XentArgs& a, const XentWs& w) {
+  const SmallPlan p = small_plan(a.N, a.V, a.D);
+  cudaError_t e = small_logits<T, true>(a, w, p);
+  if (e != cudaSuccess || (!a.dX && !a.dW)) return e;
+  auto run = [&](auto nb, auto mode) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.D + kSmallCols - 1) / kSmallCols), (unsigned)p.splits);
+    cfg.blockDim = dim3(128);
+    cfg.stream = a.stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    count_launches(1);
+    return cudaLaunchKernelEx(&cfg, small_products_kernel<T, nb, mode>, a, w, p);
+  };
+  e = with_mode(small_mode<T>(a, a.dW), [&](auto mode) {
+    using std::integral_constant;
+    if (p.nb == 1) return run(integral_constant<int, 1>{}, mode);
+    if (p.nb == 8) return run(integral_constant<int, 8>{}, mode);
+    return run(integral_constant<int, 16>{}, mode);
+  });
+  if (e != cudaSuccess || !a.dX) return e;
+  return launch(small_finish_kernel<T>, (a.N * a.D + 31) / 32, 256, 0, a.stream, true, a, w, p);
+}
+
 template <class T>
 cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
+  if constexpr (sizeof(T) == 4)
+    if (w.small) return small_forward<T>(a, w);
   MmaMaps maps{};
   // Up to one tile of rows that TMA can read is used in place: no list, no copy, and
   // the ignored rows among them cost nothing.
@@ -805,11 +915,13 @@ cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
   if (e != cudaSuccess) return e;
   const bool few = w.splits <= 8 && a.N > 32;   // up to 16 parts a row
   return launch(finish_forward_kernel, few ? (a.N + 1023) / 1024 : (a.N + 31) / 32, 1024, 0, a.stream,
-                true, a, w, (int)direct, (int)few);
+                true, a, w, 2 * w.splits, (int)direct, (int)few);
 }
 
 template <class T>
 cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
+  if constexpr (sizeof(T) == 4)
+    if (w.small) return small_backward<T>(a, w);
   MmaMaps maps{};
   cudaError_t e = make_operand_maps<T>(a, w, false, &maps);
   if (e == cudaSuccess) e = make_backward_maps<T>(w, &maps);

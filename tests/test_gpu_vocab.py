@@ -42,7 +42,8 @@ def check_xent(X, W, t, bias=None, *, reduction="none", wantgrad=True, seed=1, *
 
 
 # N, V, D: one row, odd sizes, edges of the 64/128/256 tiles and one past them
-SHAPES = [(1, 1, 1), (1, 1000, 64), (3, 7, 5), (37, 501, 103), (128, 256, 64), (129, 257, 65),
+SHAPES = [(1, 1, 1), (1, 1000, 64), (3, 7, 5), (8, 900, 516), (9, 333, 130), (16, 6001, 515),
+          (17, 600, 64), (37, 501, 103), (128, 256, 64), (129, 257, 65),
           (255, 300, 128), (257, 1024, 72), (300, 4099, 200), (513, 130, 1000), (700, 2049, 256)]
 
 
@@ -90,11 +91,12 @@ def test_xent_leading_dimensions_and_int32_targets():
     assert one.shape == () and abs((one - b[0]).item()) <= 1e-5 * max(1.0, float(b[0]))
 
 
+@pytest.mark.parametrize("N", [5, 13, 150])
 @pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("layout", ["transposed W", "transposed X", "odd row stride",
                                     "column step", "offset base", "expanded X"])
-def test_xent_strides(layout, dtype):
-    X, W, t, c = R.problem(150, 333, 48, dtype, bias=True, seed=3)
+def test_xent_strides(layout, dtype, N):
+    X, W, t, c = R.problem(N, 333, 48, dtype, bias=True, seed=3)
     if layout == "transposed W":
         W = W.t().contiguous().t()
     elif layout == "transposed X":
@@ -103,16 +105,16 @@ def test_xent_strides(layout, dtype):
         X = torch.cat([X, X[:, :3]], 1)[:, :48]
         W = torch.cat([W, W[:, :5]], 1)[:, :48]
     elif layout == "column step":
-        X = torch.stack([X, X * 0 + 9], 2).reshape(150, 96)[:, ::2]
+        X = torch.stack([X, X * 0 + 9], 2).reshape(N, 96)[:, ::2]
         W = torch.stack([W, W * 0 + 9], 2).reshape(333, 96)[:, ::2]
     elif layout == "offset base":
-        X = torch.cat([X.new_zeros(1), X.reshape(-1)])[1:].view(150, 48)
+        X = torch.cat([X.new_zeros(1), X.reshape(-1)])[1:].view(N, 48)
         W = torch.cat([W.new_zeros(1), W.reshape(-1)])[1:].view(333, 48)
     else:
-        X = X[:1].expand(150, 48)
+        X = X[:1].expand(N, 48)
     Xl, Wl, cl = X.detach().requires_grad_(), W.detach().requires_grad_(), c.requires_grad_()
     assert Xl.stride() == X.stride() and Wl.stride() == W.stride()
-    w = torch.rand(150, device=DEV) + 0.5
+    w = torch.rand(N, device=DEV) + 0.5
     loss = F.linear_cross_entropy(Xl, Wl, t, cl, reduction="none")
     got = torch.autograd.grad((loss * w).sum(), (Xl, Wl, cl))
     ref = R.xent(X, W, t, c, w=w)
@@ -122,7 +124,7 @@ def test_xent_strides(layout, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("N", [100, 300])
+@pytest.mark.parametrize("N", [7, 16, 100, 300])
 def test_xent_ignored_rows_may_hold_anything(N, dtype):
     X, W, t, c = R.problem(N, 400, 72, dtype, ignored=0.4, bias=True)
     dead = t == R.IGNORE
@@ -158,7 +160,7 @@ def test_xent_no_live_rows(N):
 
 
 @pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
-@pytest.mark.parametrize("N", [70, 400])
+@pytest.mark.parametrize("N", [6, 14, 70, 400])
 def test_xent_label_outside_the_table_is_nan(N, dtype):
     X, W, t, _ = R.problem(N, 300, 32, dtype)
     t[3], t[N - 1] = 300, -7
