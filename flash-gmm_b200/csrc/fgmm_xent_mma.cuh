@@ -10,10 +10,10 @@
 // 64 x 64 TMA boxes of 8 KB, 128-byte swizzled: read with K along the row (K-major)
 // or across rows (MN-major), so G and W serve two products each untransposed.
 //
-// A pair's MMA is M = 256 (128 rows per SM) x BN: each SM stages its 128 rows of A
+// A pair's MMA is M = 256 (128 rows per SM) x 256: each SM stages its 128 rows of A
 // and its half of B, so a 256 x 256 x 64 block costs each SM 32 KB of staged bytes
 // against 512 cycles of MMA; one SM alone would need 48 KB for half the product and
-// be bound by the L2.  Two BN-column accumulators in TMEM let eight epilogue warps
+// be bound by the L2.  Two 256-column accumulators in TMEM let eight epilogue warps
 // work on one tile while the next is multiplied.
 //
 // SPLIT (fp32 inputs): operands are pairs of fp16 words hi + lo of the values scaled
@@ -566,7 +566,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     regs_down<72>();
     // Loads and MMAs: the whole warp runs the loop, so that addresses, descriptors and
     // coordinates are warp-uniform values, and an elected lane issues.  From one lane's
-    // branch, a block of four MMAs took about 750 cycles to issue, whatever its width.
+    // branch, a K-block of four MMAs took 690 to 850 cycles against 512 at the full rate.
     auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
       return (bool)__all_sync(0xffffffffu, wait(bar, parity, code));
     };
@@ -1001,7 +1001,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           wg_sync();
           const int e = (int)threadIdx.x & 127;
           const float* cs = reinterpret_cast<const float*>(out_stage + wg * 16384) + e;
-          const float s = (cs[0] + cs[1024]) + (cs[2048] + cs[3072]);
+          const float s = (cs[0] + cs[1 * 1024]) + (cs[2 * 1024] + cs[3 * 1024]);
           p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + col0 + e] = s;
           wg_sync();
         }
