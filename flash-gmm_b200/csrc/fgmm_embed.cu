@@ -659,6 +659,12 @@ int fgmm_embed_bwd(int type, const void* dout, int64_t d_stride_n, int64_t d_str
     rc = vocab_check_array(name, "dout", dout, type_size(type), d_stride_n, d_stride_d);
     if (rc == FGMM_OK) rc = vocab_check_array(name, "dtable", dtable, type_size(type), 0, 0);
     if (rc == FGMM_OK) rc = vocab_check_array(name, "ids", ids, 8, 0, 0);
+    const int64_t out_bytes = (int64_t)V * D * type_size(type);
+    if (rc == FGMM_OK)
+      rc = vocab_check_overlap(name, "dout", dout, N, D, d_stride_n, d_stride_d, type_size(type),
+                               "dtable", dtable, out_bytes);
+    if (rc == FGMM_OK)
+      rc = vocab_check_overlap(name, "ids", ids, N, 1, 1, 1, 8, "dtable", dtable, out_bytes);
     if (rc != FGMM_OK) return rc;
     std::string why;
     rc = entry_check_device(&why);

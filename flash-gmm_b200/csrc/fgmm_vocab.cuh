@@ -109,6 +109,19 @@ inline int vocab_check_array(const char* name, const char* what, const void* p, 
   return FGMM_OK;
 }
 
+// Refuses an input (N rows of D elements at these strides) that shares bytes with an
+// output of out_bytes: blocks read the input while others write.
+inline int vocab_check_overlap(const char* name, const char* what, const void* p, int64_t N,
+                               int64_t D, int64_t s0, int64_t s1, int size, const char* out_name,
+                               const void* out, int64_t out_bytes) {
+  if (N == 0) return FGMM_OK;
+  const __int128 a = (__int128)reinterpret_cast<uintptr_t>(p);
+  const __int128 b = (__int128)reinterpret_cast<uintptr_t>(out);
+  const __int128 a_end = a + ((__int128)(N - 1) * s0 + (__int128)(D - 1) * s1 + 1) * size;
+  if (a >= b + out_bytes || b >= a_end) return FGMM_OK;
+  return entry_fail(FGMM_ERR_ARG, std::string(name) + ": " + out_name + " overlaps " + what);
+}
+
 inline int vocab_check_workspace(const char* name, const void* ws, size_t got, size_t need) {
   if (need > 0 && (ws == nullptr || got < need || (reinterpret_cast<uintptr_t>(ws) & 255))) {
     char buf[200];

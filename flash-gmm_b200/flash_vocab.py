@@ -181,7 +181,8 @@ def embedding_grad(dout: torch.Tensor, ids: torch.Tensor, V: int, *, scale: floa
     dout: (..., D); ids: (...).  ``out`` may supply the (V, D) result buffer
     (contiguous, of dout's type); with ``accumulate`` the sums are added to it,
     e.g. to the other gradient of a tied table, and its other rows are left as
-    they are.  Bitwise the same on every run.
+    they are.  ``out`` may not share memory with dout or ids (refused).
+    Bitwise the same on every run.
     """
     if ids.shape != dout.shape[:-1] or dout.dim() < 1:
         raise ValueError(f"ids must be {tuple(dout.shape[:-1])}, got {tuple(ids.shape)}")

@@ -251,7 +251,8 @@ FGMM_API int fgmm_xent_fwd(int type, const void* X, int64_t x_stride_n, int64_t 
  *   g_nv = (w_n + dlogZ_n) p_nv - w_n [v = target_n]
  *   dX = g W,   dW = g^T X,   dbias_v = sum_n g_nv
  * dloss or dlogZ may be NULL (zero), and each of dX, dW, dbias that is NULL
- * is not computed.  logZ is the forward call's. */
+ * is not computed.  logZ is the forward call's.  Outputs share no bytes with
+ * inputs or each other. */
 FGMM_API int fgmm_xent_bwd(int type, const void* X, int64_t x_stride_n, int64_t x_stride_d,
                   const void* W, int64_t w_stride_v, int64_t w_stride_d, const float* bias,
                   const int64_t* targets, int64_t ignore_index,
@@ -272,7 +273,8 @@ FGMM_API size_t fgmm_embed_workspace_bytes(int64_t N, int32_t V, int32_t D);
  * the sorted ids in an order that is the same on every run.  With
  * FGMM_FLAG_ACCUMULATE the sum is added to dtable (rows that no id names are
  * not touched); without it every row of dtable is written.  Ids equal to
- * ignore_index or outside [0, V) contribute nothing. */
+ * ignore_index or outside [0, V) contribute nothing.  dtable must not share
+ * bytes with dout or ids (refused). */
 FGMM_API int fgmm_embed_bwd(int type, const void* dout, int64_t d_stride_n, int64_t d_stride_d,
                    const int64_t* ids, int64_t ignore_index, int64_t N, int32_t V, int32_t D,
                    float scale, void* dtable, void* workspace, size_t workspace_bytes,

@@ -101,6 +101,20 @@ def test_c_entries_refuse_before_any_device_call(lib, entry, args, change, code,
     assert match in message and entry in message
 
 
+@pytest.mark.parametrize("change", [
+    dict(dout=4096, dtable=4096),                              # the gradient over its own input
+    dict(dout=1 << 20, dtable=(1 << 20) - 16),                 # its last row reaches into dout
+    dict(dtable=1 << 20, dout=(1 << 20) + 16, dsn=0),          # one row for all positions, inside
+    dict(dtable=1 << 20, ids=(1 << 20) + 8, dout=1 << 24),
+    dict(dtable=1 << 40, dout=1 << 20, dsn=1 << 38),           # rows far apart reach over it
+])
+def test_embed_bwd_refuses_overlapping_arrays(lib, change):
+    assert set(change) <= set(C.EBWD)
+    assert lib.fgmm_embed_bwd(*dict(C.EBWD, **change).values()) == 1
+    message = lib.fgmm_last_error().decode()
+    assert "overlaps" in message and "fgmm_embed_bwd" in message
+
+
 def test_workspace_sizes(lib):
     for back in (0, 1):
         for kind in (0, 1, 2):
