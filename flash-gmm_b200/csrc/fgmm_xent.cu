@@ -140,7 +140,9 @@ struct XentWs {
     // fp32 rows of W that do not take 16-byte loads: 8 rows at most (12 of 100000 x 999: 390 us
     // against 320 as words on the tensor cores)
     const bool w16 = swd == 1 && swv % 4 == 0 && D % 4 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0;
-    small = split && N <= (w16 ? kSmallRows : 8);
+    // One 16-bit row whose W would be copied for TMA: 131072 x 4095 bf16 674 -> 288 us, with
+    // gradients 3181 -> 1337, W transposed (100000 x 1000) 655 -> 253; four rows 676 -> 803.
+    small = split ? N <= (w16 ? kSmallRows : 8) : pack_w && N <= 1;
     if (small) {
       const SmallPlan sp = small_plan(N, V, D);
       if (!backward) {
@@ -847,9 +849,11 @@ cudaError_t small_logits(const XentArgs& a, const XentWs& w, const SmallPlan& p)
   };
   return with_mode(small_mode<T>(a, nullptr), [&](auto mode) {
     using std::integral_constant;
-    if (p.nb == 1) return run(integral_constant<int, 1>{}, integral_constant<int, 8>{}, mode);
-    if (p.nb == 8) return run(integral_constant<int, 8>{}, integral_constant<int, 4>{}, mode);
-    return run(integral_constant<int, 16>{}, integral_constant<int, 2>{}, mode);
+    if constexpr (sizeof(T) == 4) {   // 16-bit types come with one row
+      if (p.nb == 16) return run(integral_constant<int, 16>{}, integral_constant<int, 2>{}, mode);
+      if (p.nb == 8) return run(integral_constant<int, 8>{}, integral_constant<int, 4>{}, mode);
+    }
+    return run(integral_constant<int, 1>{}, integral_constant<int, 8>{}, mode);
   });
 }
 
@@ -881,9 +885,11 @@ cudaError_t small_backward(const XentArgs& a, const XentWs& w) {
   };
   e = with_mode(small_mode<T>(a, a.dW), [&](auto mode) {
     using std::integral_constant;
-    if (p.nb == 1) return run(integral_constant<int, 1>{}, mode);
-    if (p.nb == 8) return run(integral_constant<int, 8>{}, mode);
-    return run(integral_constant<int, 16>{}, mode);
+    if constexpr (sizeof(T) == 4) {
+      if (p.nb == 16) return run(integral_constant<int, 16>{}, mode);
+      if (p.nb == 8) return run(integral_constant<int, 8>{}, mode);
+    }
+    return run(integral_constant<int, 1>{}, mode);
   });
   if (e != cudaSuccess || !a.dX) return e;
   return launch(small_finish_kernel<T>, (a.N * a.D + 31) / 32, 256, 0, a.stream, true, a, w, p);
@@ -891,8 +897,7 @@ cudaError_t small_backward(const XentArgs& a, const XentWs& w) {
 
 template <class T>
 cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
-  if constexpr (sizeof(T) == 4)
-    if (w.small) return small_forward<T>(a, w);
+  if (w.small) return small_forward<T>(a, w);
   MmaMaps maps{};
   // Up to one tile of rows that TMA can read is used in place: no list, no copy, and
   // the ignored rows among them cost nothing.
@@ -920,8 +925,7 @@ cudaError_t xent_forward(const XentArgs& a, const XentWs& w) {
 
 template <class T>
 cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
-  if constexpr (sizeof(T) == 4)
-    if (w.small) return small_backward<T>(a, w);
+  if (w.small) return small_backward<T>(a, w);
   MmaMaps maps{};
   cudaError_t e = make_operand_maps<T>(a, w, false, &maps);
   if (e == cudaSuccess) e = make_backward_maps<T>(w, &maps);

@@ -1,9 +1,10 @@
 // The linear cross entropy of a few fp32 rows (included by fgmm_xent.cu): up to 16, as
 // when single tokens are scored.  Such a batch is bound by reading W; on the tensor cores
 // an fp32 W would first be read for its scale, and read and written as two words.  These
-// kernels read it in place, whatever its strides, and multiply in fp32.  (16-bit rows keep
-// the tensor-core tile: it reads W once, in place, at four rows of 131072 x 4096 in 243 us
-// where these kernels took 618, with fewer bytes in flight per thread.)
+// kernels read it in place, whatever its strides, and multiply in fp32.  So does one 16-bit
+// row whose W TMA cannot read.  (Other 16-bit rows keep the tensor-core tile: it reads W
+// once, in place, at four rows of 131072 x 4096 in 243 us where these kernels took 618, with
+// fewer bytes in flight per thread.)
 //
 //   small_logits_kernel   S = X W^T: a warp takes R rows of W at a time, its lanes along D,
 //                         and keeps R x NB sums; forward they are folded into running

@@ -124,6 +124,44 @@ def test_xent_strides(layout, dtype, N):
 
 
 @pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("V,D,layout", [
+    (1, 1, "rows"), (7, 3, "rows"), (9, 511, "rows"), (1003, 513, "rows"), (64, 129, "rows"),
+    (20001, 1025, "rows"), (333, 516, "rows"), (300, 200, "transposed"), (5001, 77, "transposed"),
+    (300, 64, "column step"), (401, 100, "offset base")])
+def test_xent_one_row(V, D, layout, dtype):
+    """One row, W in layouts that are read in place only by the plain loads."""
+    X, W, t, c = R.problem(1, V, D, dtype, bias=True, seed=V)
+    if layout == "transposed":
+        W = W.t().contiguous().t()
+    elif layout == "column step":
+        W = torch.stack([W, W * 0 + 9], 2).reshape(V, 2 * D)[:, ::2]
+    elif layout == "offset base":
+        W = torch.cat([W.new_zeros(1), W.reshape(-1)])[1:].view(V, D)
+    if V > 8:
+        c[(t + 1) % V] = float("-inf")
+    Xl, Wl, cl = X.requires_grad_(), W.detach().requires_grad_(), c.requires_grad_()
+    assert Wl.stride() == W.stride() and Wl.data_ptr() == W.data_ptr()
+    loss, logZ = F.linear_cross_entropy(Xl, Wl, t, cl, reduction="none", return_logZ=True)
+    ref = R.xent(X, W, t, c, w=torch.ones(1, device=DEV), dlogZ=torch.ones(1, device=DEV))
+    R.assert_within(loss.detach(), ref["loss"], ref["e_loss"], "loss")
+    R.assert_within(logZ.detach(), ref["logZ"], ref["e_logZ"], "logZ")
+    got = torch.autograd.grad(loss.sum() + logZ.sum(), (Xl, Wl, cl), retain_graph=True)
+    again = torch.autograd.grad(loss.sum() + logZ.sum(), (Xl, Wl, cl))
+    for x, y, name in zip(got, again, ("dX", "dW", "dbias")):
+        R.assert_within(x, ref[name], ref["e_" + name], name)
+        assert torch.equal(x, y)
+    # some gradients only; an ignored row; a label outside the table
+    loss = F.linear_cross_entropy(X.detach(), W.detach(), t, cl, reduction="sum")
+    ref = R.xent(X, W, t, c, w=torch.ones(1, device=DEV))
+    R.assert_within(torch.autograd.grad(loss, cl)[0], ref["dbias"], ref["e_dbias"], "dbias")
+    off = F.linear_cross_entropy(Xl, Wl, torch.full_like(t, R.IGNORE), cl, reduction="sum")
+    assert off.item() == 0.0 and not any(g.any() for g in torch.autograd.grad(off, (Xl, Wl, cl)))
+    bad = F.linear_cross_entropy(Xl, Wl, torch.full_like(t, V), cl, reduction="sum")
+    assert math.isnan(bad.item())
+    assert all(bool(torch.isnan(g).all()) for g in torch.autograd.grad(bad, (Xl, Wl)))
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("N", [7, 16, 100, 300])
 def test_xent_ignored_rows_may_hold_anything(N, dtype):
     X, W, t, c = R.problem(N, 400, 72, dtype, ignored=0.4, bias=True)

@@ -119,11 +119,14 @@ def test_workspace_sizes(lib):
     for back in (0, 1):
         for kind in (0, 1, 2):
             sizes = [lib.fgmm_xent_workspace_bytes(back, kind, n, 5000, 256, 1024, 256, 1, 0)
-                     for n in (0, 1, 1000)]
+                     for n in (0, 1, 2, 1000)]
             assert sizes == sorted(sizes) and sizes[1] > 0
             for at, s0, s1 in ((1026, 256, 1), (1024, 257, 1), (1024, 1, 5000), (1024, 0, 1)):
-                copied = lib.fgmm_xent_workspace_bytes(back, kind, 1, 5000, 256, at, s0, s1, 0)
-                assert (copied > sizes[1] + 2 * 5000 * 255) == (kind != 0)
+                one, two = (lib.fgmm_xent_workspace_bytes(back, kind, n, 5000, 256, at, s0, s1, 0)
+                            for n in (1, 2))
+                # one row reads W in place; two 16-bit rows have it copied, two fp32 rows not
+                assert one < 2 * 5000 * 255
+                assert (two > sizes[2] + 2 * 5000 * 255) == (kind != 0)
     assert lib.fgmm_xent_workspace_bytes(0, 9, 10, 10, 10, 1024, 16, 1, 0) == 0
     assert lib.fgmm_embed_workspace_bytes(1000, 50, 8) > 0
     assert lib.fgmm_embed_workspace_bytes(-1, 50, 8) == 0
