@@ -979,11 +979,12 @@ int check_common(const XentArgs& a) {
   return rc;
 }
 
-int check_device_and_workspace(const XentArgs& a, size_t need) {
+int check_workspace_and_device(const XentArgs& a, size_t need) {
+  int rc = vocab_check_workspace(a.name, a.ws, a.ws_bytes, need);
+  if (rc != FGMM_OK) return rc;
   std::string why;
-  const int rc = entry_check_device(&why);
-  if (rc != FGMM_OK) return entry_fail(rc, std::string(a.name) + ": " + why);
-  return vocab_check_workspace(a.name, a.ws, a.ws_bytes, need);
+  rc = entry_check_device(&why);
+  return rc == FGMM_OK ? rc : entry_fail(rc, std::string(a.name) + ": " + why);
 }
 
 int finish(const XentArgs& a, cudaError_t e) {
@@ -1037,7 +1038,7 @@ int fgmm_xent_fwd(int type, const void* X, int64_t x_stride_n, int64_t x_stride_
     if ((N > 0 && (!loss || !logZ)) || (reduction != FGMM_REDUCE_NONE && (!reduced || !count)))
       return entry_fail(FGMM_ERR_ARG, std::string(name) + ": null pointer argument");
     const XentWs w(workspace, false, type, N, V, D, W, w_stride_v, w_stride_d, bias != nullptr);
-    rc = check_device_and_workspace(a, w.bytes);
+    rc = check_workspace_and_device(a, w.bytes);
     if (rc != FGMM_OK) return rc;
     if (N == 0) {
       if (reduction != FGMM_REDUCE_NONE) {
@@ -1079,10 +1080,10 @@ int fgmm_xent_bwd(int type, const void* X, int64_t x_stride_n, int64_t x_stride_
     rc = vocab_check_array(name, "dX", dX, type_size(type), 0, 0);
     if (rc == FGMM_OK) rc = vocab_check_array(name, "dW", dW, type_size(type), 0, 0);
     if (rc != FGMM_OK) return rc;
-    const XentWs w(workspace, true, type, N, V, D, W, w_stride_v, w_stride_d, bias != nullptr);
+    const XentWs w(workspace, true, type, N, V, D, W, w_stride_v, w_stride_d, bias || dbias);
     if (w.units >= (int64_t(1) << 31) - (1 << 16))
       return entry_fail(FGMM_ERR_UNSUPPORTED, std::string(name) + ": N * V exceeds what one call counts; split the rows");
-    rc = check_device_and_workspace(a, w.bytes);
+    rc = check_workspace_and_device(a, w.bytes);
     if (rc != FGMM_OK) return rc;
     cudaError_t e = cudaSuccess;
     if (!dX && !dW && !dbias) return FGMM_OK;

@@ -228,7 +228,8 @@ FGMM_API int fgmm_generate_iso_rows(float* X, const int64_t* row_ids, int64_t ro
 
 /* Bytes of workspace fgmm_xent_fwd (backward = 0) or fgmm_xent_bwd
  * (backward = 1) needs for this shape and this W (which is not read: a W whose
- * address and strides TMA can take is used in place, another one is copied). */
+ * address and strides TMA can take is used in place, another one is copied).
+ * has_bias: nonzero when bias, or backward dbias, is not NULL. */
 FGMM_API size_t fgmm_xent_workspace_bytes(int backward, int type, int64_t N, int32_t V,
                                           int32_t D, const void* W, int64_t w_stride_v,
                                           int64_t w_stride_d, int has_bias);
@@ -251,7 +252,8 @@ FGMM_API int fgmm_xent_fwd(int type, const void* X, int64_t x_stride_n, int64_t 
  *   g_nv = (w_n + dlogZ_n) p_nv - w_n [v = target_n]
  *   dX = g W,   dW = g^T X,   dbias_v = sum_n g_nv
  * dloss or dlogZ may be NULL (zero), and each of dX, dW, dbias that is NULL
- * is not computed.  logZ is the forward call's.  Outputs share no bytes with
+ * is not computed; dbias may be asked where bias is NULL (zero).  logZ is the
+ * forward call's.  Outputs share no bytes with
  * inputs or each other. */
 FGMM_API int fgmm_xent_bwd(int type, const void* X, int64_t x_stride_n, int64_t x_stride_d,
                   const void* W, int64_t w_stride_v, int64_t w_stride_d, const float* bias,

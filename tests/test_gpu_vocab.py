@@ -618,3 +618,25 @@ def test_init_params_rows_are_unchanged(dtype):
         mu, _, _ = gmm_em.init_params(Y, 64, seed=3)
         idx = torch.randperm(5000, generator=torch.Generator().manual_seed(3))[:64].to(DEV)
         assert mu.dtype == torch.float32 and torch.equal(mu, X[idx].float())
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N", [1, 12, 300, 5000])
+def test_xent_bias_gradient_without_a_bias(N, dtype):
+    """The C entry takes dbias with a NULL bias: the sums of g over the rows."""
+    V, D = 2999, 40
+    X, W, t, _ = R.problem(N, V, D, dtype, seed=N)
+    kind, lib = L.FGMM_TYPES[dtype], L.load()
+    loss, logZ, _, _ = L.xent_fwd(X, W, t, None, R.IGNORE, "none")
+    w = torch.rand(N, device=DEV) + 0.5
+    need = lib.fgmm_xent_workspace_bytes(1, kind, N, V, D, W.data_ptr(), D, 1, 1)
+    # bytes behind the stated workspace have to stay as they are
+    ws = torch.full((need + (1 << 20),), 77, dtype=torch.uint8, device=DEV)
+    dX, dW, dbias = torch.empty_like(X), torch.empty_like(W), torch.empty(V, device=DEV)
+    L._launch(lib.fgmm_xent_bwd, X.device, kind, X.data_ptr(), D, 1, W.data_ptr(), D, 1, None,
+              t.data_ptr(), R.IGNORE, N, V, D, logZ.data_ptr(), w.data_ptr(), 1, None, None,
+              dX.data_ptr(), dW.data_ptr(), dbias.data_ptr(), ws.data_ptr(), need)
+    assert bool((ws[need:] == 77).all())
+    ref = R.xent(X, W, t, None, w=w)
+    for got, name in ((dX, "dX"), (dW, "dW"), (dbias, "dbias")):
+        R.assert_within(got, ref[name], ref["e_" + name], name)

@@ -132,6 +132,20 @@ def test_workspace_sizes(lib):
     assert lib.fgmm_embed_workspace_bytes(-1, 50, 8) == 0
 
 
+@pytest.mark.parametrize("kind", [0, 1, 2], ids=["fp32", "bf16", "fp16"])
+def test_xent_bwd_counts_dbias_without_a_bias(lib, kind):
+    """bias may be NULL where dbias is asked: its parts need their place in the workspace."""
+    N, V, D = 5000, 3000, 64
+    args = dict(C.BWD, type=kind, N=N, V=V, D=D, swv=D, sxn=D, dbias=256)
+    without = lib.fgmm_xent_workspace_bytes(1, kind, N, V, D, 256, D, 1, 0)
+    with_parts = lib.fgmm_xent_workspace_bytes(1, kind, N, V, D, 256, D, 1, 1)
+    assert with_parts > without
+    for bias in (None, 256):
+        got = lib.fgmm_xent_bwd(*dict(args, bias=bias, nws=without).values())
+        assert got == 2, (bias, got, lib.fgmm_last_error())
+        assert str(with_parts) in lib.fgmm_last_error().decode()
+
+
 def test_oracle_against_autograd():
     """The plain form the GPU tests compare with, against torch's own gradients in 64 bits."""
     X, W, t, c = R.problem(40, 30, 12, torch.float32, ignored=0.3, bias=True, device="cpu")
