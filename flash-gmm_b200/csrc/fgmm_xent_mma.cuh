@@ -774,10 +774,19 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     auto wg_sync = [&] {   // the warpgroup's 128 threads
       asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
     };
+    // Marks that other SMs set once their bulk stores were done.  Behind the wait come bulk
+    // stores and adds to the same memory (lane 0) and plain loads of it (all lanes): the
+    // proxy fence orders the first behind lane 0's acquire, __syncwarp the second (a vote
+    // orders no memory).
     auto wait_warp = [&](const uint32_t* count, uint32_t need) {
       bool there = true;
-      if (lane == 0) there = wait_marks(count, need, &ctl->abort_flag, err, 512);
-      return (bool)__all_sync(0xffffffffu, there);
+      if (lane == 0) {
+        there = wait_marks(count, need, &ctl->abort_flag, err, 512);
+        if (need != 0) fence_async_all();
+      }
+      there = __all_sync(0xffffffffu, there);
+      __syncwarp();
+      return there;
     };
     auto next = [&](uint32_t n) {
       if (FWD) return walk.next(t);

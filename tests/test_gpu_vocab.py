@@ -640,3 +640,23 @@ def test_xent_bias_gradient_without_a_bias(N, dtype):
     ref = R.xent(X, W, t, None, w=w)
     for got, name in ((dX, "dX"), (dW, "dW"), (dbias, "dbias")):
         R.assert_within(got, ref[name], ref["e_" + name], name)
+
+
+@pytest.mark.parametrize("dtype,N,V,D", [(BF, 5000, 70000, 64), (FH, 9000, 9000, 33),
+                                         (FS, 9000, 9000, 33)], ids=["bf16", "fp16", "fp32"])
+def test_xent_gradient_over_many_pieces(dtype, N, V, D):
+    """Pieces of g that go round the ring several times, sums of dX and dW handed from SM
+    to SM: right, and the same bits, in every one of many runs."""
+    X, W, t, _ = R.problem(N, V, D, dtype, seed=11)
+    loss, logZ, _, _ = L.xent_fwd(X, W, t, None, R.IGNORE, "none")
+    one = torch.ones((), device=DEV)
+    call = lambda: L.xent_bwd(X, W, t, None, R.IGNORE, logZ, one, None, None, (True, True, False))
+    first = call()
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(call()[:2], first[:2]))
+    rows = torch.arange(0, N, 97, device=DEV)            # dX of some rows
+    part = R.xent(X[rows], W, t[rows], None, w=torch.ones(len(rows), device=DEV))
+    R.assert_within(first[0][rows], part["dX"], part["e_dX"], "dX")
+    if V <= 10000:
+        ref = R.xent(X, W, t, None, w=torch.ones(N, device=DEV))
+        R.assert_within(first[1], ref["dW"], ref["e_dW"], "dW")
