@@ -228,6 +228,7 @@ struct MmaCtl {
   Tile feed[kFeedMax];
   uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
   uint64_t feed_full[kFeedMax], feed_empty[kFeedMax], unit_done[kFeedMax];
+  uint64_t wg_here[2];                // a warpgroup's four warps (wg_sync)
   uint32_t tmem;
   volatile int abort_flag;
 };
@@ -530,6 +531,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       mbar_init(&ctl->feed_empty[b], 2 * (kEpiWarps + 2) + 1);   // epilogue, loads, marks; MMA
       mbar_init(&ctl->unit_done[b], kEpiWarps);
     }
+    for (int b = 0; b < 2; ++b) mbar_init(&ctl->wg_here[b], 4);
     mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -771,8 +773,15 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       __syncwarp();
     };
     const uint32_t stage_at = smem_u32(stage);
-    auto wg_sync = [&] {   // the warpgroup's 128 threads
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+    // The warpgroup's four warps.  Bounded like every other wait (a hardware barrier is
+    // not): a warp that has left after a timeout does not keep the others.
+    uint32_t wg_parity = 0;
+    auto wg_sync = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->wg_here[wg]);
+      const bool there = wait(&ctl->wg_here[wg], wg_parity, 2048);
+      wg_parity ^= 1;
+      return (bool)__all_sync(0xffffffffu, there);
     };
     // Marks that other SMs set once their bulk stores were done.  Behind the wait come bulk
     // stores and adds to the same memory (lane 0) and plain loads of it (all lanes): the
@@ -1007,12 +1016,12 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
             reinterpret_cast<float*>(stage)[32 * c + lane] = column_sums(acc[c], lane);
-          wg_sync();
+          if (!wg_sync()) { ok = false; break; }
           const int e = (int)threadIdx.x & 127;
           const float* cs = reinterpret_cast<const float*>(out_stage + wg * 16384) + e;
           const float s = (cs[0] + cs[1 * 1024]) + (cs[2 * 1024] + cs[3 * 1024]);
           p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + col0 + e] = s;
-          wg_sync();
+          if (!wg_sync()) { ok = false; break; }
         }
         to_report = (int)(n % kFeed);
         continue;

@@ -2,6 +2,7 @@
 flash_vocab and of the C entries (validated before any device call)."""
 
 import ctypes
+import os
 
 import pytest
 import torch
@@ -15,7 +16,6 @@ X, W, T = torch.zeros(4, 8), torch.zeros(5, 8), torch.zeros(4, dtype=torch.int64
 
 @pytest.fixture(scope="module")
 def lib():
-    import os
     if not os.path.exists(L.LIB_PATH):
         import build_lib
         build_lib.build()
@@ -144,6 +144,18 @@ def test_xent_bwd_counts_dbias_without_a_bias(lib, kind):
         got = lib.fgmm_xent_bwd(*dict(args, bias=bias, nws=without).values())
         assert got == 2, (bias, got, lib.fgmm_last_error())
         assert str(with_parts) in lib.fgmm_last_error().decode()
+
+
+def test_no_unbounded_barrier_between_the_roles():
+    """The persistent kernel's warps leave one by one after a wait that gave up, so that they
+    may meet at mbarriers with bounded waits only: a hardware barrier of some of a block's
+    warps would keep the others for good."""
+    path = os.path.join(os.path.dirname(L.__file__), "csrc", "fgmm_xent_mma.cuh")
+    source = open(path).read()
+    assert "bar.sync" not in source and "barrier.sync" not in source
+    body = source[source.index("xent_mma_kernel("):]
+    roles = body[body.index("regs_down<72>"):body.rindex("tc_fence_before();")]
+    assert "__syncthreads" not in roles and "cluster_sync_all" not in roles
 
 
 def test_oracle_against_autograd():
