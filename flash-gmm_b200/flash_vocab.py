@@ -15,7 +15,8 @@ Nothing of size N x V is kept: the logits run through the chip in pieces of the
 vocabulary, forward and again backward.  W and X are bfloat16, float16 or
 float32 (both alike); sums, exponentials and logZ are float32.  Calls run on
 torch's current stream, do not synchronise, keep no state and can be captured
-into CUDA graphs.  There is no CPU fallback.
+into CUDA graphs.  There is no CPU fallback, and no forward-mode derivative
+(arguments with tangents are refused).
 """
 
 from __future__ import annotations
@@ -23,6 +24,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 import _fgmm_lib as L
@@ -39,6 +41,13 @@ def _need_gpu(**tensors):
             dev = t.device
         elif t.device != dev:
             raise ValueError(f"{name} is on {t.device}, the other arguments on {dev}")
+
+
+def _refuse_tangents(name: str, *tensors):
+    """The kernels see primal values only: a tangent would be lost without a word."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative: its arguments may not "
+                                  "carry tangents")
 
 
 def _tracked(*tensors) -> bool:
@@ -118,6 +127,7 @@ def linear_cross_entropy(X: torch.Tensor, W: torch.Tensor, targets: torch.Tensor
             raise ValueError(f"bias must be ({W.shape[0]},), got {tuple(bias.shape)}")
         if not bias.is_floating_point():
             raise ValueError(f"bias must be floating point, got {bias.dtype}")
+    _refuse_tangents("linear_cross_entropy", X, W, bias)
     labels = _labels("targets", targets)
     _need_gpu(X=X, W=W, targets=targets, bias=bias)
     if bias is not None:
@@ -165,6 +175,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"table must be (V, D) and not empty, got {tuple(table.shape)}")
     _need_type("table", table)
+    _refuse_tangents("embedding_lookup", table)
     flat = _labels("ids", ids)
     _need_gpu(table=table, ids=ids)
     fn = _EmbeddingLookup.apply if _tracked(table) else L.embed_fwd
@@ -182,7 +193,7 @@ def embedding_grad(dout: torch.Tensor, ids: torch.Tensor, V: int, *, scale: floa
     (contiguous, of dout's type); with ``accumulate`` the sums are added to it,
     e.g. to the other gradient of a tied table, and its other rows are left as
     they are.  ``out`` may not share memory with dout or ids (refused).
-    Bitwise the same on every run.
+    Bitwise the same on every run.  The result is not tracked by autograd.
     """
     if ids.shape != dout.shape[:-1] or dout.dim() < 1:
         raise ValueError(f"ids must be {tuple(dout.shape[:-1])}, got {tuple(ids.shape)}")
@@ -192,6 +203,7 @@ def embedding_grad(dout: torch.Tensor, ids: torch.Tensor, V: int, *, scale: floa
         raise ValueError(f"V and D must be positive, got {V} and {D}")
     if out is None and accumulate:
         raise ValueError("accumulate=True needs the out= buffer to add into")
+    _refuse_tangents("embedding_grad", dout, out)
     flat = _labels("ids", ids)
     _need_gpu(dout=dout, ids=ids, out=out)
     if out is None:

@@ -51,6 +51,27 @@ def test_refusals(call, match):
         call()
 
 
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name,call", [
+    ("linear_cross_entropy", lambda d: F.linear_cross_entropy(d(X), W, T)),
+    ("linear_cross_entropy", lambda d: F.linear_cross_entropy(X, d(W), T)),
+    ("linear_cross_entropy", lambda d: F.linear_cross_entropy(X, W, T, d(torch.zeros(5)))),
+    ("embedding_lookup", lambda d: F.embedding_lookup(d(W), T)),
+    ("embedding_grad", lambda d: F.embedding_grad(d(X), T, 5)),
+    ("embedding_grad", lambda d: F.embedding_grad(X, T, 5, out=d(W), accumulate=True)),
+])
+def test_tangents_are_refused(name, call, grad):
+    """A dual argument would give a result without its tangent."""
+    fw = torch.autograd.forward_ad
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(NotImplementedError, match=name):
+            call(lambda x: fw.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(NotImplementedError, match=name):
+        def f(x):
+            return call(lambda like: x[:like.numel()].view(like.shape))
+        torch.func.jvp(f, (torch.zeros(40),), (torch.ones(40),))
+
+
 class C:
     """One entry's arguments by name, valid ones for pointers that are never read."""
     XENT = dict(type=1, X=256, sxn=8, sxd=1, W=256, swv=8, swd=1, bias=None, targets=256,
