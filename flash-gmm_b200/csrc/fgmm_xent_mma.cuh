@@ -450,8 +450,8 @@ __device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
   return v[0];
 }
 
-// Two fp32 values in one register pair: Blackwell's packed add, multiply and FMA take
-// one issue slot for both.
+// Two fp32 values in one register pair: Blackwell's packed add and multiply take one
+// issue slot for both.
 using F2 = unsigned long long;
 __device__ __forceinline__ F2 f2(float a, float b) {
   F2 r;
@@ -469,11 +469,6 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   F2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 __device__ __forceinline__ F2 exp2_pair(F2 x) {
@@ -922,26 +917,20 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         const float mn = fmaxf(m_run, mx);
         s_run *= ex2((m_run - mn) * kLog2Ef);
         m_run = mn;
-        if (p.bias) {   // differences first, and exact zeros: a bias may be the lowest float
-          float s8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        // Differences first: the largest logit's term is exactly one, however large it is
+        // (an FMA with the rounded m log2 e was 2^60 off at logits of 1e9), and a removed
+        // entry's, or a bias of the lowest float's, exactly zero.
+        const F2 l2 = f2(kLog2Ef, kLog2Ef), nm2 = f2(-mn, -mn);
+        F2 s4[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c)
+        for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s8[i & 7] += ex2((acc[c][i] - mn) * kLog2Ef);
-          s_run += ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
-        } else {
-          const float nm = fminf(-mn, 2e38f) * kLog2Ef;   // finite where every entry is masked
-          const F2 l2 = f2(kLog2Ef, kLog2Ef), nm2 = f2(nm, nm);
-          F2 s4[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              s4[j & 3] = add2(s4[j & 3], exp2_pair(fma2(f2(acc[c][2 * j], acc[c][2 * j + 1]), l2, nm2)));
-          float sa, sb;
-          unpack(add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])), sa, sb);
-          s_run += sa + sb;
-        }
+          for (int j = 0; j < 16; ++j)
+            s4[j & 3] = add2(s4[j & 3], exp2_pair(mul2(
+                add2(f2(acc[c][2 * j], acc[c][2 * j + 1]), nm2), l2)));
+        float sa, sb;
+        unpack(add2(add2(s4[0], s4[1]), add2(s4[2], s4[3])), sa, sb);
+        s_run += sa + sb;
         if (t.flags & 1) p.part[(int64_t)(2 * t.ks + wg) * p.Np + row] = make_float2(m_run, s_run);
         continue;
       }
@@ -949,24 +938,15 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       if (t.kind == kGrad) {
         const int v0 = (int)t.brow + col0;
         const float ga = rg.a * scales.g, gb = rg.b * scales.g;
-        if (p.bias) {
+        // (S - logZ) first, for the same reason: p stays at most one
+        const F2 l2 = f2(kLog2Ef, kLog2Ef), ga2 = f2(ga, ga), off = f2(-rg.lse, -rg.lse);
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c)
+        for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c][i] = ga * ex2((acc[c][i] - rg.lse) * kLog2Ef);
-        } else {
-          // bf16 and fp16 words hide the rounding of lse log2(e) in the product's FMA
-          const F2 l2 = f2(kLog2Ef, kLog2Ef), ga2 = f2(ga, ga);
-          const F2 off = SPLIT ? f2(-rg.lse, -rg.lse) : f2(-rg.lse * kLog2Ef, -rg.lse * kLog2Ef);
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const F2 v = f2(acc[c][2 * j], acc[c][2 * j + 1]);
-              const F2 x = SPLIT ? mul2(add2(v, off), l2) : fma2(v, l2, off);
-              unpack(mul2(exp2_pair(x), ga2), acc[c][2 * j], acc[c][2 * j + 1]);
-            }
-        }
+          for (int j = 0; j < 16; ++j) {
+            const F2 v = f2(acc[c][2 * j], acc[c][2 * j + 1]);
+            unpack(mul2(exp2_pair(mul2(add2(v, off), l2)), ga2), acc[c][2 * j], acc[c][2 * j + 1]);
+          }
         const int tc = rg.target - v0;
         if (__any_sync(0xffffffffu, tc >= 0 && tc < kCols)) {
 #pragma unroll

@@ -660,3 +660,40 @@ def test_xent_gradient_over_many_pieces(dtype, N, V, D):
     if V <= 10000:
         ref = R.xent(X, W, t, None, w=torch.ones(N, device=DEV))
         R.assert_within(first[1], ref["dW"], ref["e_dW"], "dW")
+
+
+@pytest.mark.parametrize("bias", [False, True], ids=["plain", "bias"])
+@pytest.mark.parametrize("power", [6, 9, 12])
+@pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
+def test_xent_logits_far_beyond_the_exponentials_range(dtype, power, bias):
+    """Rows as a diverged model gives them: the largest logit takes all of the probability."""
+    N, V, D = 40, 500, 64
+    X, W, t, c = R.problem(N, V, D, dtype, seed=power, bias=bias)
+    X = X * 10.0 ** power
+    X.requires_grad_(), W.requires_grad_()
+    ref = R.xent(X, W, t, c)
+    loss, logZ = F.linear_cross_entropy(X, W, t, c, reduction="none", return_logZ=True)
+    R.assert_within(loss.detach(), ref["loss"], ref["e_loss"], "loss")
+    R.assert_within(logZ.detach(), ref["logZ"], ref["e_logZ"], "logZ")
+    dX, dW = torch.autograd.grad(loss.sum(), (X, W))
+    # logits are known within e_logZ: where the largest leads by more than that and 200,
+    # every other exponential is zero, in 64 bits and in 32
+    S = X.detach().double() @ W.detach().double().t()
+    top = S.topk(2, 1)
+    sure = top.values[:, 0] - top.values[:, 1] > 2 * ref["e_logZ"] + 200
+    assert int(sure.sum()) > N // 2
+    G = torch.zeros(N, V, device=DEV, dtype=torch.float64)
+    rows = torch.arange(N, device=DEV)
+    G[rows, top.indices[:, 0]] = 1.0
+    G[rows, t] -= 1.0
+    u = R.U[dtype]
+    want = G @ W.detach().double()
+    mag = G.abs() @ W.detach().double().abs()
+    R.assert_within(dX[sure], want[sure], ((u + R.chain(V)) * mag + R.TINY[dtype])[sure], "dX")
+    # entries that only such rows name
+    only = ((G != 0) & ~sure[:, None]).sum(0) == 0
+    only &= ((S - S.amax(1, keepdim=True) > -2 * ref["e_logZ"][:, None] - 200)
+             & ~sure[:, None]).sum(0) == 0
+    want = G.t() @ X.detach().double()
+    mag = G.abs().t() @ X.detach().double().abs()
+    R.assert_within(dW[only], want[only], ((u + R.chain(N)) * mag + R.TINY[dtype])[only], "dW")
