@@ -64,12 +64,12 @@ struct __align__(16) RowGrad {
 #include "fgmm_xent_mma.cuh"
 
 // First words of the workspace.  Every word is written before it is read: err and
-// done by the tensor-core kernel's first launch, the others by rows_kernel.
+// done by the tensor-core kernel, the others by rows_kernel.
 struct Header {
   int err[kErrSlots];   // nonzero: a wait of that block of the tensor-core kernel gave up
   int done;             // blocks of the closing forward kernel that have finished
   int live;             // rows that are not ignored
-  int amax[3];          // float bits of the largest finite |weight|, |x|, |w|
+  int amax;             // backward: float bits of the largest finite |weight|
 };
 
 constexpr int kRowsPerBlock = 4096;
@@ -101,13 +101,13 @@ struct XentWs {
   Header* hdr;
   int *rows, *inv, *target, *counts;
   float* bias;
-  void *Xp, *Xp2, *Wp, *Wp2;      // packed operands (SPLIT: hi and lo words)
+  void *Xp[3], *Wp[3];             // packed operands (fp32: hi, mid and lo words)
   float2* part;
   float* tlogit;
   double* loss_part;               // [blocks][2] sum, count
   RowGrad* rg;
   uint32_t* sync;
-  void *G, *G2;
+  void* G[3];
   float *dbias_part, *dx_slots, *dw_slots;
   float *small_g, *small_dx;       // of a few rows: g [V][nb], parts of dX [splits][nb][D]
 
@@ -161,10 +161,11 @@ struct XentWs {
     target = c.take<int>(Np);
     counts = c.take<int>((N + kRowsPerBlock - 1) / kRowsPerBlock);
     bias = c.take<float>(want_bias ? Vp : 0);
-    Xp = c.take<uint16_t>((size_t)Np * Dp);
-    Xp2 = c.take<uint16_t>(split ? (size_t)Np * Dp : 0);
-    Wp = c.take<uint16_t>(pack_w ? (size_t)V * Dp : 0);
-    Wp2 = c.take<uint16_t>(split ? (size_t)V * Dp : 0);
+    const int words = split ? 3 : 1;
+    for (int h = 0; h < 3; ++h) {
+      Xp[h] = c.take<uint16_t>(h < words ? (size_t)Np * Dp : 0);
+      Wp[h] = c.take<uint16_t>(h < words && pack_w ? (size_t)V * Dp : 0);
+    }
     const int64_t mt = Np / kPairRows;
     if (!backward) {
       // Vocabulary tiles per unit: the fewest rounds of the pairs, counting a quarter
@@ -181,7 +182,7 @@ struct XentWs {
       tlogit = c.take<float>(Np);
       loss_part = c.take<double>(2 * ((N + 31) / 32));
     } else {
-      const int word = split ? 4 : 2;
+      const int word = 2 * words;
       // column tiles of dX and dW: a 128-wide block takes about 0.7 of a 256-wide one's time
       bn_d = D <= 128 ? 128 : 256;
       tiles_d = (D + bn_d - 1) / bn_d;
@@ -197,9 +198,11 @@ struct XentWs {
                                      kPieceBytes / ((int64_t)row_chunk * word) / 256 * 256));
       n_chunks = (int)((Np + row_chunk - 1) / row_chunk);
       n_pieces = (int)((Vp + piece - 1) / piece);
-      // Splits of K: products of at most kUnit blocks, shorter where a product's tiles
-      // could not occupy the pairs twice; dW's only where its slots hold all of V.
-      const int64_t unit = split ? 24 : 64;
+      // Splits of K: products of at most `unit` blocks, shorter where a product's tiles
+      // could not occupy the pairs twice; dW's only where its slots hold all of V.  fp32
+      // blocks take six times the MMAs: 131072 x 1024 x 128 816 us with 12, 955 with 16,
+      // 984 with 24; 2048 x 16384 x 512 595, 607 and 659.
+      const int64_t unit = split ? 12 : 64;
       auto pick = [&](int64_t tiles, int64_t kb, int64_t slot_bytes) {
         int64_t ks = std::max<int64_t>((kb + unit - 1) / unit, (2 * kPairs + tiles - 1) / tiles);
         ks = std::min(ks, std::max<int64_t>(1, kb / 8));
@@ -215,8 +218,8 @@ struct XentWs {
       rg = c.take<RowGrad>(Np);
       sync_words = 1 + 2 * steps + (Np / kPairRows * ks_x + (int64_t)(piece / 256) * ks_w) * tiles_d;
       sync = c.take<uint32_t>(sync_words);
-      G = c.take<uint16_t>((size_t)kRing * row_chunk * piece);
-      G2 = c.take<uint16_t>(split ? (size_t)kRing * row_chunk * piece : 0);
+      for (int h = 0; h < 3; ++h)
+        G[h] = c.take<uint16_t>(h < words ? (size_t)kRing * row_chunk * piece : 0);
       dbias_part = c.take<float>(want_bias ? (size_t)(Np / 128) * Vp : 0);
       dx_slots = c.take<float>((size_t)ks_x * Np * ldS);
       dw_slots = c.take<float>(n_chunks == 1 && ks_w == 1 ? 0 : (size_t)ks_w * piece * ldS);
@@ -258,7 +261,7 @@ rows_kernel(const XentArgs a, const XentWs w, int counted) {
   __shared__ int wsum[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t base = (int64_t)blockIdx.x * kRowsPerBlock;
-  if (blockIdx.x == 0 && threadIdx.x < 3) w.hdr->amax[threadIdx.x] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.hdr->amax = 0;
   if (a.logZ_in)   // backward: the product kernel's counts
     for (int64_t i = blockIdx.x * 1024 + threadIdx.x; i < w.sync_words; i += gridDim.x * 1024)
       w.sync[i] = 0;
@@ -309,81 +312,28 @@ struct Share {
   int block, blocks;
 };
 
-// Largest finite magnitude of the listed rows (of all n without a list); a warp
-// takes four rows at a time, 16 bytes a lane where the layout allows (vec).
-__device__ __forceinline__ void amax_rows(const Share sh, const float* __restrict__ A, int64_t s0,
-                                          int64_t s1, int D, int64_t n,
-                                          const int* __restrict__ rows, int vec,
-                                          int* __restrict__ amax) {
-  const int lane = threadIdx.x & 31;
-  float m = 0.f;
-  auto see = [&](float x) {
-    x = fabsf(x);
-    if (x < INFINITY) m = fmaxf(m, x);
-  };
-  for (int64_t i0 = (sh.block * 8ll + (threadIdx.x >> 5)) * 4; i0 < n; i0 += sh.blocks * 32ll) {
-    const float* row[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t i = min(i0 + u, n - 1);
-      row[u] = A + (rows ? rows[i] : i) * s0;
-    }
-    if (vec) {
-      for (int d = lane * 4; d < D; d += 128) {
-        float4 x[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const float4*>(row[u] + d);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) { see(x[u].x); see(x[u].y); see(x[u].z); see(x[u].w); }
-      }
-    } else {
-      for (int d = lane; d < D; d += 32) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) see(row[u][d * s1]);
-      }
-    }
-  }
-  m = redux_max(m);
-  if (lane == 0 && m > 0.f) atomicMax(amax, __float_as_int(m));
-}
-
-// fp32: the magnitudes that scale X (blocks before blocks_x) and W.
-__global__ void __launch_bounds__(256)
-amax_kernel(const XentArgs a, const XentWs w, int blocks_x, int vec_x, int vec_w) {
-  pdl_trigger();
-  pdl_wait();
-  const int b = blockIdx.x;
-  if (b < blocks_x)
-    amax_rows(Share{b, blocks_x}, static_cast<const float*>(a.X), a.sxn, a.sxd, a.D, w.hdr->live,
-              w.rows, vec_x, &w.hdr->amax[1]);
-  else
-    amax_rows(Share{b - blocks_x, (int)gridDim.x - blocks_x}, static_cast<const float*>(a.W), a.swv,
-              a.swd, a.D, a.V, nullptr, vec_w, &w.hdr->amax[2]);
-}
-
 // Dense copies of X's live rows (rows != null; zero rows up to a multiple of
-// kPairRows) or of W, D padded with zeros to Dp; fp32 becomes two fp16 words of
-// the value / 2^e.  8 elements a thread, `lanes` threads (a power of two) a row.
+// kPairRows) or of W, D padded with zeros to Dp; fp32 becomes three bf16 words.
+// 8 elements a thread, `lanes` threads (a power of two) a row.
 template <class T>
 __device__ __forceinline__ void pack_rows(const Share sh, const T* __restrict__ A, int64_t s0,
                                           int64_t s1, int D, int Dp, int64_t n,
                                           const int* __restrict__ rows, int vec, int lanes,
-                                          const int* __restrict__ amax, uint16_t* __restrict__ out,
-                                          uint16_t* __restrict__ out2) {
+                                          void* const (&out)[3]) {
   constexpr bool kSplit = sizeof(T) == 4;
   const int per_row = Dp / 8, per_block = 256 / lanes;
-  const float scale = kSplit ? ldexpf(1.f, -Scales::exponent(*amax, 14)) : 1.f;
   for (int64_t i = sh.block * (int64_t)per_block + threadIdx.x / lanes; i < n;
        i += sh.blocks * (int64_t)per_block) {
     const int64_t r = rows ? rows[i] : i;
     for (int c = threadIdx.x % lanes; c < per_row; c += lanes) {
       const int64_t e = i * per_row + c;
       const int d0 = c * 8;
-      uint4 w = make_uint4(0u, 0u, 0u, 0u), w2 = w;
+      uint4 w[3];
+      w[0] = w[1] = w[2] = make_uint4(0u, 0u, 0u, 0u);
       if (r >= 0) {
         const T* src = A + r * s0 + (int64_t)d0 * s1;
         if (!kSplit && vec && d0 + 8 <= D) {
-          w = *reinterpret_cast<const uint4*>(src);
+          w[0] = *reinterpret_cast<const uint4*>(src);
         } else {
           T v[8];
           if (kSplit && vec && d0 + 8 <= D) {
@@ -393,18 +343,19 @@ __device__ __forceinline__ void pack_rows(const Share sh, const T* __restrict__ 
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = d0 + k < D ? src[k * s1] : from_f32<T>(0.f);
           }
-          uint32_t h[4], l[4];
+          uint32_t u[4][3];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            if (kSplit) split2(to_f32(v[2 * k]) * scale, to_f32(v[2 * k + 1]) * scale, h[k], l[k]);
-            else h[k] = pack2<T>(to_f32(v[2 * k]), to_f32(v[2 * k + 1]));
+            if (kSplit) split3(to_f32(v[2 * k]), to_f32(v[2 * k + 1]), u[k]);
+            else u[k][0] = pack2<T>(to_f32(v[2 * k]), to_f32(v[2 * k + 1]));
           }
-          w = make_uint4(h[0], h[1], h[2], h[3]);
-          if (kSplit) w2 = make_uint4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+          for (int h = 0; h < (kSplit ? 3 : 1); ++h)
+            w[h] = make_uint4(u[0][h], u[1][h], u[2][h], u[3][h]);
         }
       }
-      reinterpret_cast<uint4*>(out)[e] = w;
-      if (kSplit) reinterpret_cast<uint4*>(out2)[e] = w2;
+#pragma unroll
+      for (int h = 0; h < (kSplit ? 3 : 1); ++h) static_cast<uint4*>(out[h])[e] = w[h];
     }
   }
 }
@@ -430,7 +381,7 @@ __device__ __forceinline__ void row_weights(const Share sh, const XentArgs& a, c
     w.rg[i] = r;
   }
   top = redux_max(top);
-  if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&w.hdr->amax[0], __float_as_int(top));
+  if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&w.hdr->amax, __float_as_int(top));
 }
 
 // Blocks of prepare_kernel by what they do, in this order.
@@ -450,15 +401,13 @@ prepare_kernel(const XentArgs a, const XentWs w, const PrepareShares sh) {
   if (b < sh.x) {
     const int64_t n = ((int64_t)w.hdr->live + kPairRows - 1) / kPairRows * kPairRows;
     pack_rows<T>(Share{b, sh.x}, static_cast<const T*>(a.X), a.sxn, a.sxd, a.D, w.Dp, n, w.rows,
-                 sh.vec_x, sh.lanes, &w.hdr->amax[1], static_cast<uint16_t*>(w.Xp),
-                 static_cast<uint16_t*>(w.Xp2));
+                 sh.vec_x, sh.lanes, w.Xp);
     return;
   }
   b -= sh.x;
   if (b < sh.w) {
     pack_rows<T>(Share{b, sh.w}, static_cast<const T*>(a.W), a.swv, a.swd, a.D, w.Dp, a.V, nullptr,
-                 sh.vec_w, sh.lanes, &w.hdr->amax[2], static_cast<uint16_t*>(w.Wp),
-                 static_cast<uint16_t*>(w.Wp2));
+                 sh.vec_w, sh.lanes, w.Wp);
     return;
   }
   b -= sh.w;
@@ -617,7 +566,7 @@ __device__ __forceinline__ void store_dbias(int block, const XentArgs& a, const 
     s = red[0][lane];
 #pragma unroll
     for (int k = 1; k < 32; ++k) s += red[k][lane];
-    a.dbias[v] = s / Scales(w.hdr->amax, a.type != FGMM_T_BF16, a.type == FGMM_T_F32).g;
+    a.dbias[v] = s / Scales(&w.hdr->amax, a.type == FGMM_T_F16).g;
   }
 }
 
@@ -646,16 +595,16 @@ finish_backward_kernel(const XentArgs a, const XentWs w, const FinishShares sh) 
     if (a.dbias) fill_nan(a.dbias, a.V);
     return;
   }
-  const Scales sc(w.hdr->amax, !std::is_same<T, __nv_bfloat16>::value, sizeof(T) == 4);
+  const float back = Scales(&w.hdr->amax, std::is_same<T, __half>::value).back;
   int b = blockIdx.x;
   if (b < sh.dx) {
-    store_slots<T>(Share{b, sh.dx}, w.dx_slots, w.ks_x, w.Np, w.ldS, a.D, a.N, w.inv, sc.dx,
+    store_slots<T>(Share{b, sh.dx}, w.dx_slots, w.ks_x, w.Np, w.ldS, a.D, a.N, w.inv, back,
                    sh.lanes, static_cast<T*>(a.dX));
     return;
   }
   b -= sh.dx;
   if (b < sh.dw) {
-    store_slots<T>(Share{b, sh.dw}, w.dw_slots, w.ks_w, w.piece, w.ldS, a.D, a.V, nullptr, sc.dw,
+    store_slots<T>(Share{b, sh.dw}, w.dw_slots, w.ks_w, w.piece, w.ldS, a.D, a.V, nullptr, back,
                    sh.lanes, static_cast<T*>(a.dW));
     return;
   }
@@ -714,43 +663,42 @@ cudaError_t make_map(EncodeTiled encode, CUtensorMap* m, CUtensorMapDataType typ
 }
 template <class T>
 constexpr CUtensorMapDataType word_type() {
-  return std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
 // Operand word of each element type, and what dW is stored as.
 template <class T> struct Word { using type = T; };
-template <> struct Word<float> { using type = __half; };
+template <> struct Word<float> { using type = __nv_bfloat16; };
+template <class T> constexpr int kWordsOf = sizeof(T) == 4 ? 3 : 1;
 
 template <class T>
 cudaError_t make_operand_maps(const XentArgs& a, const XentWs& w, bool direct, MmaMaps* maps) {
-  constexpr bool kSplit = sizeof(T) == 4;
   constexpr CUtensorMapDataType type = word_type<T>();
   EncodeTiled enc;
   cudaError_t e = encode_fn(&enc);
-  if (e != cudaSuccess) return e;
-  e = direct ? make_map(enc, &maps->X, type, a.X, a.N, a.D, a.sxn, 64)
-             : make_map(enc, &maps->X, type, w.Xp, w.Np, a.D, w.Dp, 64);
-  if (e == cudaSuccess)
-    e = w.pack_w ? make_map(enc, &maps->W, type, w.Wp, a.V, a.D, w.Dp, 64)
-                 : make_map(enc, &maps->W, type, a.W, a.V, a.D, a.swv, 64);
-  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->X2, type, w.Xp2, w.Np, a.D, w.Dp, 64);
-  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->W2, type, w.Wp2, a.V, a.D, w.Dp, 64);
+  for (int h = 0; h < kWordsOf<T>; ++h) {
+    if (e == cudaSuccess)
+      e = direct ? make_map(enc, &maps->X[h], type, a.X, a.N, a.D, a.sxn, 64)
+                 : make_map(enc, &maps->X[h], type, w.Xp[h], w.Np, a.D, w.Dp, 64);
+    if (e == cudaSuccess)
+      e = w.pack_w ? make_map(enc, &maps->W[h], type, w.Wp[h], a.V, a.D, w.Dp, 64)
+                   : make_map(enc, &maps->W[h], type, a.W, a.V, a.D, a.swv, 64);
+  }
   return e;
 }
 
 // Maps of G, loaded and stored, and of the fp32 slots.
 template <class T>
 cudaError_t make_backward_maps(const XentWs& w, MmaMaps* maps) {
-  constexpr bool kSplit = sizeof(T) == 4;
   constexpr CUtensorMapDataType type = word_type<T>(), f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const int64_t rows = (int64_t)kRing * w.row_chunk;
   EncodeTiled enc;
   cudaError_t e = encode_fn(&enc);
-  if (e == cudaSuccess) e = make_map(enc, &maps->G, type, w.G, rows, w.piece, w.piece, 64);
-  if (e == cudaSuccess) e = make_map(enc, &maps->Gs, type, w.G, rows, w.piece, w.piece, 32);
-  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->G2, type, w.G2, rows, w.piece, w.piece, 64);
-  if (kSplit && e == cudaSuccess) e = make_map(enc, &maps->G2s, type, w.G2, rows, w.piece, w.piece, 32);
+  for (int h = 0; h < kWordsOf<T>; ++h) {
+    if (e == cudaSuccess) e = make_map(enc, &maps->G[h], type, w.G[h], rows, w.piece, w.piece, 64);
+    if (e == cudaSuccess) e = make_map(enc, &maps->Gs[h], type, w.G[h], rows, w.piece, w.piece, 32);
+  }
   if (e == cudaSuccess) e = make_map(enc, &maps->dxs, f32, w.dx_slots, w.ks_x * w.Np, w.ldS, w.ldS, 32);
   if (e == cudaSuccess)
     e = make_map(enc, &maps->dws, f32, w.dw_slots, (int64_t)w.ks_w * w.piece, w.ldS, w.ldS, 32);
@@ -761,12 +709,10 @@ cudaError_t make_backward_maps(const XentWs& w, MmaMaps* maps) {
 // tells whether there was a launch.
 template <class T>
 cudaError_t prepare(const XentArgs& a, const XentWs& w, bool direct, bool backward, bool* dependent) {
-  constexpr bool kSplit = sizeof(T) == 4;
   *dependent = false;
   cudaError_t e = cudaSuccess;
-  auto vec = [&](const void* p, int64_t s0, int64_t s1, int whole) {
-    return s1 == 1 && s0 * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 &&
-           a.D % whole == 0;
+  auto vec = [&](const void* p, int64_t s0, int64_t s1) {
+    return s1 == 1 && s0 * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
   };
   if (!direct) {
     const int64_t blocks = (a.N + kRowsPerBlock - 1) / kRowsPerBlock;
@@ -775,20 +721,14 @@ cudaError_t prepare(const XentArgs& a, const XentWs& w, bool direct, bool backwa
     if (e == cudaSuccess) e = launch(rows_kernel, blocks, 1024, 0, a.stream, counted, a, w, (int)counted);
     *dependent = true;
   }
-  if constexpr (kSplit) {
-    const int bx = blocks_for(a.N * 8), bw = blocks_for((int64_t)a.V * 8);
-    if (e == cudaSuccess)
-      e = launch(amax_kernel, bx + bw, 256, 0, a.stream, true, a, w, bx, vec(a.X, a.sxn, a.sxd, 4),
-                 vec(a.W, a.swv, a.swd, 4));
-  }
   PrepareShares sh{};
   sh.lanes = row_lanes(w.Dp / 8, 256);
   sh.x = direct ? 0 : blocks_for(w.Np * sh.lanes);
   sh.w = w.pack_w ? blocks_for((int64_t)a.V * sh.lanes) : 0;
   sh.bias = a.bias ? blocks_for(w.Vp) : 0;
   sh.rows = backward ? blocks_for(w.Np) : 0;
-  sh.vec_x = vec(a.X, a.sxn, a.sxd, 1);
-  sh.vec_w = vec(a.W, a.swv, a.swd, 1);
+  sh.vec_x = vec(a.X, a.sxn, a.sxd);
+  sh.vec_w = vec(a.W, a.swv, a.swd);
   const int grid = sh.x + sh.w + sh.bias + sh.rows;
   if (e == cudaSuccess && grid > 0) {
     e = launch(prepare_kernel<T>, grid, 256, 0, a.stream, *dependent, a, w, sh);
@@ -802,7 +742,7 @@ MmaParams common_params(const XentArgs& a, const XentWs& w) {
   p.live = &w.hdr->live;
   p.err = w.hdr->err;
   p.done = &w.hdr->done;
-  p.amax = w.hdr->amax;
+  p.amax = &w.hdr->amax;
   p.N = a.N;
   p.D = a.D;
   p.V = a.V;
@@ -943,8 +883,6 @@ cudaError_t xent_backward(const XentArgs& a, const XentWs& w) {
   p.n_pieces = w.n_pieces;
   p.sync = w.sync;
   p.rg = w.rg;
-  p.G = w.G;
-  p.G2 = w.G2;
   p.dbias_part = a.dbias ? w.dbias_part : nullptr;
   p.ks_x = w.ks_x;
   p.ks_w = w.ks_w;

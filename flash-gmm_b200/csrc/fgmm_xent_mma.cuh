@@ -16,8 +16,13 @@
 // be bound by the L2.  Two 256-column accumulators in TMEM let eight epilogue warps
 // work on one tile while the next is multiplied.
 //
-// SPLIT (fp32 inputs): operands are pairs of fp16 words hi + lo of the values scaled
-// by one power of two per matrix, and a K-block runs lo hi, hi lo and hi hi.
+// SPLIT (fp32 inputs): operands are three bf16 words hi + mid + lo, each the rounding of
+// what the ones before leave (2^-9 of it), so they hold a value to 2^-27 over fp32's whole
+// range: no scale per matrix, and small values beside large ones keep their bits.  A
+// K-block runs the six products of words above 2^-27, smallest first: lo hi, hi lo, mid mid,
+// mid hi, hi mid, hi hi.  (Two fp16 words with three products took about half the time but
+// share one exponent range of 2^-39 with the matrix's largest value: a column, a row or a
+// row weight 1e8 times the others' lost the others.)
 //
 // The tensor core cuts its running sum toward zero at each step of 16, about 2^-24 of
 // it on average: logits of 63 steps measured 2.3e-6 low.  Logits (and all of SPLIT) are
@@ -41,7 +46,7 @@ constexpr int kErrSlots = 256;    // blocks of this kernel, at most
 constexpr int kBoxBytes = 64 * 128;
 constexpr int kEpiWarps = 8;
 constexpr int kMmaThreads = (4 + kEpiWarps) * 32;
-constexpr int kSplitBlocks = 2;   // K-blocks per group: 24 steps
+constexpr int kSplitBlocks = 1;   // K-blocks per group: 4 steps of hi hi upon small ones
 constexpr int kLogitBlocks = 4;   // 16 steps
 
 enum TileKind { kLse = 0, kGrad = 1, kDx = 2, kDw = 3 };
@@ -60,7 +65,7 @@ struct MmaParams {
   const int64_t* targets;  // row i's target is targets[i]
   int64_t Np;
   const float* bias;       // padded to 256 with -inf, or null
-  const int* amax;         // float bits of the largest |g weight|, |x|, |w| (Scales)
+  const int* amax;         // backward: float bits of the largest |g weight| (Scales)
   // backward
   int has_dx, has_dw;
   int row_chunk, piece;    // rows x entries of a piece of G (multiples of 256)
@@ -68,7 +73,6 @@ struct MmaParams {
   uint32_t* sync;          // from 0: units claimed, then marks of kGrad and of the products by
                            // piece, then of each tile of dX's and of dW's slots
   const RowGrad* rg;
-  void *G, *G2;            // [kRing row_chunk][piece] words (G2: lo words)
   float* dbias_part;       // [2 Np / 256][Vp], or null
   int64_t Vp;
   int ks_x, ks_w;          // splits of K
@@ -79,35 +83,26 @@ struct MmaParams {
 };
 
 struct MmaMaps {
-  CUtensorMap X, W, G, X2, W2, G2;    // 64 x 64 boxes of words, loaded
-  CUtensorMap Gs, G2s;                // 64 x 32 boxes of words, stored
-  CUtensorMap dxs, dws;               // 32 x 32 boxes of fp32, stored or added
+  CUtensorMap X[3], W[3], G[3];   // 64 x 64 boxes of words, loaded (SPLIT: hi, mid, lo)
+  CUtensorMap Gs[3];              // 64 x 32 boxes of words, stored
+  CUtensorMap dxs, dws;           // 32 x 32 boxes of fp32, stored or added
 };
 
-// Scales of the stored words.  G is stored over the largest row weight: with equal
-// weights (a sum or a mean) the -1 at the label is then exact, where a weight like
-// 1/7372 rounded to bf16 would scale the whole gradient by up to 2^-9.  fp16 words are
-// 2^12 times that (at most 2^13, down to p = 2^-27 without losing bits).  SPLIT: X and
-// W too, by a power of two each with the largest finite magnitude in [2^13, 2^14), so
-// values down to 2^-16 of the largest keep 22 bits and smaller ones an error of 2^-39
-// of the largest.
+// Scale of the stored g, and what undoes it in the products.  G is stored over the largest
+// row weight: with equal weights (a sum or a mean) the -1 at the label is then exact, where
+// a weight like 1/7372 rounded to bf16 would scale the whole gradient by up to 2^-9.  bf16
+// words (and SPLIT's) keep their bits over fp32's range.  fp16 words are 2^12 times that:
+// |g| of 2^-26 of the largest weight and more keeps its 11 bits, smaller ones an error of
+// 2^-37 of the largest weight.
 struct Scales {
-  float s, g, dx, dw;   // S, stored G, and the products with G
-  __device__ static int exponent(int bits, int target) {
-    return max(-100, min(100, scale_exp_to(__int_as_float(bits), target)));
-  }
-  __device__ Scales(const int* amax, bool f16, bool split) {
-    if (!amax) { s = g = dx = dw = 1.f; return; }   // 16-bit logits: nothing is scaled
-    const float top = __int_as_float(amax[0]);
+  float g, back;
+  __device__ Scales(const int* amax, bool f16) {
+    const float top = __int_as_float(*amax);
     const float unit = f16 ? 4096.f : 1.f;
     // weights outside 2^-100 .. 2^100: their reciprocal would leave fp32
     const bool sane = top > 7.9e-31f && top < 1.2e30f;
     g = sane ? unit / top : unit;
-    const float back = sane ? top / unit : 1.f / unit;
-    const int ex = split ? exponent(amax[1], 14) : 0, ew = split ? exponent(amax[2], 14) : 0;
-    s = ldexpf(1.f, ex + ew);
-    dx = ldexpf(back, ew);
-    dw = ldexpf(back, ex);
+    back = sane ? top / unit : 1.f / unit;
   }
 };
 
@@ -212,11 +207,12 @@ constexpr int kFeedMax = 4;       // places of the feed
 
 template <bool SPLIT>
 struct MmaCfg {
-  static constexpr int kStages = SPLIT ? 3 : 6;
+  static constexpr int kWords = SPLIT ? 3 : 1;
+  static constexpr int kStages = SPLIT ? 2 : 6;
   static constexpr int kFeed = SPLIT ? 3 : kFeedMax;         // tiles handed out ahead
   static constexpr int kA = 2 * kBoxBytes;                   // 128 rows x 64
   static constexpr int kB = (kBN / 2 / 64) * kBoxBytes;      // this SM's half of B
-  static constexpr int kStage = (SPLIT ? 2 : 1) * (kA + kB);
+  static constexpr int kStage = kWords * (kA + kB);
   static constexpr int kStageOut = kEpiWarps * 4096;         // 32 rows x 128 B per warp
   static constexpr int kCtl = 768;
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStageOut + kCtl;
@@ -496,8 +492,23 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
 }
 template <>
 __device__ __forceinline__ uint32_t pack2<float>(float, float) { return 0; }
+// What a pair of bf16 words leaves of (a, b), exact in fp32.
+__device__ __forceinline__ void minus_word(float& a, float& b, uint32_t w) {
+  a -= __uint_as_float(w << 16);
+  b -= __uint_as_float(w & 0xffff0000u);
+}
+// The three words of a pair of fp32 values.  Values that would round to infinity are cut.
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
+  w[0] = pack2<__nv_bfloat16>(a, b);
+  if (fmaxf(fabsf(a), fabsf(b)) >= 0x1p127f)
+    w[0] = (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u);
+  minus_word(a, b, w[0]);
+  w[1] = pack2<__nv_bfloat16>(a, b);
+  minus_word(a, b, w[1]);
+  w[2] = pack2<__nv_bfloat16>(a, b);
+}
 
-// T: the type of the operand words (SPLIT: __half); TO: the type of dW.
+// T: the type of the operand words (SPLIT: bf16); TO: the type of dW.
 template <bool FWD, bool SPLIT, class T, class TO>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMmaThreads, 1)
 xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ MmaMaps maps) {
@@ -590,13 +601,11 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           fence_async_all();
         }
         const bool a_mn = t.kind == kDw, b_mn = t.kind >= kDx;
-        const CUtensorMap* ma = t.kind <= kGrad ? &maps.X : &maps.G;
-        const CUtensorMap* mb = t.kind == kDw ? &maps.X : &maps.W;
-        const CUtensorMap* ma2 = t.kind <= kGrad ? &maps.X2 : &maps.G2;
-        const CUtensorMap* mb2 = t.kind == kDw ? &maps.X2 : &maps.W2;
+        const CUtensorMap* ma = t.kind <= kGrad ? maps.X : maps.G;
+        const CUtensorMap* mb = t.kind == kDw ? maps.X : maps.W;
         const bool wide = t.bn == 256;                       // two 64-row boxes of B per SM
         const int ar = t.arow + 128 * (int)rank, br = t.brow + t.bn / 2 * (int)rank;
-        const uint32_t bytes = (uint32_t)((SPLIT ? 4 : 2) * (wide ? 4 : 3) * kBoxBytes);
+        const uint32_t bytes = (uint32_t)(2 * Cfg::kWords * (wide ? 4 : 3) * kBoxBytes);
         // coordinates of the boxes at K-block 0, and what a K-block and a box add to them
         int ax = a_mn ? ar : t.ak, ay = a_mn ? t.ak : ar, bx = b_mn ? br : t.bk, by = b_mn ? t.bk : br;
         const int akx = a_mn ? 0 : 64, aky = 64 - akx, bkx = b_mn ? 0 : 64, bky = 64 - bkx;
@@ -607,9 +616,8 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           if (elect_one()) {
             if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], bytes);
 #pragma unroll
-            for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
-              const CUtensorMap* a = h ? ma2 : ma;
-              const CUtensorMap* b = h ? mb2 : mb;
+            for (int h = 0; h < Cfg::kWords; ++h) {
+              const CUtensorMap *a = ma + h, *b = mb + h;
               const uint32_t d = dst + h * (Cfg::kA + Cfg::kB);
               tma_load_pair(d, a, ax, ay, bar);
               tma_load_pair(d + kBoxBytes, a, ax + aky, ay + akx, bar);
@@ -654,16 +662,18 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
             tc_fence_after();
             const uint32_t a0 = (smem0 + (uint32_t)(s * Cfg::kStage)) >> 4;
             const uint32_t ad = a0 | alo, bd = (a0 + (Cfg::kA >> 4)) | blo;
-            constexpr uint32_t lo = (Cfg::kA + Cfg::kB) >> 4;
+            // the words of each product, from the smallest up
+            constexpr uint32_t word = (Cfg::kA + Cfg::kB) >> 4;
+            constexpr int kTerms = SPLIT ? 6 : 1;
+            constexpr int wa[6] = {SPLIT ? 2 : 0, 0, 1, 1, 0, 0}, wb[6] = {0, 2, 1, 0, 1, 0};
             const uint32_t more = kb > k0 ? 1u : 0u;
             if (elect_one()) {
 #pragma unroll
-              for (int term = SPLIT ? 0 : 2; term < 3; ++term) {   // lo hi, hi lo, hi hi
-                const uint32_t at = ad + (term == 0 ? lo : 0u), bt = bd + (term == 1 ? lo : 0u);
+              for (int term = 0; term < kTerms; ++term) {
+                const uint32_t at = ad + wa[term] * word, bt = bd + wb[term] * word;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  mma_pair(d, at + k * as, bt + k * bs, idesc,
-                           (k > 0 || term > (SPLIT ? 0 : 2)) ? 1u : more);
+                  mma_pair(d, at + k * as, bt + k * bs, idesc, (k > 0 || term > 0) ? 1u : more);
               }
               commit_pair(&ctl->empty[s]);
               if (kb + 1 == k1) commit_pair(&ctl->acc_full[ac & 1]);
@@ -735,8 +745,12 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
     uint8_t* stage = out_stage + (warp - 4) * 4096;
     const uint32_t empty0 = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
     constexpr bool f16 = std::is_same<T, __half>::value;
-    const Scales scales(FWD && !SPLIT ? nullptr : p.amax, f16, SPLIT);
-    const float sc_s = scales.s;
+    float scale_g = 1.f, scale_back = 1.f;
+    if (!FWD) {
+      const Scales scales(p.amax, f16);
+      scale_g = scales.g;
+      scale_back = scales.back;
+    }
     float m_run = -3.402823466e38f, s_run = 0.f;            // kLse, over the unit's tiles
     int target = -1;
     constexpr int kCols = 128;                              // columns per warp
@@ -867,12 +881,6 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
 
       if (t.kind <= kGrad) {   // products -> logits
         const int v0 = (int)t.brow + col0;
-        if (SPLIT) {
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c][i] *= sc_s;
-        }
         if (p.bias) {
           const float4* b = reinterpret_cast<const float4*>(p.bias + v0);
 #pragma unroll
@@ -937,7 +945,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
 
       if (t.kind == kGrad) {
         const int v0 = (int)t.brow + col0;
-        const float ga = rg.a * scales.g, gb = rg.b * scales.g;
+        const float ga = rg.a * scale_g, gb = rg.b * scale_g;
         // (S - logZ) first, for the same reason: p stays at most one
         const F2 l2 = f2(kLog2Ef, kLog2Ef), ga2 = f2(ga, ga), off = f2(-rg.lse, -rg.lse);
 #pragma unroll
@@ -964,13 +972,31 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
             for (int i = 0; i < 32; ++i)
               if (empty || v0 + 32 * c + i >= p.V) acc[c][i] = 0.f;
         }
+        if (p.dbias_part) {
+          // column sums of the unrounded g; the four quadrants' meet in the warpgroup's
+          // stages
+          stage_free();
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = acc[c][i];
+            reinterpret_cast<float*>(stage)[32 * c + lane] = column_sums(v, lane);
+          }
+          if (!wg_sync()) { ok = false; break; }
+          const int e = (int)threadIdx.x & 127;
+          const float* cs = reinterpret_cast<const float*>(out_stage + wg * 16384) + e;
+          const float s = (cs[0] + cs[1 * 1024]) + (cs[2 * 1024] + cs[3 * 1024]);
+          p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + col0 + e] = s;
+          if (!wg_sync()) { ok = false; break; }
+        }
         // 64 columns of words at a time are a warp's stage (SPLIT: their hi words, then
-        // their lo words)
+        // their mid, then their lo words)
         const int gx = t.x1 + col0, gy = t.x0 + 128 * (int)rank + 32 * q;
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
 #pragma unroll
-          for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
+          for (int h = 0; h < Cfg::kWords; ++h) {
             stage_free();
 #pragma unroll
             for (int g = 0; g < 8; ++g) {
@@ -978,30 +1004,16 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int e = 8 * g + 2 * i;
-                const float a = acc[c + e / 32][e % 32], bb = acc[c + e / 32][e % 32 + 1];
-                w[i] = pack2<T>(a, bb);
-                if (SPLIT && h) w[i] = pack_f16(a - f16lo_f(w[i]), bb - f16hi_f(w[i]));
+                float &a = acc[c + e / 32][e % 32], &b = acc[c + e / 32][e % 32 + 1];
+                w[i] = pack2<T>(a, b);
+                if (h + 1 < Cfg::kWords) minus_word(a, b, w[i]);
               }
               *reinterpret_cast<uint4*>(stage + lane * 128 + ((g ^ (lane & 7)) << 4)) =
                   make_uint4(w[0], w[1], w[2], w[3]);
             }
             stage_full();
-            if (lane == 0) tma_store(h ? &maps.G2s : &maps.Gs, gx + 32 * c, gy, stage_at);
+            if (lane == 0) tma_store(&maps.Gs[h], gx + 32 * c, gy, stage_at);
           }
-        }
-        if (p.dbias_part) {
-          // column sums of the unrounded g; the four quadrants' meet in the warpgroup's
-          // stages
-          stage_free();
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c)
-            reinterpret_cast<float*>(stage)[32 * c + lane] = column_sums(acc[c], lane);
-          if (!wg_sync()) { ok = false; break; }
-          const int e = (int)threadIdx.x & 127;
-          const float* cs = reinterpret_cast<const float*>(out_stage + wg * 16384) + e;
-          const float s = (cs[0] + cs[1 * 1024]) + (cs[2 * 1024] + cs[3 * 1024]);
-          p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + col0 + e] = s;
-          if (!wg_sync()) { ok = false; break; }
         }
         to_report = (int)(n % kFeed);
         continue;
@@ -1011,7 +1023,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       const bool dw = t.kind == kDw, add = t.flags & 1, direct = t.flags & 2;
       const int row0 = t.x0 + 128 * (int)rank + 32 * q;
       const int slot_row = dw ? t.ks * p.piece + row0 : t.ks * (int)p.Np + row0;
-      const float so = scales.dw;
+      const float so = scale_back;
       const int rows_left = p.V - t.x1 - row0;                // kDw: rows of dW from row0
       const int g = lane & 7;                                 // direct: 8 lanes a row
       // the sums so far of a chunk's rows r = 4 i + lane / 8, written by other SMs: all in

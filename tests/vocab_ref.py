@@ -2,8 +2,8 @@
 kernels are held to (elementwise, from the arithmetic; no fitted constants).
 
 u is half a step of the element type (2^-8 bf16, 2^-11 fp16, 2^-24 fp32).  fp32
-operands run as two 11-bit fp16 words each, so a product's operands carry a
-relative error of 2^-21 together; bf16 and fp16 products are exact in fp32.
+operands run as three bf16 words each, which carry a relative error of 2^-24 per
+product together (held to 2^-21 here); bf16 and fp16 products are exact in fp32.
 
 An fp32 sum of K products on the tensor core is kept in steps of 16, each
 cutting the running sum at 2^-23 of its magnitude and the aligned products at
