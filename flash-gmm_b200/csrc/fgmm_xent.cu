@@ -117,7 +117,7 @@ struct XentWs {
   int vtiles, per_split, splits;
   int bn_d, tiles_d;
   int64_t ldS;
-  int row_chunk, piece, n_chunks, n_pieces, ks_x, ks_w;
+  int row_chunk, piece, n_chunks, n_pieces, ks_x, ks_w, parts;
   int64_t sync_words, units = 0;
   size_t bytes;
 
@@ -220,7 +220,9 @@ struct XentWs {
       sync = c.take<uint32_t>(sync_words);
       for (int h = 0; h < 3; ++h)
         G[h] = c.take<uint16_t>(h < words ? (size_t)kRing * row_chunk * piece : 0);
-      dbias_part = c.take<float>(want_bias ? (size_t)(Np / 128) * Vp : 0);
+      // one part per 128 rows of the first kRing chunks, to which the later ones add
+      parts = (int)std::min<int64_t>(n_chunks, kRing) * (row_chunk / 128);
+      dbias_part = c.take<float>(want_bias ? (size_t)parts * Vp : 0);
       dx_slots = c.take<float>((size_t)ks_x * Np * ldS);
       dw_slots = c.take<float>(n_chunks == 1 && ks_w == 1 ? 0 : (size_t)ks_w * piece * ldS);
     }
@@ -555,7 +557,7 @@ __device__ __forceinline__ void store_slots(const Share sh, const float* __restr
 __device__ __forceinline__ void store_dbias(int block, const XentArgs& a, const XentWs& w) {
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int nparts = (int)(((int64_t)w.hdr->live + kPairRows - 1) / kPairRows) * 2;
+  const int nparts = min((int)(((int64_t)w.hdr->live + kPairRows - 1) / kPairRows) * 2, w.parts);
   const int64_t v = block * 32ll + lane;      // < Vp
   float s = 0.f;
 #pragma unroll 4

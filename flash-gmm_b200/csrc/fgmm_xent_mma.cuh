@@ -73,7 +73,7 @@ struct MmaParams {
   uint32_t* sync;          // from 0: units claimed, then marks of kGrad and of the products by
                            // piece, then of each tile of dX's and of dW's slots
   const RowGrad* rg;
-  float* dbias_part;       // [2 Np / 256][Vp], or null
+  float* dbias_part;       // [2 kRing row_chunk / 256][Vp] at most, or null
   int64_t Vp;
   int ks_x, ks_w;          // splits of K
   const float* dw_slots;   // [ks_w][piece][ldS]
@@ -113,11 +113,12 @@ struct __align__(16) Tile {
   int ak, bk;           // first K of A / B
   int nkb, bn;          // K blocks, columns
   int ks;               // split of K; kLse: the unit's range of the vocabulary
-  int flags;            // kLse: 1 last, 2 first tile of its unit; products: 1 add, 2 final
+  int flags;            // kLse: 1 last, 2 first tile of its unit; kGrad: 1 add to dbias's part;
+                        // products: 1 add, 2 final
   int j;                // backward: the piece
   int x0, x1;           // kGrad: row, column of G; kDx: row of dX; kDw: row of the piece, v0
   uint32_t w0, w1;      // marks to wait for (wait_marks)
-  int cell;             // products: their tile of the slots
+  int cell;             // products: their tile of the slots; kGrad: row tile of dbias's parts
   int pad;
 };
 
@@ -268,6 +269,8 @@ struct ForwardWalk {
 // claim units in this one order, and a unit waits only for units before it in the order,
 // so whichever pairs are resident make progress.  What a unit needs of others:
 //   kGrad j       the products of piece j - kRing (the ring's buffer is free)
+//                 and, where it adds to the parts of dbias, that piece's g: chunk rc uses those
+//                 of chunk rc - kRing, which is kRing pieces back, so they do not grow with N
 //   products i    all of piece i's g, and the unit before it on the same tile of the slots
 // Each is a count of marks, one per SM that has finished its half of a unit (mark role).
 constexpr int kRing = 5;
@@ -341,11 +344,14 @@ struct BackwardList {
       t.arow = (step % chunks) * p.row_chunk + m * kPairRows; t.ak = 0;   // of Xp
       t.brow = s.v0 + vt * kBN; t.bk = 0;                                 // of W
       t.nkb = p.kbD; t.bn = kBN;
-      t.ks = 0; t.flags = 0;
+      t.ks = 0;
+      const int rc = step % chunks;
+      t.flags = rc >= kRing ? 1 : 0;
+      t.cell = (rc % kRing) * (p.row_chunk / kPairRows) + m;
       t.x0 = (step % kRing) * p.row_chunk + m * kPairRows;
       t.x1 = vt * kBN;
       t.w0 = kMarks * (uint32_t)products(step - kRing);
-      t.w1 = 0;
+      t.w1 = kMarks * (uint32_t)grads(step - kRing);
       return;
     }
     const int j = step - lag;
@@ -975,6 +981,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
         if (p.dbias_part) {
           // column sums of the unrounded g; the four quadrants' meet in the warpgroup's
           // stages
+          if (t.flags && !wait_warp(grad_marks + t.j - kRing, t.w1)) { ok = false; break; }
           stage_free();
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
@@ -987,7 +994,8 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
           const int e = (int)threadIdx.x & 127;
           const float* cs = reinterpret_cast<const float*>(out_stage + wg * 16384) + e;
           const float s = (cs[0] + cs[1 * 1024]) + (cs[2 * 1024] + cs[3 * 1024]);
-          p.dbias_part[(2 * (t.arow / kPairRows) + rank) * p.Vp + t.brow + col0 + e] = s;
+          float* part = p.dbias_part + (2 * t.cell + rank) * p.Vp + t.brow + col0 + e;
+          *part = t.flags ? __ldcg(part) + s : s;
           if (!wg_sync()) { ok = false; break; }
         }
         // 64 columns of words at a time are a warp's stage (SPLIT: their hi words, then

@@ -697,3 +697,25 @@ def test_xent_logits_far_beyond_the_exponentials_range(dtype, power, bias):
     want = G.t() @ X.detach().double()
     mag = G.abs().t() @ X.detach().double().abs()
     R.assert_within(dW[only], want[only], ((u + R.chain(N)) * mag + R.TINY[dtype])[only], "dW")
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N,V,D", [(27011, 5000, 16), (150000, 700, 8)])
+def test_xent_bias_gradient_over_many_chunks_of_rows(N, V, D, dtype):
+    """More chunks of rows than the ring has pieces: their parts of dbias add up."""
+    X, W, t, c = R.problem(N, V, D, dtype, seed=12, ignored=0.1, bias=True)
+    w = torch.rand(N, device=DEV) + 0.5
+    parts = [R.xent(X[i:i + 30000], W, t[i:i + 30000], c, w=w[i:i + 30000])
+             for i in range(0, N, 30000)]
+    want, bound = (sum(p[k] for p in parts) for k in ("dbias", "e_dbias"))
+    # the parts' own terms of the sum's length are for 30,000 rows each
+    bound = bound + 2.0 ** -24 * (N / 32 + 64) * sum(p["dbias"].abs() for p in parts)
+    for others in (False, True):
+        leaves = [X.clone().requires_grad_(others), W.clone().requires_grad_(others),
+                  c.clone().requires_grad_()]
+        loss = F.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+        wanted = [x for x in leaves if x.requires_grad]
+        got = torch.autograd.grad((loss * w).sum(), wanted, retain_graph=True)
+        R.assert_within(got[-1], want, bound, "dbias")
+        again = torch.autograd.grad((loss * w).sum(), wanted)
+        assert all(torch.equal(a, b) for a, b in zip(got, again))

@@ -167,6 +167,20 @@ def test_xent_bwd_counts_dbias_without_a_bias(lib, kind):
         assert str(with_parts) in lib.fgmm_last_error().decode()
 
 
+@pytest.mark.parametrize("kind", [0, 1, 2], ids=["fp32", "bf16", "fp16"])
+def test_bias_workspace_does_not_grow_with_the_rows(lib, kind):
+    def extra(N, V, D=64):
+        return [lib.fgmm_xent_workspace_bytes(1, kind, N, V, D, 256, D, 1, b) for b in (0, 1)]
+    for V in (1000, 5000, 131072):
+        without, given = extra(1 << 17, V)
+        # five chunks of a piece's 32 MB of words: at most this share of them a part
+        assert given - without <= 4 * V * (5 * 32 * 2 ** 20 / (128 * 2 * min(V, 4096)) + 256) + 4096
+        more, much_more = extra(1 << 22, V)
+        assert abs((much_more - more) - (given - without)) <= 4096 or V == 1000
+    without, given = extra(1 << 22, 1000)
+    assert extra(1 << 26, 1000)[1] - extra(1 << 26, 1000)[0] == given - without
+
+
 def test_no_unbounded_barrier_between_the_roles():
     """The persistent kernel's warps leave one by one after a wait that gave up, so that they
     may meet at mbarriers with bounded waits only: a hardware barrier of some of a block's
