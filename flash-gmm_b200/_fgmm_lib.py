@@ -26,6 +26,8 @@ FGMM_FLAG_FORCE_GENERAL = 2
 FGMM_X_F32 = 0
 FGMM_X_BF16 = 1
 FGMM_REDUCE = {"none": 0, "sum": 1, "mean": 2}
+FGMM_VOCAB_MAX_ROWS = 1 << 30  # N and V of the vocabulary operators stay below
+FGMM_VOCAB_MAX_D = 1 << 16
 FGMM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 _ERRORS = {1: "invalid argument", 2: "workspace", 3: "unsupported shape",

@@ -43,9 +43,13 @@ def _need_gpu(**tensors):
             raise ValueError(f"{name} is on {t.device}, the other arguments on {dev}")
 
 
+def _has_tangent(*tensors) -> bool:
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _refuse_tangents(name: str, *tensors):
     """The kernels see primal values only: a tangent would be lost without a word."""
-    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if _has_tangent(*tensors):
         raise NotImplementedError(f"{name} has no forward-mode derivative: its arguments may not "
                                   "carry tangents")
 
@@ -181,6 +185,15 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
     fn = _EmbeddingLookup.apply if _tracked(table) else L.embed_fwd
     out = fn(table, flat, float(scale), int(ignore_index))
     return out if ids.dim() == 1 else out.reshape(*ids.shape, table.shape[1])
+
+
+def lookup_takes(table: torch.Tensor) -> bool:
+    """Whether `embedding_lookup` can stand for indexing the rows of ``table`` in every
+    respect: its type and size, and no derivative (indexing has those of any order)."""
+    return (table.dim() == 2 and table.dtype in L.FGMM_TYPES
+            and 0 < table.shape[0] < L.FGMM_VOCAB_MAX_ROWS
+            and 0 < table.shape[1] <= L.FGMM_VOCAB_MAX_D
+            and not _tracked(table) and not _has_tangent(table))
 
 
 def embedding_grad(dout: torch.Tensor, ids: torch.Tensor, V: int, *, scale: float = 1.0,

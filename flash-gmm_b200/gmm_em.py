@@ -45,8 +45,8 @@ def init_params(X: torch.Tensor, K: int, covariance_type: str = "iso", seed: int
     g = torch.Generator(device="cpu")
     g.manual_seed(seed)
     idx = torch.randperm(N, generator=g)[:K].to(X.device)
-    if X.is_cuda and X.dtype in L.FGMM_TYPES and N < 2 ** 30:
-        mu = FV.embedding_lookup(X.detach(), idx).float()
+    if X.is_cuda and FV.lookup_takes(X):
+        mu = FV.embedding_lookup(X, idx).float()
     else:
         mu = X[idx].float().clone()
     dev = X.device

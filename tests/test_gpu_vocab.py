@@ -719,3 +719,28 @@ def test_xent_bias_gradient_over_many_chunks_of_rows(N, V, D, dtype):
         R.assert_within(got[-1], want, bound, "dbias")
         again = torch.autograd.grad((loss * w).sum(), wanted)
         assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_init_params_of_more_columns_than_the_lookup_takes():
+    import gmm_em
+    X = torch.randn(6, 65537, device=DEV)
+    mu, _, _ = gmm_em.init_params(X, 3, seed=1)
+    idx = torch.randperm(6, generator=torch.Generator().manual_seed(1))[:3].to(DEV)
+    assert torch.equal(mu, X[idx])
+
+
+@pytest.mark.parametrize("dtype", [FS, BF], ids=["fp32", "bf16"])
+def test_init_params_passes_derivatives_to_its_rows(dtype):
+    import gmm_em
+    X = torch.randn(50, 24, device=DEV).to(dtype).requires_grad_()
+    idx = torch.randperm(50, generator=torch.Generator().manual_seed(1))[:7].to(DEV)
+    mu, _, _ = gmm_em.init_params(X, 7, seed=1)
+    g = torch.randn(7, 24, device=DEV)
+    want = torch.zeros(50, 24, device=DEV, dtype=dtype)
+    want[idx] = g.to(dtype)
+    assert torch.equal(torch.autograd.grad(mu, X, g)[0], want)
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        tangent = torch.randn(50, 24, device=DEV).to(dtype)
+        mu, _, _ = gmm_em.init_params(fw.make_dual(X.detach(), tangent), 7, seed=1)
+        assert torch.equal(fw.unpack_dual(mu).tangent, tangent[idx].float())

@@ -72,6 +72,18 @@ def test_tangents_are_refused(name, call, grad):
         torch.func.jvp(f, (torch.zeros(40),), (torch.ones(40),))
 
 
+def test_lookup_takes():
+    assert F.lookup_takes(W) and F.lookup_takes(W.t()) and F.lookup_takes(W.half())
+    for x in (W.double(), W[0], W[:0], W[:, :0], torch.zeros(2, 65537),
+              torch.zeros(1, 1).expand(1 << 30, 1), W.clone().requires_grad_()):
+        assert not F.lookup_takes(x)
+    with torch.no_grad():
+        assert F.lookup_takes(W.clone().requires_grad_())
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        assert not F.lookup_takes(fw.make_dual(W, W))
+
+
 class C:
     """One entry's arguments by name, valid ones for pointers that are never read."""
     XENT = dict(type=1, X=256, sxn=8, sxd=1, W=256, swv=8, swd=1, bias=None, targets=256,
