@@ -223,5 +223,8 @@ def embedding_grad(dout: torch.Tensor, ids: torch.Tensor, V: int, *, scale: floa
         out = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
     elif out.shape != (V, D) or out.dtype != dout.dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous ({V}, {D}) tensor of {dout.dtype}")
-    return L.embed_bwd(dout.detach().reshape(-1, D), flat, float(scale), int(ignore_index),
-                       out.detach(), bool(accumulate))
+    got = L.embed_bwd(dout.detach().reshape(-1, D), flat, float(scale), int(ignore_index),
+                      out.detach(), bool(accumulate))
+    if not out.is_inference():   # the kernel wrote to it: autograd has to see that
+        torch.autograd.graph.increment_version(out)
+    return got

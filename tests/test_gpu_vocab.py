@@ -744,3 +744,18 @@ def test_init_params_passes_derivatives_to_its_rows(dtype):
         tangent = torch.randn(50, 24, device=DEV).to(dtype)
         mu, _, _ = gmm_em.init_params(fw.make_dual(X.detach(), tangent), 7, seed=1)
         assert torch.equal(fw.unpack_dual(mu).tangent, tangent[idx].float())
+
+
+def test_embedding_grad_into_a_buffer_is_seen_by_autograd():
+    ids, dout = torch.randint(0, 20, (30,), device=DEV), torch.randn(30, 8, device=DEV)
+    out = torch.randn(20, 8, device=DEV)
+    for accumulate in (False, True):
+        a = torch.randn(20, 8, device=DEV, requires_grad=True)
+        product = (a * out).sum()          # saves out for a's gradient
+        before = out._version
+        F.embedding_grad(dout, ids, 20, out=out, accumulate=accumulate)
+        assert out._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()
+    with torch.inference_mode():
+        F.embedding_grad(dout, ids, 20, out=torch.zeros(20, 8, device=DEV), accumulate=True)
