@@ -43,6 +43,12 @@ def _need_gpu(**tensors):
             raise ValueError(f"{name} is on {t.device}, the other arguments on {dev}")
 
 
+def _values(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t with its values in memory: the imaginary part of a conjugate holds their negatives
+    and a bit that says so, which a kernel does not see."""
+    return t.resolve_neg() if t is not None and t.is_neg() else t
+
+
 def _has_tangent(*tensors) -> bool:
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
@@ -89,8 +95,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         X, W, bias, targets, logZ, count = ctx.saved_tensors
         if dloss is None and dlogZ is None:
             return (None,) * 6
-        dloss = None if dloss is None else dloss.contiguous()
-        dlogZ = None if dlogZ is None else dlogZ.contiguous()
+        dloss = None if dloss is None else _values(dloss).contiguous()
+        dlogZ = None if dlogZ is None else _values(dlogZ).contiguous()
         grads = L.xent_bwd(X, W, targets, bias, ctx.ignore_index, logZ, dloss, count, dlogZ,
                            ctx.needs_input_grad[:3])
         return (*grads, None, None, None)
@@ -134,6 +140,7 @@ def linear_cross_entropy(X: torch.Tensor, W: torch.Tensor, targets: torch.Tensor
     _refuse_tangents("linear_cross_entropy", X, W, bias)
     labels = _labels("targets", targets)
     _need_gpu(X=X, W=W, targets=targets, bias=bias)
+    X, W, bias = _values(X), _values(W), _values(bias)
     if bias is not None:
         bias = bias.float().contiguous()
     shape = targets.shape
@@ -163,6 +170,7 @@ class _EmbeddingLookup(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         ids, = ctx.saved_tensors
+        dout = _values(dout)
         out = torch.empty(ctx.table_shape, device=dout.device, dtype=dout.dtype)
         return L.embed_bwd(dout, ids, ctx.scale, ctx.ignore_index, out, False), None, None, None
 
@@ -183,7 +191,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1
     flat = _labels("ids", ids)
     _need_gpu(table=table, ids=ids)
     fn = _EmbeddingLookup.apply if _tracked(table) else L.embed_fwd
-    out = fn(table, flat, float(scale), int(ignore_index))
+    out = fn(_values(table), flat, float(scale), int(ignore_index))
     return out if ids.dim() == 1 else out.reshape(*ids.shape, table.shape[1])
 
 
@@ -221,9 +229,10 @@ def embedding_grad(dout: torch.Tensor, ids: torch.Tensor, V: int, *, scale: floa
     _need_gpu(dout=dout, ids=ids, out=out)
     if out is None:
         out = torch.empty(V, D, device=dout.device, dtype=dout.dtype)
-    elif out.shape != (V, D) or out.dtype != dout.dtype or not out.is_contiguous():
+    elif (out.shape != (V, D) or out.dtype != dout.dtype or not out.is_contiguous()
+          or out.is_neg()):
         raise ValueError(f"out must be a contiguous ({V}, {D}) tensor of {dout.dtype}")
-    got = L.embed_bwd(dout.detach().reshape(-1, D), flat, float(scale), int(ignore_index),
+    got = L.embed_bwd(_values(dout.detach()).reshape(-1, D), flat, float(scale), int(ignore_index),
                       out.detach(), bool(accumulate))
     if not out.is_inference():   # the kernel wrote to it: autograd has to see that
         torch.autograd.graph.increment_version(out)

@@ -759,3 +759,40 @@ def test_embedding_grad_into_a_buffer_is_seen_by_autograd():
             product.backward()
     with torch.inference_mode():
         F.embedding_grad(dout, ids, 20, out=torch.zeros(20, 8, device=DEV), accumulate=True)
+
+
+def negated(x):
+    """x's values as the imaginary part of a conjugate: a view whose memory holds -x."""
+    z = torch.complex(torch.zeros_like(x), -x).conj().imag
+    assert z.is_neg() and torch.equal(z, x)
+    return z
+
+
+@pytest.mark.parametrize("N", [5, 50])
+def test_negated_views_have_their_values(N):
+    X, W, t, c = R.problem(N, 90, 24, FS, bias=True)
+    w = torch.rand(N, device=DEV) + 0.5
+
+    def grads(X, W, c, w):
+        leaves = [x.detach().requires_grad_() for x in (X, W, c)]
+        assert [x.is_neg() for x in leaves] == [x.is_neg() for x in (X, W, c)]
+        loss, logZ = F.linear_cross_entropy(*leaves[:2], t, leaves[2], reduction="none",
+                                            return_logZ=True)
+        return loss.detach(), *torch.autograd.grad((loss, logZ), leaves, (w, w))
+
+    want = grads(X, W, c, w)
+    for mask in range(1, 16):
+        args = [negated(x) if mask >> i & 1 else x for i, x in enumerate((X, W, c, w))]
+        for got, ref in zip(grads(*args), want):
+            # a W of two floats' steps is summed in another order: both within 2^-18
+            assert float((got - ref).abs().max()) <= 2.0 ** -18 * float(ref.abs().max().clamp_min(1))
+    table = W.detach()
+    assert torch.equal(F.embedding_lookup(negated(table), t), table[t])
+    dout = torch.randn(N, 24, device=DEV)
+    leaf = table.clone().requires_grad_()
+    got, = torch.autograd.grad(F.embedding_lookup(leaf, t), leaf, negated(dout))
+    assert torch.equal(got, F.embedding_grad(dout, t, 90))
+    assert torch.equal(F.embedding_grad(negated(dout), t, 90), got)
+    import gmm_em
+    mu, _, _ = gmm_em.init_params(negated(table), 5, seed=1)
+    assert torch.equal(mu, gmm_em.init_params(table, 5, seed=1)[0])
