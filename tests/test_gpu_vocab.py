@@ -796,3 +796,28 @@ def test_negated_views_have_their_values(N):
     import gmm_em
     mu, _, _ = gmm_em.init_params(negated(table), 5, seed=1)
     assert torch.equal(mu, gmm_em.init_params(table, 5, seed=1)[0])
+
+
+@pytest.mark.parametrize("dtype", [BF, FH], ids=["bf16", "fp16"])
+def test_xent_probabilities_of_the_longest_rows(dtype):
+    """D = 65536 and logits near 800, all products positive: the gradient's logits may not
+    be cut more than those of logZ."""
+    N, V, D = 70, 40, 65536
+    g = torch.Generator().manual_seed(4)
+    X = (0.5 + torch.rand(N, D, generator=g)).to(dtype).to(DEV)
+    W = (800.0 / D * (1 + 0.5 * torch.randn(V, D, generator=g)).abs()).to(dtype).to(DEV)
+    X.requires_grad_(), W.requires_grad_()
+    t = torch.zeros(N, dtype=torch.int64, device=DEV)
+    logZ = F.linear_cross_entropy(X, W, t, reduction="none", return_logZ=True)[1]
+    dX, dW = torch.autograd.grad(logZ.sum(), (X, W))
+    Xd, Wd = X.detach().double(), W.detach().double()
+    S = Xd @ Wd.t()
+    p = torch.softmax(S, 1)
+    # a group of 64 steps cuts 2^-22 of its own sum a step (8 more for joining), forward 16;
+    # the groups are added at 2^-24 of the sum so far each
+    e = S.max() * (2.0 ** -22 * (64 + 8 + 16 + 8) + 2.0 ** -24 * (D / 1024 + D / 256)) + 2.0 ** -16
+    u = R.U[dtype]
+    relative = torch.expm1(e) + 2 * u + R.chain(max(V, N))     # g's and the result's rounding
+    assert 2.0 ** -7 < float(relative) < 0.06
+    for got, want in ((dX, p @ Wd), (dW, p.t() @ Xd)):
+        R.assert_within(got, want, relative * want + R.TINY[dtype], "gradient")
