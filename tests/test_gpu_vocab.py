@@ -821,3 +821,96 @@ def test_xent_probabilities_of_the_longest_rows(dtype):
     assert 2.0 ** -7 < float(relative) < 0.06
     for got, want in ((dX, p @ Wd), (dW, p.t() @ Xd)):
         R.assert_within(got, want, relative * want + R.TINY[dtype], "gradient")
+
+
+@pytest.mark.parametrize("V", [200, 5000, 70001], ids=["1 pass", "2 passes", "3 passes"])
+@pytest.mark.parametrize("N", [16385, 65536, 65537, 131072, 131073, 300001])
+@pytest.mark.parametrize("dtype", [BF, FS], ids=["bf16", "fp32"])
+def test_embedding_of_many_ids(N, V, dtype):
+    """Each form of the sort: one cluster with 2, 8 and 16 ids a thread, and the long one."""
+    D = 11
+    g = torch.Generator().manual_seed(N + V)
+    ids = torch.where(torch.rand(N, generator=g) < 0.3, torch.randint(0, 3, (N,), generator=g),
+                      torch.randint(0, V, (N,), generator=g)).to(DEV)
+    ids[::13] = R.IGNORE
+    ids[5], ids[N - 1] = V, -1                     # outside the table
+    table = torch.randn(V, D, generator=g).to(dtype).to(DEV).requires_grad_()
+    dout = torch.randn(N, D, generator=g).to(dtype).to(DEV)
+    out = F.embedding_lookup(table, ids)
+    valid = (ids >= 0) & (ids < V)
+    assert torch.equal(out[valid].detach(), table.detach()[ids[valid]])
+    assert bool(torch.isnan(out[5]).all() & torch.isnan(out[N - 1]).all())
+    assert not out.detach()[ids == R.IGNORE].any()
+    got, = torch.autograd.grad(out, table, dout)
+    ref, bound = R.embed_grad(dout, ids, V, 1.0)
+    R.assert_within(got, ref, bound, "dtable")
+    assert torch.equal(F.embedding_grad(dout, ids, V), got)
+    # every position counted once: whole sums are exact
+    ones = F.embedding_grad(torch.ones(N, D, device=DEV), ids, V)
+    assert torch.equal(ones, torch.bincount(ids[valid], minlength=V)[:, None].float().expand(V, D))
+
+
+@pytest.mark.parametrize("dtype", [BF, FH, FS], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("N", [16384, 16385, 20480, 40001])
+def test_xent_lists_long_batches(N, dtype):
+    """Live rows counted in blocks of 4096 before they are listed, blocks without any among
+    them; each row's loss and gradient at its own place."""
+    V, D = 90, 24
+    X, W, t, c = R.problem(N, V, D, dtype, seed=N, ignored=0.4, bias=True)
+    t[4096:8192] = R.IGNORE
+    t[9000:12500] = R.IGNORE
+    X[t == R.IGNORE] = float("nan")
+    X.requires_grad_(), W.requires_grad_(), c.requires_grad_()
+    w = torch.rand(N, device=DEV) + 0.5
+    loss, logZ = F.linear_cross_entropy(X, W, t, c, reduction="none", return_logZ=True)
+    ref = R.xent(X, W, t, c, w=w)
+    R.assert_within(loss.detach(), ref["loss"], ref["e_loss"], "loss")
+    R.assert_within(logZ.detach(), ref["logZ"], ref["e_logZ"], "logZ")
+    got = torch.autograd.grad((loss * w).sum(), (X, W, c))
+    for x, name in zip(got, ("dX", "dW", "dbias")):
+        R.assert_within(x, ref[name], ref["e_" + name], name)
+    assert not got[0][t == R.IGNORE].any()
+    mean = F.linear_cross_entropy(X, W, t, c)
+    live = int((t != R.IGNORE).sum())
+    R.assert_within(mean.detach(), ref["loss"].sum() / live,
+                    (ref["e_loss"].sum() + 2 ** -23 * ref["loss"].sum()) / live, "mean")
+
+
+def test_xent_gradient_of_a_table_longer_than_32_bit_offsets():
+    """V * D > 2^31 elements in W and dW: entries at both ends and between."""
+    N, V, D = 40, 1_200_000, 2048
+    W = torch.empty(V, D, device=DEV, dtype=BF)
+    for i in range(0, V, 100_000):
+        W[i:i + 100_000] = torch.randn(1, D, device=DEV) * 0.02
+    some = torch.cat([torch.arange(5), torch.arange(600_000, 600_005), torch.arange(V - 5, V)])
+    some = some.to(DEV)
+    W[some] = (torch.randn(15, D, device=DEV) * 0.05).to(BF)
+    t = some[torch.arange(N, device=DEV) % 15]
+    X = (W[t].float() * 4 + 0.1 * torch.randn(N, D, device=DEV)).to(BF)
+    X.requires_grad_(), W.requires_grad_()
+    loss, logZ = F.linear_cross_entropy(X, W, t, reduction="none", return_logZ=True)
+    dX, dW = torch.autograd.grad(loss.sum(), (X, W))
+    Xd, lz = X.detach().double(), torch.empty(N, V, device=DEV, dtype=torch.float64)
+    for i in range(0, V, 100_000):
+        lz[:, i:i + 100_000] = Xd @ W.detach()[i:i + 100_000].double().t()
+    # all of one logit's products at once: steps of 16 that cut 2^-22 of the sum of magnitudes
+    e = float(R.chain(D) * (Xd.abs() @ W.detach()[some].double().abs().t()).max()) * 2
+    S, lz = lz, torch.logsumexp(lz, 1)
+    assert float((logZ.detach().double() - lz).abs().max()) <= e + 2.0 ** -12
+    G = torch.exp(S - lz[:, None])
+    G[torch.arange(N, device=DEV), t] -= 1.0
+    relative = math.expm1(2 * e + 2.0 ** -12) + 2.0 ** -8 + R.chain(V)
+    want = torch.zeros(N, D, device=DEV, dtype=torch.float64)
+    mag = torch.zeros_like(want)
+    for i in range(0, V, 100_000):
+        w = W.detach()[i:i + 100_000].double()
+        want += G[:, i:i + 100_000] @ w
+        mag += G[:, i:i + 100_000].abs() @ w.abs()
+    # a label's p - 1 carries p's error, not that of its difference
+    mag += W.detach()[t].double().abs()
+    R.assert_within(dX, want, relative * mag + 2.0 ** -8 * want.abs(), "dX")
+    for rows in (some, torch.tensor([99_999, 100_000, 1_048_575, 1_048_576], device=DEV)):
+        g = G[:, rows]
+        mag = (g.abs() + (t[:, None] == rows).double()).t() @ Xd.abs()
+        R.assert_within(dW[rows], g.t() @ Xd, relative * mag + 2.0 ** -8 * (g.t() @ Xd).abs()
+                        + R.TINY[BF], "dW")
