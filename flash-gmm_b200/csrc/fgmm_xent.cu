@@ -10,7 +10,7 @@
 // they hold never meets a product.  Forward, logits stay in TMEM and registers and
 // leave as a (max, sum) per row and range of the vocabulary.  Backward, they are
 // computed again in pieces; a piece's g goes to a small ring of buffers and is
-// multiplied with W and X, out of the L2, while the next pieces' are made.
+// multiplied with W and X, partly still in the L2, while the next pieces' are made.
 #include <cuda.h>
 
 #include <algorithm>
@@ -122,7 +122,7 @@ struct XentWs {
   size_t bytes;
 
   static constexpr int kPairs = 74;                        // SM pairs the plan is made for
-  static constexpr int64_t kPieceBytes = int64_t(1) << 25; // one buffer of G: kRing stay in the L2
+  static constexpr int64_t kPieceBytes = int64_t(1) << 25; // one buffer of G, of kRing
   static constexpr int kPiecesWanted = 4;   // of a short batch: products begin while g is made
   static constexpr int64_t kSlotBytes = int64_t(1) << 28;
 

@@ -48,8 +48,8 @@ constexpr int kEpiWarps = 8;
 constexpr int kMmaThreads = (4 + kEpiWarps) * 32;
 constexpr int kSplitBlocks = 1;   // K-blocks per group: 4 steps of hi hi upon small ones
 constexpr int kLogitBlocks = 4;   // 16 steps
-constexpr int kGradBlocks = 16;   // 64 steps, D = 1024: a cut of 2^-18 of the logit at any D
-                                  // (in one chain of 4096 steps, D = 65536, p came out 26% low at S = 800)
+constexpr int kGradBlocks = 16;   // 64 steps, D = 1024: a cut of 2^-18 of the logit at any D (one
+                                  // chain of 4096 steps: p 26% low at D = 65536, logits of 800)
 
 enum TileKind { kLse = 0, kGrad = 1, kDx = 2, kDw = 3 };
 
@@ -266,7 +266,8 @@ struct ForwardWalk {
 };
 
 // The backward tiles.  G runs through a ring of kRing pieces (row chunk x piece of the
-// vocabulary, the chunks of one piece of the vocabulary in a row) that stays in the L2:
+// vocabulary, the chunks of one piece of the vocabulary in a row).  It bounds the workspace
+// (kRing buffers of 32 MB, more than the 126 MB L2 holds, so part of G meets the DRAM):
 // step j makes piece j's g (kGrad) and multiplies piece j - lag's (kDx, kDw), the two
 // kinds mixed, since one is bound by its epilogue and the other by its products.  Pairs
 // claim units in this one order, and a unit waits only for units before it in the order,
@@ -604,7 +605,7 @@ xent_mma_kernel(const __grid_constant__ MmaParams p, const __grid_constant__ Mma
       bool ok = true;
       const uint32_t smem0 = smem_u32(smem), full0 = map_to_cta(smem_u32(&ctl->full[0]), 0);
       for (uint32_t n = 0; ok && (FWD ? walk.next(t) : take(n, t)); ++n) {
-        if (!FWD && t.kind >= kDx) {   // its G was written by other SMs' plain stores
+        if (!FWD && t.kind >= kDx) {   // its G was written by other SMs' bulk stores
           const bool there = wait_marks(grad_marks + t.j, t.w0, &ctl->abort_flag, err, 128);
           if (!__all_sync(0xffffffffu, there)) { ok = false; break; }
           fence_async_all();

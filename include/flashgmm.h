@@ -215,8 +215,15 @@ FGMM_API int fgmm_generate_iso_rows(float* X, const int64_t* row_ids, int64_t ro
  *  - Workspaces are 256-byte aligned, as for the E-step; nothing in them has
  *    to be initialised and nothing is kept in them between calls.  Results
  *    are bitwise reproducible run to run.
- *  - Limits: N < 2^30, V < 2^30, D <= 2^16; the gradient of the loss also
- *    about N * V < 2^46 (FGMM_ERR_UNSUPPORTED beyond).
+ *  - fp32 calls keep fp32's precision over its range, except that infinities
+ *    in X or W give NaN in batches of more than 16 rows.  In 16-bit calls a
+ *    gradient's g (below) is stored in the type; FGMM_T_F16 keeps its bits
+ *    down to 2^-26 of the call's largest row weight and an error of 2^-37 of
+ *    that weight below, so weights further apart than that belong in separate
+ *    calls, or in FGMM_T_BF16.
+ *  - Limits: N < 2^30, V < 2^30, D <= 2^16; the gradient of the loss takes
+ *    N * V up to 2^55 / max(D, 1024) at least (FGMM_ERR_UNSUPPORTED where the
+ *    units of its work pass 2^31).
  * ------------------------------------------------------------------------- */
 #define FGMM_T_F32 0
 #define FGMM_T_BF16 1

@@ -193,6 +193,18 @@ def test_bias_workspace_does_not_grow_with_the_rows(lib, kind):
     assert extra(1 << 26, 1000)[1] - extra(1 << 26, 1000)[0] == given - without
 
 
+@pytest.mark.parametrize("kind", [0, 1, 2], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("D", [1, 64, 128, 129, 1000, 1024, 1025, 4096, 8192, 16384, 65536])
+def test_xent_bwd_takes_the_stated_sizes(lib, D, kind):
+    """N V up to 2^55 / max(D, 1024) is not refused for its size (no workspace is given, which
+    is found before anything runs)."""
+    for log_v in range(8, 30, 3):
+        V = (1 << log_v) - 1
+        N = min((1 << 30) - 1, (1 << 55) // max(D, 1024) // V)
+        got = lib.fgmm_xent_bwd(*dict(C.BWD, type=kind, N=N, V=V, D=D, swv=D, sxn=D, nws=0).values())
+        assert got == 2, (N, V, lib.fgmm_last_error())
+
+
 def test_no_unbounded_barrier_between_the_roles():
     """The persistent kernel's warps leave one by one after a wait that gave up, so that they
     may meet at mbarriers with bounded waits only: a hardware barrier of some of a block's
