@@ -137,12 +137,13 @@ struct XentWs {
     pack_w = split || swd != 1 || swv < D || swv % 8 != 0 || swv >= (int64_t(1) << 38) ||
              (reinterpret_cast<uintptr_t>(W) & 15) != 0;
     hdr = c.take<Header>(1);
-    // fp32 rows of W that do not take 16-byte loads: 8 rows at most (12 of 100000 x 999: 390 us
-    // against 320 as words on the tensor cores)
+    // fp32 rows of W that do not take 16-byte loads: forward 8 rows at most (12 of 5000 x 4095:
+    // 291 us against 169 as words on the tensor cores; of 100000 x 999 393 and 405), with
+    // gradients all 16 (12 of 100000 x 999: 735 against 995, of 5000 x 4095 267 and 309).
     const bool w16 = swd == 1 && swv % 4 == 0 && D % 4 == 0 && (reinterpret_cast<uintptr_t>(W) & 15) == 0;
     // One 16-bit row whose W would be copied for TMA: 131072 x 4095 bf16 674 -> 288 us, with
     // gradients 3181 -> 1337, W transposed (100000 x 1000) 655 -> 253; four rows 676 -> 803.
-    small = split ? N <= (w16 ? kSmallRows : 8) : pack_w && N <= 1;
+    small = split ? N <= (w16 || backward ? kSmallRows : 8) : pack_w && N <= 1;
     if (small) {
       const SmallPlan sp = small_plan(N, V, D);
       if (!backward) {
